@@ -22,7 +22,10 @@ from .api import (  # noqa: F401
     chunked_forward,
     fused_gdn_gating,
     gated_rmsnorm,
+    group_norm,
     init,
+    linear_attention_chunked,
+    linear_attention_recurrent,
     recurrent_forward,
     transpose_to_mn_major,
 )

@@ -78,6 +78,28 @@ class ConvArgs(C.Structure):
                 ("channels", C.c_int32), ("width", C.c_int32), ("silu", C.c_int32)]
 
 
+class GroupNormArgs(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("z", C.c_void_p), ("y", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p),
+                ("samples", C.c_int64), ("rows", C.c_int64), ("channels", C.c_int32), ("groups", C.c_int32),
+                ("x_stride_sample", C.c_int64), ("x_stride_row", C.c_int64), ("z_stride_sample", C.c_int64),
+                ("z_stride_row", C.c_int64), ("y_stride_sample", C.c_int64), ("y_stride_row", C.c_int64),
+                ("dtype", C.c_int32), ("param_dtype", C.c_int32), ("eps", C.c_float), ("silu", C.c_int32),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class LinearRecurrentArgs(C.Structure):
+    _fields_ = [("shape", Shape), ("q", TokenTensor), ("k", TokenTensor), ("v", TokenTensor), ("out", TokenTensor),
+                ("gate", TokenScalar), ("state_in", State), ("state_out", State), ("num_accepted_tokens", C.c_void_p),
+                ("state_indices", C.c_void_p), ("num_slots", C.c_int32), ("scale", C.c_float),
+                ("store_step_state", C.c_int32), ("state_dtype", C.c_int32)]
+
+
+class LinearChunkedArgs(C.Structure):
+    _fields_ = [("shape", Shape), ("q", TokenTensor), ("k", TokenTensor), ("v", TokenTensor), ("out", TokenTensor),
+                ("gate", TokenScalar), ("initial_state", State), ("final_state", State), ("scale", C.c_float),
+                ("state_dtype", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/gdn_b200.h declares
 SYMBOLS = {
     "gdn_init": (C.c_int, [C.c_char_p, C.c_char_p]),
@@ -101,6 +123,11 @@ SYMBOLS = {
     "gdn_causal_conv1d": (C.c_int, [C.POINTER(ConvArgs), C.c_void_p]),
     "gdn_gated_rmsnorm": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int64,
                                     C.c_int64, C.c_int64, C.c_float, C.c_void_p]),
+    "gdn_group_norm_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int64, C.c_int32, C.c_int32]),
+    "gdn_group_norm": (C.c_int, [C.POINTER(GroupNormArgs), C.c_void_p]),
+    "gdn_linear_recurrent": (C.c_int, [C.POINTER(LinearRecurrentArgs), C.c_void_p]),
+    "gdn_linear_chunked_workspace_bytes": (C.c_size_t, [C.POINTER(Shape)]),
+    "gdn_linear_chunked": (C.c_int, [C.POINTER(LinearChunkedArgs), C.c_void_p]),
 }
 
 _lib = None

@@ -36,7 +36,8 @@ _state = {"library_root": None, "cuda_home": None}
 # a short prompt was several times the GPU's own time.  The ctypes bodies serve installations of the library alone
 # and the private arguments of the tests and the benchmark.
 _ext = None
-_FAST = ("_fast_recurrent_forward", "_fast_chunked_forward", "_fast_fused_gdn_gating", "_fast_causal_conv1d", "_fast_gated_rmsnorm")
+_FAST = ("_fast_recurrent_forward", "_fast_chunked_forward", "_fast_fused_gdn_gating", "_fast_causal_conv1d", "_fast_gated_rmsnorm",
+         "_fast_linear_attention_recurrent", "_fast_linear_attention_chunked", "_fast_group_norm")
 
 
 def _load_ext():
@@ -582,3 +583,205 @@ def gated_rmsnorm(x, z, weight, eps: float = 1e-6):
     cabi.check(cabi.load().gdn_gated_rmsnorm(x2.data_ptr(), z2.data_ptr(), y.data_ptr(), weight.contiguous().data_ptr(), x2.shape[0], D,
                                              x2.stride(0), z2.stride(0), y.stride(0), float(eps), _stream()), "gated_rmsnorm")
     return y.view(x.shape)
+
+
+def group_norm(x, num_groups: int, weight=None, bias=None, z=None, eps: float = 1e-5, activation: bool = True):
+    """Group norm, channels last.  x: (samples, ..., C) bf16 or fp32; the mean and variance of a sample and a group (C / num_groups
+    neighbouring channels) are those of all its rows.  weight, bias: (C), bf16 or fp32 (one dtype), or None.  Returns, in x's shape and dtype,
+    silu(u) of u = (x - mean) / sqrt(var + eps) * weight + bias (u itself without `activation`), or with a gate z shaped like x
+    u * silu(z) (u * z without `activation`).  The output norm of linear attention is one sample per token, a group per head:
+    group_norm(out.view(tokens, heads * dv), heads, weight, bias, z)."""
+    ext = _ext if _ext is not None else _load_ext()
+    if ext:
+        return ext._fast_group_norm(x, num_groups, weight, bias, z, eps, activation)
+    _require(x.is_cuda, "x must be a CUDA tensor")
+    _require(x.dim() >= 2, "x must be (samples, ..., channels)")
+    N, C_ = x.shape[0], x.shape[-1]
+    _require(num_groups > 0 and C_ > 0 and C_ % num_groups == 0, "the number of channels must be a positive multiple of num_groups")
+    _require(C_ < 1 << 31, "too many channels")
+    args = cabi.GroupNormArgs()
+    args.dtype = _dt(x)
+    for t, n in ((weight, "weight"), (bias, "bias"), (z, "z")):
+        _same_device(t, x, n)
+
+    def rows_of(t):
+        if t.stride(-1) != 1 and C_ > 1:
+            t = t.contiguous()
+        return t.unsqueeze(1) if t.dim() == 2 else t if t.dim() == 3 else t.reshape(N, x.numel() // (N * C_), C_)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.numel() == 0:
+        return y
+    xr, yr, zr = rows_of(x), rows_of(y), None
+    if z is not None:
+        _require(z.shape == x.shape and z.dtype == x.dtype, "z must have the shape and dtype of x")
+        zr = rows_of(z)
+    params = []
+    for t in (weight, bias):
+        if t is not None:
+            _require(t.dim() == 1 and t.shape[0] == C_, "weight and bias must be (channels)")
+            args.param_dtype = _dt(t)
+            t = t.contiguous()
+        params.append(t)
+    _require(weight is None or bias is None or weight.dtype == bias.dtype, "weight and bias must share a dtype")
+    args.x, args.y, args.z = xr.data_ptr(), yr.data_ptr(), None if zr is None else zr.data_ptr()
+    args.weight, args.bias = (None if t is None else t.data_ptr() for t in params)
+    args.samples, args.rows, args.channels, args.groups = N, xr.shape[1], C_, int(num_groups)
+    args.x_stride_sample, args.x_stride_row, _ = xr.stride()
+    args.y_stride_sample, args.y_stride_row, _ = yr.stride()
+    if zr is not None:
+        args.z_stride_sample, args.z_stride_row, _ = zr.stride()
+    args.eps, args.silu = float(eps), int(bool(activation))
+    lib = cabi.load()
+    with torch.cuda.device(x.device):
+        ws = torch.empty(lib.gdn_group_norm_workspace_bytes(N, args.rows, C_, args.groups), dtype=torch.uint8, device=x.device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+        cabi.check(lib.gdn_group_norm(C.byref(args), _stream()), "group_norm")
+    return y
+
+
+# --------------------------------------------------------------------------
+# linear attention with decay (not in the reference: the layer without the delta rule)
+# --------------------------------------------------------------------------
+def _same_device(t: Optional[torch.Tensor], like: torch.Tensor, name: str):
+    _require(t is None or (t.is_cuda and t.device == like.device), "%s must be a CUDA tensor on the device of the first input" % name)
+
+
+def _linear_ready(t: torch.Tensor, dim: int) -> torch.Tensor:
+    """What the kernels read 16 bytes at a time: a contiguous head dim, aligned, no broadcast axis.  Any other view is compacted."""
+    t = _pad_last(t, dim)
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and (t.shape[-2] <= 1 or t.stride(-2) >= dim)
+    ok = ok and all(n <= 1 or (st > 0 and st % 8 == 0) for n, st in zip(t.shape[:-1], t.stride()[:-1]))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)  # (contiguous() would return an unaligned tensor as it is)
+
+
+def _strides(t: torch.Tensor, *axes):
+    return [0 if t.shape[i] <= 1 else t.stride(i) for i in axes]  # (an axis of one may have any stride)
+
+
+def _linear_tokens(t: torch.Tensor, varlen: bool) -> cabi.TokenTensor:
+    return cabi.TokenTensor(t.data_ptr(), *([0] + _strides(t, 0, 1) if varlen else _strides(t, 0, 1, 2)))
+
+
+def _linear_inputs(query, key, value, gate, initial_state, cu_seqlens, pool, in_place):
+    """The checks that both forms share -> (shape, q, k, v, gate descriptor, state, state dtype, sequences)."""
+    for t, n in ((query, "query"), (key, "key"), (value, "value")):
+        _cuda_bf16(t, n)
+    for t, n in ((key, "key"), (value, "value"), (gate, "gate"), (initial_state, "initial_state"), (cu_seqlens, "cu_seqlens")):
+        _same_device(t, query, n)
+    varlen = cu_seqlens is not None
+    _require(query.dim() == (3 if varlen else 4), "packed tensors are rank 3 (tokens, heads, dim)" if varlen
+             else "padded tensors are rank 4 (batch, tokens, heads, dim)")
+    _require(key.shape == query.shape, "query and key must have the same shape")
+    _require(value.dim() == query.dim() and value.shape[:-2] == query.shape[:-2], "value must have the batch and token axes of query")
+    dk, (vh, dv) = query.shape[-1], value.shape[-2:]
+    _require(0 < dk <= 256 and 0 < dv <= 256, "linear attention supports head dims from 1 to 256")
+    _require(query.shape[-2] > 0 and vh > 0 and vh % query.shape[-2] == 0,
+             "the number of v-heads must be a positive multiple of that of k-heads")
+    _require(not varlen or (cu_seqlens.dim() == 1 and cu_seqlens.numel() >= 1), "cu_seqlens holds one entry more than there are sequences")
+    seqs = cu_seqlens.numel() - 1 if varlen else query.shape[0]
+    dk_al, dv_al = (dk + 7) // 8 * 8, (dv + 7) // 8 * 8
+    s_in, state_dtype = initial_state, torch.bfloat16
+    if s_in is not None:
+        _require(s_in.dtype in (torch.bfloat16, torch.float32), "initial_state must be bf16 or fp32")
+        _require(s_in.dim() == 4 and (pool or s_in.shape[0] == seqs) and tuple(s_in.shape[1:]) == (vh, dv, dk),
+                 "initial_state must be a pool (slots, v-heads, dv, dk)" if pool else "initial_state must be (sequences, v-heads, dv, dk)")
+        state_dtype = s_in.dtype
+        if (dk, dv) != (dk_al, dv_al):
+            s_in = torch.nn.functional.pad(s_in, (0, dk_al - dk, 0, dv_al - dv))
+        if not (s_in.stride(-1) == 1 and s_in.stride(-2) == dk_al and s_in.data_ptr() % 16 == 0 and all(st % 8 == 0 for st in _strides(s_in, 0, 1))):
+            s_in = s_in.clone(memory_format=torch.contiguous_format)
+        if in_place:  # a padded or compacted copy would never reach the caller's tensor
+            _require(s_in.data_ptr() == initial_state.data_ptr() and (s_in.shape[0] <= 1 or s_in.stride(0) > 0) and (vh <= 1 or s_in.stride(1) > 0),
+                     "inplace_state / state_indices need head dims that are multiples of 8 and aligned, contiguous (dv, dk) blocks")
+    _require(not in_place or s_in is not None, "inplace_state / state_indices need an initial_state")
+    q, k, v = _linear_ready(query, dk_al), _linear_ready(key, dk_al), _linear_ready(value, dv_al)
+    total = q.shape[0] if varlen else q.shape[0] * q.shape[1]
+    shape = _shape(seqs, 0 if varlen else q.shape[1], total, q.shape[-2], vh, dk_al, dv_al, cu_seqlens)
+    if gate is None:
+        g = cabi.TokenScalar(None, 0, 0, 0, 0)
+    elif gate.dim() == 1:
+        _require(gate.shape[0] == vh, "gate must be (v-heads), (batch, tokens, v-heads) or packed (tokens, v-heads)")
+        g = cabi.TokenScalar(gate.data_ptr(), _dt(gate), 0, 0, gate.stride(0))
+    else:
+        _require(gate.shape == value.shape[:-1], "gate must be (v-heads), (batch, tokens, v-heads) or packed (tokens, v-heads)")
+        g = cabi.TokenScalar(gate.data_ptr(), _dt(gate), *([0] * varlen), *gate.stride())
+    return shape, q, k, v, g, s_in, state_dtype, seqs
+
+
+def _linear_state(t: torch.Tensor) -> cabi.State:
+    return cabi.State(t.data_ptr(), *_strides(t, 0, 1))
+
+
+def linear_attention_recurrent(query, key, value, initial_state=None, gate=None, cu_seqlens=None, num_accepted_tokens=None,
+                               inference_mode: int = 0, scale: Optional[float] = None, *, inplace_state: bool = False,
+                               state_indices=None):
+    """Linear attention with decay, token by token (decode, draft runs, short prompts): per token and v-head
+        S <- exp(gate) S + v k^T ,   o = scale S q .
+
+    query/key (B,T,kh,dk) or packed (N,kh,dk) with cu_seqlens, value (B,T,vh,dv) / (N,vh,dv), bf16, head dims up to 256; `gate` holds log-decays
+    (<= 0; -inf forgets all before the token), bf16 or fp32: (vh), one per head, or (B,T,vh) / (N,vh), one per token and head; None: no decay.  The state is (sequences,vh,dv,dk), bf16
+    or fp32 as `initial_state` is (bf16 without one), and is computed with in fp32.  Returns (output, new_state), with a state per token when
+    inference_mode == SpecVerify.  num_accepted_tokens, inplace_state and state_indices are those of recurrent_forward: outputs past a
+    sequence's cap, of a padding sequence or behind the last packed one are not written.  A slot outside the pool is a padding sequence; the
+    slots of a call must differ.  No gradients."""
+    ext = _ext if _ext is not None else _load_ext()
+    if ext:
+        return ext._fast_linear_attention_recurrent(query, key, value, initial_state, gate, cu_seqlens, num_accepted_tokens,
+                                                    inference_mode, scale, inplace_state, state_indices)
+    pool, steps = state_indices is not None, int(inference_mode) == int(InferenceMode.SpecVerify)
+    in_place = inplace_state or pool
+    _require(not (steps and in_place), "per-token states cannot be combined with inplace_state or state_indices")
+    shape, q, k, v, g, s_in, state_dtype, seqs = _linear_inputs(query, key, value, gate, initial_state, cu_seqlens, pool, in_place)
+    _same_device(num_accepted_tokens, query, "num_accepted_tokens")
+    _same_device(state_indices, query, "state_indices")
+    _require(not pool or state_indices.numel() == seqs, "state_indices needs one entry per sequence")
+    _require(num_accepted_tokens is None or num_accepted_tokens.numel() == seqs, "num_accepted_tokens needs one entry per sequence")
+    varlen, (vh, dv), dk = cu_seqlens is not None, v.shape[-2:], q.shape[-1]
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    if steps:
+        s_out = torch.empty(*v.shape[:-2], vh, dv, dk, dtype=state_dtype, device=v.device)
+        so = cabi.State(s_out.data_ptr(), vh * dv * dk, dv * dk)
+    else:
+        s_out = s_in if in_place else torch.empty(seqs, vh, dv, dk, dtype=state_dtype, device=v.device)
+        so = _linear_state(s_out)
+    args = cabi.LinearRecurrentArgs(shape, _linear_tokens(q, varlen), _linear_tokens(k, varlen), _linear_tokens(v, varlen),
+                                    _linear_tokens(out, varlen), g, cabi.State(None, 0, 0) if s_in is None else _linear_state(s_in), so,
+                                    _i32(num_accepted_tokens, "num_accepted_tokens"), _i32(state_indices, "state_indices"),
+                                    s_in.shape[0] if pool else 0, float(1.0 / math.sqrt(query.shape[-1]) if scale is None else scale),
+                                    int(steps), cabi.GDN_F32 if state_dtype == torch.float32 else cabi.GDN_BF16)
+    if seqs == 0 or (not varlen and v.shape[1] == 0):
+        if not steps and not in_place:
+            s_out.zero_() if s_in is None else s_out.copy_(s_in)
+    else:
+        with torch.cuda.device(query.device):
+            cabi.check(cabi.load().gdn_linear_recurrent(C.byref(args), _stream()), "linear_attention_recurrent")
+    return out[..., :value.shape[-1]], initial_state if in_place else s_out[..., :value.shape[-1], :query.shape[-1]]
+
+
+def linear_attention_chunked(query, key, value, gate=None, scale: Optional[float] = None, initial_state=None, cu_seqlens=None):
+    """Linear attention with decay over whole prompts: what linear_attention_recurrent computes, 64 tokens at a time.
+
+    The arguments are those of linear_attention_recurrent (packed inputs need cu_seqlens alone).  Returns (output, final_state), the
+    final state in initial_state's dtype (bf16 without one).  Matrix products take bf16 operands: scores with their decay and the
+    state a chunk reads are rounded to bf16 there, the state itself is kept in fp32 throughout.  A NaN or an infinity in `value` reaches
+    all tokens of its 64-token chunk.  No gradients."""
+    ext = _ext if _ext is not None else _load_ext()
+    if ext:
+        return ext._fast_linear_attention_chunked(query, key, value, gate, scale, initial_state, cu_seqlens)
+    shape, q, k, v, g, s_in, state_dtype, seqs = _linear_inputs(query, key, value, gate, initial_state, cu_seqlens, False, False)
+    varlen, (vh, dv), dk = cu_seqlens is not None, v.shape[-2:], q.shape[-1]
+    out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+    final = torch.empty(seqs, vh, dv, dk, dtype=state_dtype, device=v.device)
+    if seqs == 0 or (not varlen and v.shape[1] == 0):
+        final.zero_() if s_in is None else final.copy_(s_in)
+    else:
+        lib = cabi.load()
+        args = cabi.LinearChunkedArgs(shape, _linear_tokens(q, varlen), _linear_tokens(k, varlen), _linear_tokens(v, varlen),
+                                      _linear_tokens(out, varlen), g, cabi.State(None, 0, 0) if s_in is None else _linear_state(s_in),
+                                      _linear_state(final), float(1.0 / math.sqrt(query.shape[-1]) if scale is None else scale),
+                                      cabi.GDN_F32 if state_dtype == torch.float32 else cabi.GDN_BF16, None, 0)
+        with torch.cuda.device(query.device):
+            ws = torch.empty(lib.gdn_linear_chunked_workspace_bytes(C.byref(shape)), dtype=torch.uint8, device=query.device)
+            args.workspace, args.workspace_bytes = ws.data_ptr(), ws.numel()
+            cabi.check(lib.gdn_linear_chunked(C.byref(args), _stream()), "linear_attention_chunked")
+    return out[..., :value.shape[-1]], final[..., :value.shape[-1], :query.shape[-1]]

@@ -17,7 +17,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIBDIR = os.path.join(PKG, "lib")
 OBJDIR = os.path.join(PKG, "build")
 LIB = os.path.join(LIBDIR, "libgdn_b200.so")
-SOURCES = ["gdn_b200.cu", "gdn_prefill.cu", "gdn_jit.cu"]
+SOURCES = ["gdn_b200.cu", "gdn_prefill.cu", "gdn_jit.cu", "gdn_linear.cu", "gdn_norm.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-std=c++17", "-lineinfo",
               "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC"]
 

@@ -77,23 +77,6 @@ __global__ void gdn_selftest_wait_kernel(long long limit_cycles, int* status) {
 }
 
 // ------------------------------------------------------------------ recurrent
-// Launch with programmatic stream serialization: the kernel's CTAs may be placed while the preceding work in the
-// stream drains; every kernel launched this way waits (griddepcontrol.wait) before its first global access.
-template <typename P>
-static cudaError_t launch_dependent(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t st, const P& params) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, params);
-}
-
 template <int DK, bool kRing, bool kLean = false, bool kF32 = false, bool kSplit = false, bool kPool = false>
 static int launch_recurrent_t(const RecurrentParams& p, int sms, cudaStream_t st) {
     constexpr int smem = recurrent_smem_bytes<DK, kRing, kF32>();

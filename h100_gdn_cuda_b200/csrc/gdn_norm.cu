@@ -1,0 +1,132 @@
+// C-ABI entry point of the channels-last group norm (see include/gdn_b200.h).
+#include "host_common.hpp"
+#include "kernels/group_norm.cuh"
+
+using namespace gdn;
+
+namespace {
+
+// How a long sample is cut: channels of a block (whole groups), rows of a part.
+struct NormPlan {
+    int block_channels, blocks, part_rows, parts;
+};
+
+NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int vec) {
+    const int width = channels / groups;
+    NormPlan plan;
+    int unit = 1;  // groups of a block come in multiples that are whole vectors
+    while (unit * width % vec != 0) ++unit;
+    int per = std::max(unit, 256 * vec / width / unit * unit);
+    per = std::min(per, kNormMaxGroups / unit * unit);
+    plan.block_channels = std::min(per * width, channels);
+    plan.blocks = (channels + plan.block_channels - 1) / plan.block_channels;
+    const int64_t want = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, samples * plan.blocks));
+    plan.part_rows = static_cast<int>(std::max<int64_t>(16, (rows + want - 1) / want));
+    plan.parts = static_cast<int>((rows + plan.part_rows - 1) / plan.part_rows);
+    return plan;
+}
+
+constexpr int kShortValues = 1024;  // values of a (sample, group) that stay in the registers of a warp
+bool short_groups(int64_t rows, int width) { return rows * width <= kShortValues; }
+
+template <typename T, int V>
+int launch_short(const GroupNormParams& p, cudaStream_t st) {
+    const long long size = p.l * p.width;
+    int lpr = 4;
+    while (lpr < 32 && lpr * V < size) lpr *= 2;
+    const int passes = static_cast<int>((size + lpr * V - 1) / (lpr * V));
+    const long long per_block = 8ll * (32 / lpr), blocks = (p.n * p.groups + per_block - 1) / per_block;
+    GDN_REQUIRE(blocks < (1ll << 31), "gdn_group_norm: too many samples");
+    auto launch = [&](auto kernel) { return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, p); };
+    if (lpr == 4) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 4, 1>));
+    else if (lpr == 8) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 8, 1>));
+    else if (lpr == 16) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 16, 1>));
+    else if (passes <= 1) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 1>));
+    else if (passes <= 2) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 2>));
+    else if (passes <= 4) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 4>));
+    else if (passes <= 8) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 8>));
+    else GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 32>));
+    return GDN_OK;
+}
+
+template <typename T, int V>
+int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
+    p.part_rows = plan.part_rows;
+    p.parts = plan.parts;
+    p.block_channels = plan.block_channels;
+    GDN_REQUIRE(p.n <= 65535 && plan.blocks <= 65535, "gdn_group_norm: too many samples or channels for one launch");
+    const dim3 grid(static_cast<unsigned>(plan.parts), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
+    GDN_CUDA(launch_dependent(gdn_group_norm_stats_kernel<T, V>, grid, kNormThreads, 0, st, p));
+    GDN_CUDA(launch_dependent(gdn_group_norm_apply_kernel<T, V>, grid, kNormThreads, 0, st, p));
+    return GDN_OK;
+}
+
+template <typename T, int V>
+int launch_norm(const GroupNormParams& p, bool is_short, const GdnGroupNormArgs& a, cudaStream_t st) {
+    if (is_short) return launch_short<T, V>(p, st);
+    return launch_long<T, V>(p, norm_plan(a.samples, a.rows, a.channels, a.groups, V), st);
+}
+
+}  // namespace
+
+extern "C" {
+
+// An upper bound over the vector widths, which go by pointers and strides.
+size_t gdn_group_norm_workspace_bytes(int64_t samples, int64_t rows, int32_t channels, int32_t groups) {
+    if (samples <= 0 || rows <= 0 || groups <= 0 || channels <= 0 || channels % groups != 0 || short_groups(rows, channels / groups)) return 0;
+    size_t parts = 0;
+    for (int v = 1; v <= 8; v *= 2)
+        if (channels % v == 0) parts = std::max<size_t>(parts, norm_plan(samples, rows, channels, groups, v).parts);
+    return parts * static_cast<size_t>(samples) * groups * sizeof(float2);
+}
+
+int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
+    GDN_REQUIRE(a != nullptr, "gdn_group_norm: args is NULL");
+    GDN_REQUIRE(a->samples >= 0 && a->rows >= 0 && a->channels > 0 && a->groups > 0 && a->channels % a->groups == 0,
+                "gdn_group_norm: channels (%d) must be a positive multiple of groups (%d)", a->channels, a->groups);
+    GDN_REQUIRE(a->dtype == GDN_BF16 || a->dtype == GDN_F32, "gdn_group_norm: dtype must be bf16 or f32");
+    GDN_REQUIRE(a->param_dtype == GDN_BF16 || a->param_dtype == GDN_F32, "gdn_group_norm: param_dtype must be bf16 or f32");
+    DeviceInfo* d = nullptr;
+    if (int rc = get_device_info(&d)) return rc;
+    if (a->samples == 0 || a->rows == 0) return GDN_OK;
+    GDN_REQUIRE(a->x && a->y, "gdn_group_norm: x and y are required");
+    GroupNormParams p{};
+    p.x = a->x; p.z = a->z; p.y = a->y; p.weight = a->weight; p.bias = a->bias;
+    p.param_f32 = a->param_dtype == GDN_F32;
+    p.n = a->samples; p.l = a->rows;
+    p.channels = a->channels; p.groups = a->groups; p.width = a->channels / a->groups;
+    p.x_sn = a->x_stride_sample; p.x_sl = a->x_stride_row;
+    p.z_sn = a->z_stride_sample; p.z_sl = a->z_stride_row;
+    p.y_sn = a->y_stride_sample; p.y_sl = a->y_stride_row;
+    p.eps = a->eps; p.silu = a->silu != 0;
+    const bool is_short = short_groups(a->rows, p.width);
+    if (!is_short) {
+        const size_t need = gdn_group_norm_workspace_bytes(a->samples, a->rows, a->channels, a->groups);
+        if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+            return fail(GDN_ERR_WORKSPACE, "gdn_group_norm: workspace of %zu bytes (16-byte aligned) required, got %zu", need, a->workspace_bytes);
+        p.partial = static_cast<float2*>(a->workspace);
+    }
+    // the widest access, up to 16 bytes, that pointers, strides and (where lanes share a group) the group's width allow
+    const int size = a->dtype == GDN_F32 ? 4 : 2;
+    auto fits = [&](int v) {
+        auto whole = [&](const void* ptr, int64_t sn, int64_t sl) {
+            return reinterpret_cast<uintptr_t>(ptr) % (static_cast<unsigned>(v * size)) == 0 && (a->samples == 1 || sn % v == 0) && (a->rows == 1 || sl % v == 0);
+        };
+        return (is_short ? p.width : p.channels) % v == 0 && whole(p.x, p.x_sn, p.x_sl) && whole(p.y, p.y_sn, p.y_sl) &&
+               (!p.z || whole(p.z, p.z_sn, p.z_sl));
+    };
+    int v = 16 / size;
+    while (!fits(v)) v /= 2;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->dtype == GDN_F32) {
+        if (v == 4) return launch_norm<float, 4>(p, is_short, *a, st);
+        if (v == 2) return launch_norm<float, 2>(p, is_short, *a, st);
+        return launch_norm<float, 1>(p, is_short, *a, st);
+    }
+    if (v == 8) return launch_norm<__nv_bfloat16, 8>(p, is_short, *a, st);
+    if (v == 4) return launch_norm<__nv_bfloat16, 4>(p, is_short, *a, st);
+    if (v == 2) return launch_norm<__nv_bfloat16, 2>(p, is_short, *a, st);
+    return launch_norm<__nv_bfloat16, 1>(p, is_short, *a, st);
+}
+
+}  // extern "C"

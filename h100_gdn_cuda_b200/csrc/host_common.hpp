@@ -82,4 +82,21 @@ inline int check_token_tensor(const GdnTokenTensor& t, const char* name, int hea
     return GDN_OK;
 }
 
+// Launch with programmatic stream serialization: the kernel's CTAs may be placed while the preceding work in the
+// stream drains; every kernel launched this way waits (griddepcontrol.wait) before its first global access.
+template <typename P>
+cudaError_t launch_dependent(void (*kernel)(P), dim3 grid, int threads, size_t smem, cudaStream_t st, const P& params) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
 }  // namespace gdn

@@ -163,10 +163,56 @@ PyObject* gated_rmsnorm(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// query, key, value, initial_state, gate, cu_seqlens, num_accepted_tokens, inference_mode, scale, inplace_state, state_indices
+PyObject* linear_attention_recurrent(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    require(n == 11, "linear_attention_recurrent takes 11 positional arguments");
+    at::Tensor q = tensor(a[0], "query"), k = tensor(a[1], "key"), v = tensor(a[2], "value");
+    auto state = optional_tensor(a[3], "initial_state"), gate = optional_tensor(a[4], "gate");
+    auto cu = optional_tensor(a[5], "cu_seqlens"), accepted = optional_tensor(a[6], "num_accepted_tokens");
+    const auto mode = static_cast<gdn_cuda::InferenceMode>(integer(a[7]));
+    const auto scale = optional_real(a[8]);
+    gdn_cuda::RecurrentExtensions ext;
+    ext.inplace_state = truth(a[9]);
+    ext.state_indices = optional_tensor(a[10], "state_indices");
+    OnDevice dev(q, "query");
+    const auto r = unlocked([&] { return gdn_cuda::linear_attention_recurrent(q, k, v, state, gate, cu, accepted, mode, dev.stream(), scale, ext); });
+    return pair(r.first, r.second);
+    END_HANDLE_TH_ERRORS
+}
+
+// query, key, value, gate, scale, initial_state, cu_seqlens
+PyObject* linear_attention_chunked(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    require(n == 7, "linear_attention_chunked takes 7 positional arguments");
+    at::Tensor q = tensor(a[0], "query"), k = tensor(a[1], "key"), v = tensor(a[2], "value");
+    auto gate = optional_tensor(a[3], "gate"), state = optional_tensor(a[5], "initial_state"), cu = optional_tensor(a[6], "cu_seqlens");
+    const auto scale = optional_real(a[4]);
+    OnDevice dev(q, "query");
+    const auto r = unlocked([&] { return gdn_cuda::linear_attention_chunked(q, k, v, gate, scale, state, cu, dev.stream()); });
+    return pair(r.first, r.second);
+    END_HANDLE_TH_ERRORS
+}
+
+// x, num_groups, weight, bias, z, eps, activation
+PyObject* group_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    require(n == 7, "group_norm takes 7 positional arguments");
+    at::Tensor x = tensor(a[0], "x");
+    const long groups = integer(a[1]);
+    auto w = optional_tensor(a[2], "weight"), b = optional_tensor(a[3], "bias"), z = optional_tensor(a[4], "z");
+    const float eps = static_cast<float>(real(a[5]));
+    const bool activation = truth(a[6]);
+    OnDevice dev(x, "x");
+    return THPVariable_Wrap(unlocked([&] { return gdn_cuda::group_norm(x, groups, w, b, z, eps, activation, dev.stream()); }));
+    END_HANDLE_TH_ERRORS
+}
+
 #define GDN_FAST(name) \
     { "_fast_" #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(&name)), METH_FASTCALL, "positional form of " #name }
 PyMethodDef kMethods[] = {GDN_FAST(recurrent_forward), GDN_FAST(chunked_forward), GDN_FAST(fused_gdn_gating),
-                          GDN_FAST(causal_conv1d),     GDN_FAST(gated_rmsnorm),   {nullptr, nullptr, 0, nullptr}};
+                          GDN_FAST(causal_conv1d),     GDN_FAST(gated_rmsnorm),   GDN_FAST(linear_attention_recurrent),
+                          GDN_FAST(linear_attention_chunked), GDN_FAST(group_norm), {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
 

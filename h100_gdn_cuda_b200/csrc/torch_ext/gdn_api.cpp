@@ -406,6 +406,237 @@ at::Tensor gated_rmsnorm(at::Tensor& x, at::Tensor& z, at::Tensor& weight, float
     return y;
 }
 
+namespace {
+// ---------------------------------------------------------------- linear attention with decay, group norm
+int64_t align8(int64_t d) { return (d + 7) / 8 * 8; }
+void on_device(const std::optional<at::Tensor>& t, const at::Tensor& like, const char* name) {
+    require(!t.has_value() || (t->is_cuda() && t->device() == like.device()), name, " must be a CUDA tensor on the device of the first input");
+}
+// What the kernels copy and read 16 bytes at a time: a contiguous head dim, aligned, no broadcast axis.  Any other view is compacted.
+at::Tensor linear_ready(const at::Tensor& t, int64_t dim) {
+    const at::Tensor p = pad_last(t, dim);
+    bool ok = p.stride(-1) == 1 && reinterpret_cast<uintptr_t>(p.data_ptr()) % 16 == 0;
+    for (int64_t i = 0; ok && i + 1 < p.dim(); ++i) ok = p.size(i) <= 1 || (p.stride(i) > 0 && p.stride(i) % 8 == 0);
+    ok = ok && (p.size(-2) <= 1 || p.stride(-2) >= dim);
+    return ok ? p : p.clone(at::MemoryFormat::Contiguous);  // (contiguous() would return an unaligned tensor as it is)
+}
+int64_t stride_of(const at::Tensor& t, int64_t i) { return t.size(i) <= 1 ? 0 : t.stride(i); }  // (an axis of one may have any stride)
+GdnTokenTensor linear_tok(const at::Tensor& t, bool packed) {
+    return packed ? GdnTokenTensor{t.data_ptr(), 0, stride_of(t, 0), stride_of(t, 1)}
+                  : GdnTokenTensor{t.data_ptr(), stride_of(t, 0), stride_of(t, 1), stride_of(t, 2)};
+}
+// (vh): one decay per head; otherwise one per token and head
+GdnTokenScalar linear_gate(const std::optional<at::Tensor>& gate, const at::Tensor& v, bool packed) {
+    if (!gate.has_value()) return GdnTokenScalar{nullptr, 0, 0, 0, 0};
+    const at::Tensor& g = *gate;
+    if (g.dim() == 1) {
+        require(g.size(0) == v.size(-2), "gate must be (v-heads), (batch, tokens, v-heads) or packed (tokens, v-heads)");
+        return GdnTokenScalar{g.data_ptr(), dtype_tag(g), 0, 0, g.stride(0)};
+    }
+    require(g.sizes() == v.sizes().slice(0, v.dim() - 1), "gate must be (v-heads), (batch, tokens, v-heads) or packed (tokens, v-heads)");
+    if (packed) return GdnTokenScalar{g.data_ptr(), dtype_tag(g), 0, g.stride(0), g.stride(1)};
+    return GdnTokenScalar{g.data_ptr(), dtype_tag(g), g.stride(0), g.stride(1), g.stride(2)};
+}
+// The inputs that both forms share, checked and ready for the library.
+struct LinearInputs {
+    bool packed;
+    int64_t dk, dv, dk_al, dv_al, seqs, vh;
+    at::Tensor q, k, v;
+    std::optional<at::Tensor> s_in;
+    at::ScalarType state_type = at::kBFloat16;
+    GdnShape shape;
+    LinearInputs(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const std::optional<at::Tensor>& gate,
+                 const std::optional<at::Tensor>& initial_state, const std::optional<at::Tensor>& cu_seqlens, bool pool, bool in_place) {
+        cuda_bf16(query, "query");
+        cuda_bf16(key, "key");
+        cuda_bf16(value, "value");
+        on_device(key, query, "key");
+        on_device(value, query, "value");
+        on_device(gate, query, "gate");
+        on_device(initial_state, query, "initial_state");
+        on_device(cu_seqlens, query, "cu_seqlens");
+        packed = cu_seqlens.has_value();
+        require(query.dim() == (packed ? 3 : 4), packed ? "packed tensors are rank 3 (tokens, heads, dim)" : "padded tensors are rank 4 (batch, tokens, heads, dim)");
+        require(key.sizes() == query.sizes(), "query and key must have the same shape");
+        require(value.dim() == query.dim() && value.sizes().slice(0, value.dim() - 2) == query.sizes().slice(0, query.dim() - 2),
+                "value must have the batch and token axes of query");
+        dk = query.size(-1);
+        dv = value.size(-1);
+        vh = value.size(-2);
+        require(dk > 0 && dk <= 256 && dv > 0 && dv <= 256, "linear attention supports head dims from 1 to 256");
+        require(query.size(-2) > 0 && vh > 0 && vh % query.size(-2) == 0, "the number of v-heads must be a positive multiple of that of k-heads");
+        require(!packed || (cu_seqlens->dim() == 1 && cu_seqlens->numel() >= 1), "cu_seqlens holds one entry more than there are sequences");
+        seqs = packed ? cu_seqlens->numel() - 1 : query.size(0);
+        dk_al = align8(dk);
+        dv_al = align8(dv);
+        if (initial_state.has_value()) {
+            const at::Tensor& s0 = *initial_state;
+            require(s0.scalar_type() == at::kBFloat16 || s0.scalar_type() == at::kFloat, "initial_state must be bf16 or fp32");
+            require(s0.dim() == 4 && (pool || s0.size(0) == seqs) && s0.size(1) == vh && s0.size(2) == dv && s0.size(3) == dk,
+                    pool ? "initial_state must be a pool (slots, v-heads, dv, dk)" : "initial_state must be (sequences, v-heads, dv, dk)");
+            state_type = s0.scalar_type();
+            at::Tensor t = pad_state(s0, dv_al, dk_al);
+            const bool ok = t.stride(-1) == 1 && t.stride(-2) == dk_al && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                            (t.size(0) <= 1 || t.stride(0) % 8 == 0) && (t.size(1) <= 1 || t.stride(1) % 8 == 0);
+            if (!ok) t = t.clone(at::MemoryFormat::Contiguous);
+            if (in_place) {  // a padded or compacted copy would never reach the caller's tensor
+                require(t.data_ptr() == s0.data_ptr() && (t.size(0) <= 1 || t.stride(0) > 0) && (vh <= 1 || t.stride(1) > 0),
+                        "inplace_state / state_indices need head dims that are multiples of 8 and aligned, contiguous (dv, dk) blocks");
+            }
+            s_in = t;
+        }
+        require(!in_place || s_in.has_value(), "inplace_state / state_indices need an initial_state");
+        q = linear_ready(query, dk_al);
+        k = linear_ready(key, dk_al);
+        v = linear_ready(value, dv_al);
+        shape = make_shape(q, v, cu_seqlens, std::nullopt, std::nullopt, 0);
+    }
+    GdnState state(const at::Tensor& t) const { return GdnState{t.data_ptr(), stride_of(t, 0), stride_of(t, 1)}; }
+    bool empty_call() const { return seqs == 0 || (!packed && v.size(1) == 0); }  // no sequences, or padded ones of no tokens
+    at::Tensor crop_out(const at::Tensor& o) const { return dv == dv_al ? o : o.narrow(-1, 0, dv); }
+    at::Tensor crop_state(const at::Tensor& s) const { return dk == dk_al && dv == dv_al ? s : s.narrow(-1, 0, dk).narrow(-2, 0, dv); }
+};
+}  // namespace
+
+std::pair<at::Tensor, at::Tensor> linear_attention_recurrent(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                                                             const std::optional<at::Tensor>& initial_state, const std::optional<at::Tensor>& gate,
+                                                             const std::optional<at::Tensor>& cu_seqlens,
+                                                             const std::optional<at::Tensor>& num_accepted_tokens, InferenceMode inference_mode,
+                                                             cudaStream_t stream, std::optional<float> scale, const RecurrentExtensions& ext) {
+    const bool pool = ext.state_indices.has_value(), in_place = ext.inplace_state || pool;
+    const bool steps = inference_mode == InferenceMode::SpecVerify;
+    require(!(steps && in_place), "per-token states cannot be combined with inplace_state or state_indices");
+    LinearInputs in(query, key, value, gate, initial_state, cu_seqlens, pool, in_place);
+    on_device(num_accepted_tokens, query, "num_accepted_tokens");
+    on_device(ext.state_indices, query, "state_indices");
+    require(!pool || ext.state_indices->numel() == in.seqs, "state_indices needs one entry per sequence");
+    require(!num_accepted_tokens.has_value() || num_accepted_tokens->numel() == in.seqs, "num_accepted_tokens needs one entry per sequence");
+    GdnLinearRecurrentArgs a{};
+    a.shape = in.shape;
+    a.gate = linear_gate(gate, value, in.packed);
+    a.num_accepted_tokens = i32(num_accepted_tokens, "num_accepted_tokens");
+    a.state_indices = i32(ext.state_indices, "state_indices");
+    at::Tensor out = empty(in.v.sizes(), in.v, at::kBFloat16), s_out;
+    if (steps) {
+        s_out = in.packed ? empty({in.q.size(0), in.vh, in.dv_al, in.dk_al}, in.v, in.state_type)
+                          : empty({in.q.size(0), in.q.size(1), in.vh, in.dv_al, in.dk_al}, in.v, in.state_type);
+        a.state_out = GdnState{s_out.data_ptr(), in.vh * in.dv_al * in.dk_al, in.dv_al * in.dk_al};
+    } else {
+        s_out = in_place ? *in.s_in : empty({in.seqs, in.vh, in.dv_al, in.dk_al}, in.v, in.state_type);
+        a.state_out = in.state(s_out);
+    }
+    if (in.empty_call()) {
+        if (!steps && !in_place && s_out.numel() > 0) in.s_in.has_value() ? (void)s_out.copy_(*in.s_in) : (void)s_out.zero_();
+        return {in.crop_out(out), in_place ? *initial_state : in.crop_state(s_out)};
+    }
+    a.q = linear_tok(in.q, in.packed);
+    a.k = linear_tok(in.k, in.packed);
+    a.v = linear_tok(in.v, in.packed);
+    a.out = linear_tok(out, in.packed);
+    if (in.s_in.has_value()) a.state_in = in.state(*in.s_in);
+    a.num_slots = pool ? static_cast<int32_t>(in.s_in->size(0)) : 0;
+    a.scale = scale.value_or(default_scale(in.dk));
+    a.store_step_state = steps ? 1 : 0;
+    a.state_dtype = in.state_type == at::kFloat ? GDN_F32 : GDN_BF16;
+    check(gdn_linear_recurrent(&a, stream), "linear_attention_recurrent");
+    return {in.crop_out(out), in_place ? *initial_state : in.crop_state(s_out)};
+}
+
+std::pair<at::Tensor, at::Tensor> linear_attention_chunked(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                                                           const std::optional<at::Tensor>& gate, std::optional<float> scale,
+                                                           const std::optional<at::Tensor>& initial_state,
+                                                           const std::optional<at::Tensor>& cu_seqlens, cudaStream_t stream) {
+    LinearInputs in(query, key, value, gate, initial_state, cu_seqlens, false, false);
+    GdnLinearChunkedArgs a{};
+    a.shape = in.shape;
+    a.gate = linear_gate(gate, value, in.packed);
+    at::Tensor out = empty(in.v.sizes(), in.v, at::kBFloat16), fin = empty({in.seqs, in.vh, in.dv_al, in.dk_al}, in.v, in.state_type);
+    if (in.empty_call()) {
+        if (fin.numel() > 0) in.s_in.has_value() ? (void)fin.copy_(*in.s_in) : (void)fin.zero_();
+        return {in.crop_out(out), in.crop_state(fin)};
+    }
+    a.q = linear_tok(in.q, in.packed);
+    a.k = linear_tok(in.k, in.packed);
+    a.v = linear_tok(in.v, in.packed);
+    a.out = linear_tok(out, in.packed);
+    if (in.s_in.has_value()) a.initial_state = in.state(*in.s_in);
+    a.final_state = in.state(fin);
+    a.scale = scale.value_or(default_scale(in.dk));
+    a.state_dtype = in.state_type == at::kFloat ? GDN_F32 : GDN_BF16;
+    at::Tensor ws;
+    if (const size_t bytes = gdn_linear_chunked_workspace_bytes(&a.shape)) {
+        ws = empty({static_cast<int64_t>(bytes)}, in.v, at::kByte);
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    check(gdn_linear_chunked(&a, stream), "linear_attention_chunked");
+    return {in.crop_out(out), in.crop_state(fin)};
+}
+
+at::Tensor group_norm(const at::Tensor& x, int64_t num_groups, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                      const std::optional<at::Tensor>& z, float eps, bool activation, cudaStream_t stream) {
+    require(x.is_cuda(), "x must be a CUDA tensor");
+    require(x.dim() >= 2, "x must be (samples, ..., channels)");
+    const int64_t N = x.size(0), C = x.size(-1);
+    require(num_groups > 0 && C > 0 && C % num_groups == 0, "the number of channels must be a positive multiple of num_groups");
+    require(C < (1ll << 31), "too many channels");
+    GdnGroupNormArgs a{};
+    a.dtype = dtype_tag(x);
+    on_device(weight, x, "weight");
+    on_device(bias, x, "bias");
+    on_device(z, x, "z");
+    // (samples, rows, channels) with contiguous channels: a view where the axes between can be one
+    auto rows_of = [&](const at::Tensor& t) {
+        if (t.stride(-1) != 1 && C > 1) return t.contiguous().view({N, -1, C});
+        if (t.dim() == 2) return t.unsqueeze(1);
+        if (t.dim() == 3) return t;
+        return t.is_contiguous() ? t.view({N, -1, C}) : t.reshape({N, x.numel() / std::max<int64_t>(N * C, 1), C});
+    };
+    at::Tensor y = empty(x.sizes(), x, x.scalar_type()), w, b;
+    if (x.numel() == 0) return y;
+    const at::Tensor xr = rows_of(x), yr = rows_of(y);
+    at::Tensor zr;
+    if (z.has_value()) {
+        require(z->sizes() == x.sizes() && z->scalar_type() == x.scalar_type(), "z must have the shape and dtype of x");
+        zr = rows_of(*z);
+    }
+    for (const auto* t : {&weight, &bias})
+        if (t->has_value()) {
+            require((*t)->dim() == 1 && (*t)->size(0) == C, "weight and bias must be (channels)");
+            a.param_dtype = dtype_tag(**t);
+        }
+    if (weight.has_value()) w = weight->contiguous();
+    if (bias.has_value()) b = bias->contiguous();
+    require(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias must share a dtype");
+    a.x = xr.data_ptr();
+    a.y = yr.data_ptr();
+    a.z = zr.defined() ? zr.data_ptr() : nullptr;
+    a.weight = w.defined() ? w.data_ptr() : nullptr;
+    a.bias = b.defined() ? b.data_ptr() : nullptr;
+    a.samples = N;
+    a.rows = xr.size(1);
+    a.channels = static_cast<int32_t>(C);
+    a.groups = static_cast<int32_t>(num_groups);
+    a.x_stride_sample = xr.stride(0);
+    a.x_stride_row = xr.stride(1);
+    a.y_stride_sample = yr.stride(0);
+    a.y_stride_row = yr.stride(1);
+    if (zr.defined()) {
+        a.z_stride_sample = zr.stride(0);
+        a.z_stride_row = zr.stride(1);
+    }
+    a.eps = eps;
+    a.silu = activation ? 1 : 0;
+    at::Tensor ws;
+    if (const size_t bytes = gdn_group_norm_workspace_bytes(a.samples, a.rows, a.channels, a.groups)) {
+        ws = empty({static_cast<int64_t>(bytes)}, x, at::kByte);
+        a.workspace = ws.data_ptr();
+        a.workspace_bytes = bytes;
+    }
+    check(gdn_group_norm(&a, stream), "group_norm");
+    return y;
+}
+
 void bf16_gdn_recurrent(at::Tensor& q, at::Tensor& k, at::Tensor& v, std::optional<at::Tensor>& initial_state,
                         at::Tensor& final_state, at::Tensor& out, std::optional<at::Tensor>& gate, at::Tensor& beta,
                         const std::string& /*compiled_dims*/, cudaStream_t stream, std::optional<at::Tensor>& cu_seqlens,

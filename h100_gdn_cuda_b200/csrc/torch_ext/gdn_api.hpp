@@ -79,6 +79,22 @@ std::pair<at::Tensor, std::optional<at::Tensor>> causal_conv1d(at::Tensor& x, at
                                                                bool return_final_state, cudaStream_t stream);
 at::Tensor gated_rmsnorm(at::Tensor& x, at::Tensor& z, at::Tensor& weight, float eps, cudaStream_t stream);
 
+// Linear attention with decay (no counterpart in the reference: the layer without the delta rule),
+//     S <- e^gate S + v k^T ,  o = scale S q ,
+// token by token (decode, draft runs; RecurrentExtensions as in recurrent_forward_ext) and for whole prompts, and the channels-last group
+// norm with SiLU or a gate that follows it.  `gate`: log-decays, one per head (v-heads) or one per token and head; nothing: no decay.
+std::pair<at::Tensor, at::Tensor> linear_attention_recurrent(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                                                             const std::optional<at::Tensor>& initial_state, const std::optional<at::Tensor>& gate,
+                                                             const std::optional<at::Tensor>& cu_seqlens,
+                                                             const std::optional<at::Tensor>& num_accepted_tokens, InferenceMode inference_mode,
+                                                             cudaStream_t stream, std::optional<float> scale, const RecurrentExtensions& ext);
+std::pair<at::Tensor, at::Tensor> linear_attention_chunked(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value,
+                                                           const std::optional<at::Tensor>& gate, std::optional<float> scale,
+                                                           const std::optional<at::Tensor>& initial_state,
+                                                           const std::optional<at::Tensor>& cu_seqlens, cudaStream_t stream);
+at::Tensor group_norm(const at::Tensor& x, int64_t num_groups, const std::optional<at::Tensor>& weight, const std::optional<at::Tensor>& bias,
+                      const std::optional<at::Tensor>& z, float eps, bool activation, cudaStream_t stream);
+
 // csrc/apis/gdn_forward.hpp:43-49: the recurrence on caller-provided output tensors.  `final_state` is
 // (B, vh, dv, dk), or one state per token when `store_step_state`; head dims must be multiples of 64
 // here (no padding can be done on the caller's tensors); `compiled_dims` is accepted and ignored.

@@ -92,6 +92,48 @@ PYBIND11_MODULE(gdn_cuda, m) {
         "y = x * rsqrt(mean(x^2) + eps) * weight * silu(z) over the last axis.  Not part of the reference's module.");
 
     m.def(
+        "linear_attention_recurrent",
+        [](at::Tensor& q, at::Tensor& k, at::Tensor& v, std::optional<at::Tensor> initial_state, std::optional<at::Tensor> gate,
+           std::optional<at::Tensor> cu_seqlens, std::optional<at::Tensor> num_accepted_tokens, int inference_mode,
+           std::optional<float> scale, bool inplace_state, std::optional<at::Tensor> state_indices) {
+            OnDevice dev(q);
+            gdn_cuda::RecurrentExtensions ext;
+            ext.inplace_state = inplace_state;
+            ext.state_indices = state_indices;
+            return gdn_cuda::linear_attention_recurrent(q, k, v, initial_state, gate, cu_seqlens, num_accepted_tokens,
+                                                        static_cast<gdn_cuda::InferenceMode>(inference_mode), dev.stream(), scale, ext);
+        },
+        py::arg("query"), py::arg("key"), py::arg("value"), py::arg("initial_state") = py::none(), py::arg("gate") = py::none(),
+        py::arg("cu_seqlens") = py::none(), py::arg("num_accepted_tokens") = py::none(), py::arg("inference_mode") = 0,
+        py::arg("scale") = py::none(), py::kw_only(), py::arg("inplace_state") = false, py::arg("state_indices") = py::none(),
+        "Linear attention with decay, token by token: S <- exp(gate) S + v k^T, o = scale S q.  gate: log-decays, (v-heads) or one "
+        "per token and head.  Returns (output, new_state).  Not part of the reference's module.");
+
+    m.def(
+        "linear_attention_chunked",
+        [](at::Tensor& q, at::Tensor& k, at::Tensor& v, std::optional<at::Tensor> gate, std::optional<float> scale,
+           std::optional<at::Tensor> initial_state, std::optional<at::Tensor> cu_seqlens) {
+            OnDevice dev(q);
+            return gdn_cuda::linear_attention_chunked(q, k, v, gate, scale, initial_state, cu_seqlens, dev.stream());
+        },
+        py::arg("query"), py::arg("key"), py::arg("value"), py::arg("gate") = py::none(), py::arg("scale") = py::none(),
+        py::arg("initial_state") = py::none(), py::arg("cu_seqlens") = py::none(),
+        "Linear attention with decay over whole prompts, padded or packed.  Returns (output, final_state).  Not part of the "
+        "reference's module.");
+
+    m.def(
+        "group_norm",
+        [](at::Tensor& x, int64_t num_groups, std::optional<at::Tensor> weight, std::optional<at::Tensor> bias,
+           std::optional<at::Tensor> z, float eps, bool activation) {
+            OnDevice dev(x);
+            return gdn_cuda::group_norm(x, num_groups, weight, bias, z, eps, activation, dev.stream());
+        },
+        py::arg("x"), py::arg("num_groups"), py::arg("weight") = py::none(), py::arg("bias") = py::none(),
+        py::arg("z") = py::none(), py::arg("eps") = 1e-5f, py::arg("activation") = true,
+        "Group norm over channels-last (samples, ..., channels), followed by SiLU or multiplied by silu(z).  Not part of the "
+        "reference's module.");
+
+    m.def(
         "fused_gdn_gating",
         [](at::Tensor& A_log, at::Tensor& dt_bias, at::Tensor& a, at::Tensor& b, bool is_var_len) {
             OnDevice dev(a);

@@ -357,6 +357,73 @@ int gdn_gated_rmsnorm(const void* x, const void* z, void* y, const void* weight,
                       int64_t x_row_stride, int64_t z_row_stride, int64_t y_row_stride, float eps,
                       gdn_stream_t stream);
 
+/* gdn_group_norm: group norm over the channels of (samples, rows, channels) tensors, channels last and contiguous.  The channels are
+ * `groups` equal runs; mean m and variance s2 (of the population) are those of all rows of a sample and the channels of a group:
+ *     u = (x - m) / sqrt(s2 + eps) * weight[c] + bias[c]
+ *     y = act(u), or with a gate z of the same shape  y = u * act(z);     act = SiLU where `silu` != 0, else the identity
+ * The output norm of linear attention is one sample per token (rows = 1, channels = heads * dv, groups = heads) with a gate.
+ * x, z, y share `dtype` (GDN_BF16 or GDN_F32) and are addressed sample*stride_sample + row*stride_row + c (elements; any strides and
+ * alignment: 16-byte aligned pointers, channels and strides that are multiples of 16 bytes are the fast case).  weight, bias: (channels) of `param_dtype`,
+ * either may be NULL (1 and 0).  y may be x or z itself (same strides).  Samples of more than 1024 values per group need a workspace of gdn_group_norm_workspace_bytes() bytes,
+ * 16-byte aligned. */
+typedef struct {
+    const void* x;
+    const void* z;
+    void* y;
+    const void* weight;
+    const void* bias;
+    int64_t samples, rows;
+    int32_t channels, groups;
+    int64_t x_stride_sample, x_stride_row, z_stride_sample, z_stride_row, y_stride_sample, y_stride_row;
+    int32_t dtype, param_dtype;
+    float eps;
+    int32_t silu;
+    void* workspace;
+    size_t workspace_bytes;
+} GdnGroupNormArgs;
+size_t gdn_group_norm_workspace_bytes(int64_t samples, int64_t rows, int32_t channels, int32_t groups);
+int gdn_group_norm(const GdnGroupNormArgs* args, gdn_stream_t stream);
+
+/* ---------------------------------------------------------------- linear attention with decay
+ * No counterpart in the reference: the layer without the delta rule.  Per token t of sequence s, v-head h:
+ *     S <- exp(g) S + v k^T ;  o = scale * S q
+ * Layouts, heads and states as above.  `gate` holds log-decays g <= 0 addressed like every per-token scalar (one decay per head: token
+ * and batch strides of 0; ptr == NULL: no decay); -infinity forgets everything before the token.  States may be bf16 or fp32
+ * (`state_dtype`, of both; strides in elements of it); they are computed with in fp32.  cu_seqlens alone describes packed inputs
+ * (chunk_indices, cu_chunks and total_chunks are not read); entries are clamped to the tokens there are, tokens behind the last sequence are left alone.
+ *
+ * gdn_linear_recurrent: token by token, for decode, draft runs and short prompts; dk a multiple of 8 up to 256, dv a multiple of 8.
+ * num_accepted_tokens, store_step_state and state_indices as in gdn_recurrent_forward; a slot outside [0, num_slots) is a padding sequence as
+ * well, and the slots of a call have to differ.  state_out may be state_in; it may be NULL where no state is wanted. */
+typedef struct {
+    GdnShape shape;
+    GdnTokenTensor q, k, v, out;
+    GdnTokenScalar gate;
+    GdnState state_in, state_out;
+    const int32_t* num_accepted_tokens;
+    const int32_t* state_indices;
+    int32_t num_slots;
+    float scale;
+    int32_t store_step_state;
+    int32_t state_dtype;
+} GdnLinearRecurrentArgs;
+int gdn_linear_recurrent(const GdnLinearRecurrentArgs* args, gdn_stream_t stream);
+
+/* gdn_linear_chunked: whole prompts.  dk a multiple of 8 up to 128 (up to 256 on the kernel of gdn_linear_recurrent), dv a multiple of 8.  initial_state.ptr and final_state.ptr may be NULL.
+ * `workspace`: gdn_linear_chunked_workspace_bytes(&shape) bytes or more, 256-byte aligned. */
+typedef struct {
+    GdnShape shape;
+    GdnTokenTensor q, k, v, out;
+    GdnTokenScalar gate;
+    GdnState initial_state, final_state;
+    float scale;
+    int32_t state_dtype;
+    void* workspace;
+    size_t workspace_bytes;
+} GdnLinearChunkedArgs;
+size_t gdn_linear_chunked_workspace_bytes(const GdnShape* shape);
+int gdn_linear_chunked(const GdnLinearChunkedArgs* args, gdn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -359,3 +359,38 @@ def max_abs_over_max(x: torch.Tensor, ref: torch.Tensor) -> float:
     x, ref = x.double(), ref.double()
     d = ref.abs().max().item() if ref.numel() else 0.0
     return (x - ref).abs().max().item() / (d if d > 0 else 1.0) if ref.numel() else 0.0
+
+
+# --------------------------------------------------------------------------
+# linear attention with decay, group norm (no counterpart in the reference)
+# --------------------------------------------------------------------------
+def linear_attention_ref(q, k, v, g, scale, state=None, steps=False):
+    """S <- e^g S + v k^T, o = scale S q, token by token in fp64.  Padded layouts; g (vh), (B,T,vh) or None.
+    Returns (out, final state or the state after every token)."""
+    B, T, vh, dv = v.shape
+    rep = vh // q.shape[2]
+    q, k, v = (x.double() for x in (q, k, v))
+    q, k = q.repeat_interleave(rep, 2), k.repeat_interleave(rep, 2)
+    g = torch.zeros(vh, device=v.device) if g is None else g
+    lam = torch.exp(g.double()).expand(B, T, vh) if g.dim() == 1 else torch.exp(g.double())
+    S = torch.zeros(B, vh, dv, q.shape[-1], dtype=torch.float64, device=v.device) if state is None else state.double()
+    out, kept = torch.empty_like(v), []
+    for t in range(T):
+        S = lam[:, t, :, None, None] * S + v[:, t, :, :, None] * k[:, t, :, None, :]
+        out[:, t] = scale * (S * q[:, t, :, None, :]).sum(-1)
+        if steps:
+            kept.append(S)
+    return out, (torch.stack(kept, 1) if steps else S)
+
+
+def group_norm_ref(x, groups, weight=None, bias=None, z=None, eps=1e-5, activation=True):
+    """Channels-last group norm in fp64; silu(u), or u * silu(z)."""
+    N, C = x.shape[0], x.shape[-1]
+    y = x.double().reshape(N, -1, groups, C // groups)
+    y = (y - y.mean((1, 3), keepdim=True)) / torch.sqrt(y.var((1, 3), unbiased=False, keepdim=True) + eps)
+    y = y.reshape(x.shape)
+    y = y if weight is None else y * weight.double()
+    y = y if bias is None else y + bias.double()
+    a = y if z is None else z.double()
+    a = a * torch.sigmoid(a) if activation else a
+    return a if z is None else y * a

@@ -1,0 +1,119 @@
+"""group_norm against the formula in 64 bits.
+
+Bound: with n values in a group, mean and variance are fp32 sums in trees or runs of at most a few thousand terms joined pairwise; a
+group of very many values is off by less than (64 + sqrt(n)) u, u = 2^-24, of the mean of the values' sizes.  u = (x - m) r w + b then is off by at most
+  E = (64 + sqrt(n)) u (|x| + mean|x|) r |w| + 16 u (|u| + |b|) ,  r = 1 / sqrt(var + eps)
+SiLU has a slope of at most 1.1 and costs a few more roundings; a gate multiplies by |act(z)|; the result is rounded once (half a step)."""
+import math
+
+import pytest
+import torch
+
+import h100_gdn_cuda_b200 as gdn
+from oracle import gdn_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+def check(y, x, G, w=None, b=None, z=None, eps=1e-5, activation=True):
+    assert y.shape == x.shape and y.dtype == x.dtype
+    ref = O.group_norm_ref(x, G, w, b, z, eps, activation)
+    lin = O.group_norm_ref(x, G, w, b, None, eps, False)
+    N, C = x.shape[0], x.shape[-1]
+    xs = x.double().reshape(N, -1, G, C // G)
+    n = xs.shape[1] * xs.shape[3]
+    size = (xs.abs() + xs.abs().mean((1, 3), keepdim=True)) / torch.sqrt(xs.var((1, 3), unbiased=False, keepdim=True) + eps)
+    size = size.reshape(x.shape) * (1 if w is None else w.double().abs())
+    u = 2.0 ** -24
+    E = (64 + math.sqrt(n)) * u * size + 16 * u * (lin.abs() + (0 if b is None else b.double().abs()))
+    if z is not None:
+        gate = z.double() * torch.sigmoid(z.double()) if activation else z.double()
+        E = E * gate.abs() + 16 * u * ref.abs()
+    elif activation:
+        E = 1.1 * E + 16 * u * lin.abs()
+    tol = E + torch.finfo(x.dtype).eps / 2 * (ref.abs() + E) + 1e-30
+    err = (y.double() - ref).abs()
+    assert bool((err <= tol).all()), (err / tol).max().item()
+
+
+def make(shape, dtype, offset=0.0, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    C = shape[-1]
+    x = (torch.randn(*shape, generator=gen, device="cuda") + offset).to(dtype)
+    z = torch.randn(*shape, generator=gen, device="cuda").to(dtype)
+    return x, z, torch.randn(C, generator=gen, device="cuda"), torch.randn(C, generator=gen, device="cuda")
+
+
+SHAPES = [((1, 8), 1), ((3, 4096), 32), ((5, 128), 128), ((7, 96), 3), ((2, 1040), 1), ((33, 2 * 1500), 2), ((300, 3 * 80), 3), ((2, 5, 12), 4),
+          ((2, 7, 9), 3), ((1, 1000, 64), 8), ((4, 4095, 40), 2), ((2, 33, 17, 30), 3), ((1, 300, 4100), 1), ((3, 50, 5000), 1000), ((2, 2000, 6), 6), ((1, 1, 4, 1, 16), 2)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,G", SHAPES, ids=str)
+def test_shapes(shape, G, dtype):
+    x, z, w, b = make(shape, dtype)
+    check(gdn.group_norm(x, G, w, b, z), x, G, w, b, z)
+    check(gdn.group_norm(x, G, w.bfloat16(), None), x, G, w.bfloat16())
+    check(gdn.group_norm(x, G, None, b, activation=False), x, G, None, b, activation=False)
+    check(gdn.group_norm(x, G, None, None, z, 1e-3, False), x, G, None, None, z, 1e-3, False)
+
+
+@pytest.mark.parametrize("shape,G", [((64, 256), 2), ((2, 3000, 64), 4)], ids=str)
+def test_large_mean(shape, G):
+    """A mean 1000 times the spread costs no more digits than the values themselves have."""
+    x, z, w, b = make(shape, torch.float32, 1000.0)
+    check(gdn.group_norm(x, G, w, b, z), x, G, w, b, z)
+
+
+@pytest.mark.parametrize("shape,G", [((6, 256), 2), ((2, 700, 64), 4)], ids=str)
+def test_constant_groups_and_nan(shape, G):
+    x, z, w, b = make(shape, torch.float32)
+    x[0] = 3.0
+    check(gdn.group_norm(x, G, w, b), x, G, w, b)
+    x[1, ..., 0] = math.nan  # stays in its group
+    y = gdn.group_norm(x, G, w, b)
+    W = shape[-1] // G
+    assert bool(torch.isnan(y[1, ..., :W]).all()) and bool(torch.isfinite(y[1, ..., W:]).all()) and bool(torch.isfinite(y[0]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_views(dtype):
+    x, z, w, b = make((4, 600, 48), dtype)
+    wide = torch.cat([x, z], -1)
+    for xv, zv in ((wide[..., :48], wide[..., 48:]), (x.transpose(0, 1).contiguous().transpose(0, 1), z), (x.transpose(1, 2).contiguous().transpose(1, 2), z),
+                   (torch.cat([x.flatten()[:1], x.flatten()])[1:].view_as(x), z), (x, z[:, :1].expand_as(z)), (x[:1].expand_as(x), z)):
+        check(gdn.group_norm(xv, 6, w, b, zv), xv, 6, w, b, zv)
+    rows = torch.cat([x[0], z[0]], -1)[:, :48]
+    check(gdn.group_norm(rows, 6, w, b), rows, 6, w, b)
+    four = x.view(4, 20, 30, 48).transpose(1, 2)
+    check(gdn.group_norm(four, 6, w, b), four, 6, w, b)
+
+
+def test_same_bits_alone_and_in_a_batch():
+    x, z, w, b = make((5, 1300, 64), torch.bfloat16)
+    y = gdn.group_norm(x, 4, w, b, z)
+    assert torch.equal(y, gdn.group_norm(x, 4, w, b, z))
+
+
+def test_nothing_to_do():
+    for shape in ((0, 16), (2, 0, 16), (0, 5, 16)):
+        assert gdn.group_norm(torch.zeros(shape, device="cuda"), 4).shape == shape
+
+
+def test_large():
+    """More than 2^31 elements."""
+    x = torch.empty(2 ** 19 + 3, 4096, dtype=torch.bfloat16, device="cuda")
+    x.normal_(generator=torch.Generator(device="cuda").manual_seed(0))
+    y = gdn.group_norm(x, 32)
+    check(y[-50:], x[-50:], 32)
+    check(y[:50], x[:50], 32)
+
+
+def test_refusals():
+    x, z, w, b = make((2, 5, 12), torch.float32)
+    for bad in (lambda: gdn.group_norm(x, 5), lambda: gdn.group_norm(x, 0), lambda: gdn.group_norm(x, -3), lambda: gdn.group_norm(x.half(), 3),
+                lambda: gdn.group_norm(x.cpu(), 3), lambda: gdn.group_norm(x[0, 0], 3), lambda: gdn.group_norm(x, 3, w[:6]),
+                lambda: gdn.group_norm(x, 3, w, b.bfloat16()), lambda: gdn.group_norm(x, 3, w.double()), lambda: gdn.group_norm(x, 3, z=z[:1]),
+                lambda: gdn.group_norm(x, 3, z=z.bfloat16()), lambda: gdn.group_norm(x, 3, w.cpu())):
+        with pytest.raises(RuntimeError):
+            bad()
