@@ -1,4 +1,5 @@
 // C-ABI entry points of linear attention with decay (see include/gdn_b200.h): argument checks and launches.
+#include "kernels/linear_chunked.cuh"
 #include "kernels/linear_recurrent.cuh"
 #include "token_host.hpp"
 
@@ -30,6 +31,35 @@ int launch_linear_recurrent(const LinRecurrentParams& p, cudaStream_t st) {
     if (p.dk <= 64) GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<8, kF32>, g, kLinThreads, 0, st, p));
     else if (p.dk <= 128) GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<16, kF32>, g, kLinThreads, 0, st, p));
     else GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<32, kF32>, g, kLinThreads, 0, st, p));
+    return GDN_OK;
+}
+
+// Tensor map of a token tensor; an axis of one token or head may come with any stride, the map wants a positive one.
+int linear_map(CUtensorMap* out, GdnTokenTensor t, const GdnShape& s, int heads, int dim, const char* name) {
+    if (heads == 1) t.stride_head = dim;
+    const int64_t tokens = s.cu_seqlens ? s.total_tokens : s.seq_len;
+    if (tokens == 1) t.stride_token = std::max<int64_t>(t.stride_token, static_cast<int64_t>(heads) * t.stride_head);
+    return make_token_map(out, t, s, heads, name, dim);
+}
+
+bool wide_linear(const GdnShape& s) { return s.head_dim_k > 128; }
+
+template <int DK, int DV>
+int launch_linear_chunked(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmO, const LinChunkedParams& p,
+                          int sms, cudaStream_t st) {
+    using L = LinSmem<DK, DV>;
+    if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV>>(L::kBytes)) return rc;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.num_items, sms)));
+    cfg.blockDim = dim3(lin::kThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV>, tmQ, tmK, tmV, tmO, p));
     return GDN_OK;
 }
 
@@ -79,15 +109,57 @@ size_t gdn_linear_chunked_workspace_bytes(const GdnShape*) { return 0; }
 
 int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     GDN_REQUIRE(a != nullptr, "gdn_linear_chunked: args is NULL");
-    GdnLinearRecurrentArgs r{};
-    r.shape = a->shape;
-    r.q = a->q; r.k = a->k; r.v = a->v; r.out = a->out;
-    r.gate = a->gate;
-    r.state_in = a->initial_state;
-    r.state_out = a->final_state;
-    r.scale = a->scale;
-    r.state_dtype = a->state_dtype;
-    return gdn_linear_recurrent(&r, stream);
+    const GdnShape& s = a->shape;
+    if (int rc = check_linear_shape(s, "gdn_linear_chunked")) return rc;
+    const long long tokens = s.cu_seqlens ? s.total_tokens : static_cast<long long>(s.batch) * s.seq_len;
+    if (wide_linear(s) || tokens == 0) {  // (no tokens: the states are handed through)
+        GdnLinearRecurrentArgs r{};
+        r.shape = s;
+        r.q = a->q; r.k = a->k; r.v = a->v; r.out = a->out;
+        r.gate = a->gate;
+        r.state_in = a->initial_state;
+        r.state_out = a->final_state;
+        r.scale = a->scale;
+        r.state_dtype = a->state_dtype;
+        return gdn_linear_recurrent(&r, stream);
+    }
+    GDN_REQUIRE(a->state_dtype == GDN_BF16 || a->state_dtype == GDN_F32, "gdn_linear_chunked: state_dtype must be bf16 or f32");
+    if (int rc = check_linear_tokens(a->q, s, s.num_k_heads, s.head_dim_k, "q")) return rc;
+    if (int rc = check_linear_tokens(a->k, s, s.num_k_heads, s.head_dim_k, "k")) return rc;
+    if (int rc = check_linear_tokens(a->v, s, s.num_v_heads, s.head_dim_v, "v")) return rc;
+    if (int rc = check_linear_tokens(a->out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
+    if (int rc = check_scalar(a->gate, "gate", false)) return rc;
+    if (int rc = check_state(a->initial_state, "initial_state")) return rc;
+    if (int rc = check_state(a->final_state, "final_state")) return rc;
+    GDN_REQUIRE(tokens < (1ll << 31) - kChunk, "gdn_linear_chunked: too many tokens");
+    DeviceInfo* d = nullptr;
+    if (int rc = get_device_info(&d)) return rc;
+    CUtensorMap tmQ, tmK, tmV, tmO;
+    if (int rc = linear_map(&tmQ, a->q, s, s.num_k_heads, s.head_dim_k, "q")) return rc;
+    if (int rc = linear_map(&tmK, a->k, s, s.num_k_heads, s.head_dim_k, "k")) return rc;
+    if (int rc = linear_map(&tmV, a->v, s, s.num_v_heads, s.head_dim_v, "v")) return rc;
+    if (int rc = linear_map(&tmO, a->out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
+    LinChunkedParams p{};
+    p.out = token_view(a->out);
+    p.gate = scalar_view(a->gate);
+    p.state_in = a->initial_state.ptr; p.si_ss = a->initial_state.stride_seq; p.si_sh = a->initial_state.stride_head;
+    p.state_out = a->final_state.ptr; p.so_ss = a->final_state.stride_seq; p.so_sh = a->final_state.stride_head;
+    p.cu_seqlens = s.cu_seqlens;
+    p.total_tokens = s.total_tokens;
+    p.num_seqs = s.batch; p.seq_len = s.seq_len; p.kh = s.num_k_heads; p.vh = s.num_v_heads;
+    p.dk = s.head_dim_k; p.dv = s.head_dim_v; p.dv_tiles = (s.head_dim_v + 127) / 128;
+    p.state_f32 = a->state_dtype == GDN_F32;
+    p.scale = a->scale;
+    p.status = d->status;
+    p.seg_chunks = 1 << 26;  // (more than there are)
+    p.num_segments = 1;
+    const long long items = static_cast<long long>(s.batch) * p.vh * p.dv_tiles;
+    GDN_REQUIRE(items < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
+    p.num_items = static_cast<int>(items);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.dk <= 64)
+        return p.dv <= 64 ? launch_linear_chunked<64, 64>(tmQ, tmK, tmV, tmO, p, d->sms, st) : launch_linear_chunked<64, 128>(tmQ, tmK, tmV, tmO, p, d->sms, st);
+    return p.dv <= 64 ? launch_linear_chunked<128, 64>(tmQ, tmK, tmV, tmO, p, d->sms, st) : launch_linear_chunked<128, 128>(tmQ, tmK, tmV, tmO, p, d->sms, st);
 }
 
 }  // extern "C"
