@@ -145,13 +145,13 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     p.state_in = a->initial_state.ptr; p.si_ss = a->initial_state.stride_seq; p.si_sh = a->initial_state.stride_head;
     p.state_out = a->final_state.ptr; p.so_ss = a->final_state.stride_seq; p.so_sh = a->final_state.stride_head;
     p.cu_seqlens = s.cu_seqlens;
-    p.total_tokens = s.total_tokens;
+    p.total_tokens = static_cast<int>(s.total_tokens);
     p.num_seqs = s.batch; p.seq_len = s.seq_len; p.kh = s.num_k_heads; p.vh = s.num_v_heads;
     p.dk = s.head_dim_k; p.dv = s.head_dim_v; p.dv_tiles = (s.head_dim_v + 127) / 128;
     p.state_f32 = a->state_dtype == GDN_F32;
     p.scale = a->scale;
     p.status = d->status;
-    p.seg_chunks = 1 << 26;  // (more than there are)
+    p.seg_chunks = static_cast<int>((tokens + kChunk - 1) / kChunk);  // (no sequence has more)
     p.num_segments = 1;
     const long long items = static_cast<long long>(s.batch) * p.vh * p.dv_tiles;
     GDN_REQUIRE(items < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");

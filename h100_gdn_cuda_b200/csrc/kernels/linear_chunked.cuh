@@ -8,11 +8,16 @@
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
 // items and chunks, handing tiles on through mbarriers:
 //   warps 0-7   state warps: the fp32 state in registers (lane = dv row, half of the columns each), its bf16 copy into tensor memory
-//   warps 8-11  output warps: both parts of O scaled and added, transposed through shared memory, stored
-//   warps 12-15 score warps: e^{G_L - G_j} K as bf16 tile; the scores with their decay as bf16 tile
-//   warp 16     producer: tensor copies of Q, K, V into a ring of stages
-//   warp 17     issues every tcgen05.mma
-//   warp 18     the gates' running sums and the factors made of them
+//   warps 8-11  output warps: both parts of O added, transposed through shared memory, stored
+//   warps 12-15 score warps: the scores with their decay as bf16 tile
+//   warps 16-19 key warps: K times e^{G_L - G_j} as bf16 tile
+//   warp 20     producer: tensor copies of Q, K, V into a ring of stages
+//   warp 21     issues Q K^T and V^T P^T
+//   warp 22     issues the state's products, D = V^T (decayed K) and S Q^T
+//   warp 23     finds the items; the gates' running sums and the factors made of them
+// What bounds a chunk is not the tensor pipe (900 cycles of products) but what a warp of each role needs for its part, a few hundred
+// instructions one behind the other, and how much of the roles' code the instruction cache holds: the waits are the short form and the
+// item search is one warp's (104 KB of code took 5200 cycles a chunk with both SMs of a pair at work, 2900 with one).
 // All accumulators that feed the output are transposed (128 dv rows = M): S is an A operand in tensor memory, V one read MN-major
 // from the tile as it was copied, Q and the scores are B operands.
 #pragma once
@@ -29,8 +34,7 @@ struct LinChunkedParams {
     void* state_out;
     long long si_ss, si_sh, so_ss, so_sh;
     const int* cu_seqlens;
-    long long total_tokens;
-    int num_seqs, seq_len, kh, vh, dk, dv, dv_tiles;
+    int total_tokens, num_seqs, seq_len, kh, vh, dk, dv, dv_tiles;
     int state_f32;
     float scale;
     int* status;
@@ -48,27 +52,29 @@ __device__ __forceinline__ float lin_gate_log2(float g) {
     return x < -160.f ? -160.f : x;
 }
 
-struct LinItem {
-    int seq, head, dvt, batch, segment, segments;
-    long long slot, tok0, tokens;  // of the segment
-    int chunks;
+struct alignas(16) LinItem {
+    int seq, head, khead, dvt;
+    int batch, segment, segments, index;  // index: of the item
+    int slot, tok0, tokens, chunks;       // of the segment; chunks < 0: no more items
 };
 
-// Walks the items of a CTA in rising order; warp-collective (every warp keeps its own).
+// Walks the items of a CTA in rising order; warp-collective.
 struct LinWalker {
-    int base = 0;         // packed mode: first sequence of the 32 that were looked at last
-    long long first = 0;  // its first slot
+    int base = 0;   // packed mode: first sequence of the 32 that were looked at last
+    int first = 0;  // its first slot
     // false: a surplus item
-    __device__ __forceinline__ bool locate(const LinChunkedParams& p, long long it, LinItem& o) {
+    __device__ __forceinline__ bool locate(const LinChunkedParams& p, int it, LinItem& o) {
         const int per = p.vh * p.dv_tiles;
         o.slot = it / per;
-        const int r = static_cast<int>(it - o.slot * per);
+        const int r = it - o.slot * per;
         o.head = r / p.dv_tiles;
         o.dvt = r - o.head * p.dv_tiles;
-        long long bos = 0, len = p.seq_len;
+        o.khead = o.head / (p.vh / p.kh);
+        o.index = it;
+        int bos = 0, len = p.seq_len;
         if (!p.cu_seqlens) {
-            o.seq = static_cast<int>(o.slot / p.num_segments);
-            o.segment = static_cast<int>(o.slot - static_cast<long long>(o.seq) * p.num_segments);
+            o.seq = o.slot / p.num_segments;
+            o.segment = o.slot - o.seq * p.num_segments;
             o.segments = p.num_segments;
             o.batch = o.seq;
         } else {
@@ -77,13 +83,11 @@ struct LinWalker {
             while (true) {
                 if (base >= p.num_seqs) return false;
                 const int s = base + lane;
-                long long b = 0, e = 0;
-                int n = 0;
+                int b = 0, e = 0, n = 0;
                 if (s < p.num_seqs) {
-                    b = min(max(static_cast<long long>(p.cu_seqlens[s]), 0ll), p.total_tokens);
-                    e = min(max(static_cast<long long>(p.cu_seqlens[s + 1]), b), p.total_tokens);
-                    const long long chunks = (e - b + kChunk - 1) / kChunk;
-                    n = max(1, static_cast<int>((chunks + p.seg_chunks - 1) / p.seg_chunks));
+                    b = min(max(p.cu_seqlens[s], 0), p.total_tokens);
+                    e = min(max(p.cu_seqlens[s + 1], b), p.total_tokens);
+                    n = max(1, ((e - b + kChunk - 1) / kChunk + p.seg_chunks - 1) / p.seg_chunks);
                 }
                 int incl = n;
 #pragma unroll
@@ -100,16 +104,16 @@ struct LinWalker {
                 const int mine = __ffs(__ballot_sync(0xffffffffu, o.slot < first + incl)) - 1;
                 o.seq = base + mine;
                 o.segments = __shfl_sync(0xffffffffu, n, mine);
-                o.segment = static_cast<int>(o.slot - first) - (__shfl_sync(0xffffffffu, incl, mine) - o.segments);
+                o.segment = o.slot - first - (__shfl_sync(0xffffffffu, incl, mine) - o.segments);
                 bos = __shfl_sync(0xffffffffu, b, mine);
                 len = __shfl_sync(0xffffffffu, e, mine) - bos;
                 break;
             }
         }
-        const long long t0 = static_cast<long long>(o.segment) * p.seg_chunks * kChunk;
+        const int t0 = o.segment * p.seg_chunks * kChunk;
         o.tok0 = bos + t0;
-        o.tokens = min(len - t0, static_cast<long long>(p.seg_chunks) * kChunk);
-        o.chunks = static_cast<int>((o.tokens + kChunk - 1) / kChunk);
+        o.tokens = min(len - t0, p.seg_chunks * kChunk);
+        o.chunks = (o.tokens + kChunk - 1) / kChunk;
         return true;
     }
 };
@@ -119,17 +123,18 @@ struct LinSmem {
     static constexpr int kStages = 3;
     static constexpr int kTileK = kChunk * DK * 2, kTileV = kChunk * DV * 2;
     static constexpr int kOffQ = 0, kOffK = kTileK, kOffV = 2 * kTileK, kStage = 2 * kTileK + kTileV;
-    static constexpr int kOffKT = kStages * kStage;        // 2 x decayed K
-    static constexpr int kOffP = kOffKT + 2 * kTileK;      // 2 x scores, 64 x 64
-    static constexpr int kOffO = kOffP + 2 * 8192;         // output staging
-    static constexpr int kOffGate = kOffO + kTileV;        // 4 x { G[64], e^{G_L - G_j}[64], scale e^{G_i}[64], e^{G_L} }
-    static constexpr int kGateStride = (3 * 64 + 4) * 4;
+    static constexpr int kOffKT = kStages * kStage;    // 2 x decayed K
+    static constexpr int kOffP = kOffKT + 2 * kTileK;  // 2 x scores, 64 x 64
+    static constexpr int kOffO = kOffP + 2 * 8192;     // output staging
+    // 4 x gate factors, fp32: G[64] (log2); e^{G_r - G_j}[64], r the last token of j's eight; e^{G_L - G_j}[64]; scale e^{G_i}[64]; e^{G_L}
+    static constexpr int kOffGate = kOffO + kTileV;
+    static constexpr int kGateStride = (4 * 64 + 4) * 4;
     static constexpr int kOffBar = kOffGate + 4 * kGateStride;
-    static constexpr int kBytes = kOffBar + 256 + 1024;
+    static constexpr int kBytes = kOffBar + 512 + 1024;
 };
 
 namespace lin {
-constexpr int kThreads = 640;  // 5 warpgroups: 2 x state, output, scores, the rest
+constexpr int kThreads = 768;  // 6 warpgroups: 2 x state, output, scores, keys, the rest
 constexpr uint32_t kTmS = 0;     // bf16 state, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
 constexpr uint32_t kTmD = 128;   // fp32 state increment, 128 columns
@@ -145,6 +150,30 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two fp32 values in a 64-bit register pair
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 pk(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ f2 pk(uint32_t lo, uint32_t hi) { return pk(__uint_as_float(lo), __uint_as_float(hi)); }
+__device__ __forceinline__ void unpk(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+    f2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+    f2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack2(f2 v) {
+    float lo, hi;
+    unpk(v, lo, hi);
+    return ptx::pack_bf16(lo, hi);
+}
 // the running sums of 64 log2-decays, lane l: tokens l and l + 32
 __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
 #pragma unroll
@@ -157,13 +186,14 @@ __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
     }
     g1 += __shfl_sync(0xffffffffu, g0, 31);
 }
-// 16 bytes of K times a factor
+// 16 bytes of K times a factor (rounded to bf16 once, as an operand)
 __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
     using namespace ptx;
-    v.x = pack_bf16(bf16_lo(v.x) * f, bf16_hi(v.x) * f);
-    v.y = pack_bf16(bf16_lo(v.y) * f, bf16_hi(v.y) * f);
-    v.z = pack_bf16(bf16_lo(v.z) * f, bf16_hi(v.z) * f);
-    v.w = pack_bf16(bf16_lo(v.w) * f, bf16_hi(v.w) * f);
+    const f2 w = pk(f, f);
+    v.x = pack2(mul2(pk(bf16_lo(v.x), bf16_hi(v.x)), w));
+    v.y = pack2(mul2(pk(bf16_lo(v.y), bf16_hi(v.y)), w));
+    v.z = pack2(mul2(pk(bf16_lo(v.z), bf16_hi(v.z)), w));
+    v.w = pack2(mul2(pk(bf16_lo(v.w), bf16_hi(v.w)), w));
     return v;
 }
 }  // namespace lin
@@ -179,33 +209,33 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
-    // (no barrier may run two phases ahead of somebody who waits on it: each one's next phase needs what its waiters do after theirs)
-    uint64_t* bar_qk = bars;          // [3] Q and K of a stage have arrived
-    uint64_t* bar_v = bars + 3;       // [3] V
-    uint64_t* bar_empty = bars + 6;   // [3] the products of the stage's chunk are done
-    uint64_t* bar_gate = bars + 9;    // [4] gate factors of a chunk
-    uint64_t* bar_gfree = bars + 13;  // [4] read by state and output warps
-    uint64_t* bar_score = bars + 17;  // [2] Q K^T done
-    uint64_t* bar_p = bars + 19;      // [2] scores written
-    uint64_t* bar_kt = bars + 21;     // [2] decayed K written (and rows of V past the end cleared)
-    uint64_t* bar_ktfree = bars + 23; // [2] and read
-    uint64_t* bar_o = bars + 25;      // [2] both parts of O done
-    uint64_t* bar_ofree = bars + 27;  // [2] and read
-    uint64_t* bar_d = bars + 29;      // state increment done
-    uint64_t* bar_dfree = bars + 30;  // and read
-    uint64_t* bar_s = bars + 31;      // the state a chunk reads is in tensor memory; (256 bytes of barriers end here)
-    __shared__ uint64_t bar_sq;       // and has been read
-    __shared__ uint32_t tmem_slot;
-    __shared__ int abort_word;
-    int* abort_flag = &abort_word;
+    // No barrier may run two phases ahead of somebody who waits on it: each one's next phase but one needs what its waiters do after
+    // theirs.  Barriers of two are those of even and of odd chunks.
+    uint64_t* bar_full = bars;                  // [stages] Q, K, V of a stage have arrived
+    uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done (both issuers)
+    uint64_t* bar_gate = bar_empty + kStages;   // [4] gate factors of a chunk
+    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps
+    uint64_t* bar_score = bar_gfree + 4;        // [2] Q K^T done
+    uint64_t* bar_p = bar_score + 2;            // [2] scores written, and the accumulator of V^T P^T read two chunks before
+    uint64_t* bar_dgo = bar_p + 2;              // [2] decayed K written (rows of V past the end cleared), and the increment before read
+    uint64_t* bar_ktfree = bar_dgo + 2;         // [2] decayed K read
+    uint64_t* bar_sgo = bar_ktfree + 2;         // [2] the state is in tensor memory, and the accumulator of S Q^T read two chunks before
+    uint64_t* bar_o = bar_sgo + 2;              // [2] both parts of O done
+    uint64_t* bar_d = bar_o + 2;                // state increment done
+    uint64_t* bar_sq = bar_d + 1;               // the bf16 state has been read
+    uint64_t* bar_item = bar_sq + 1;            // [2] an item is there
+    uint64_t* bar_itemfree = bar_item + 2;      // [2] and every warp has it
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_itemfree + 2);
+    int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
+    LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
+    static_assert((2 * kStages + 26) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         *abort_flag = 0;
-        for (int i = 0; i < 3; ++i) {
-            mbar_init(&bar_qk[i], 1);
-            mbar_init(&bar_v[i], 1);
-            mbar_init(&bar_empty[i], 1);
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&bar_full[i], 1);
+            mbar_init(&bar_empty[i], 2);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar_gate[i], 1);
@@ -213,128 +243,141 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_score[i], 1);
-            mbar_init(&bar_p[i], 4);
-            mbar_init(&bar_kt[i], 4);
+            mbar_init(&bar_p[i], 8);
+            mbar_init(&bar_dgo[i], 12);
             mbar_init(&bar_ktfree[i], 1);
-            mbar_init(&bar_o[i], 1);
-            mbar_init(&bar_ofree[i], 4);
+            mbar_init(&bar_sgo[i], 12);
+            mbar_init(&bar_o[i], 2);
+            mbar_init(&bar_item[i], 1);
+            mbar_init(&bar_itemfree[i], 23);
         }
         mbar_init(bar_d, 1);
-        mbar_init(bar_dfree, 8);
-        mbar_init(bar_s, 8);
-        mbar_init(&bar_sq, 1);
+        mbar_init(bar_sq, 1);
         mbar_fence_init();
     }
-    if (warp == 0) tmem_alloc(&tmem_slot, 512);
+    // the scores' blocks above the diagonal stay zero: nobody writes them
+    for (int i = tid; i < 2 * 8192 / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + L::kOffP + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+    if (warp == 0) tmem_alloc(tmem_slot, 512);
     fence_proxy_async_smem();
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = tmem_slot;
+    const uint32_t tmem = *tmem_slot;
     grid_dep_wait();
     grid_dep_launch();
 
     auto gate_buf = [&](uint32_t gc) { return reinterpret_cast<float*>(smem + L::kOffGate + (gc & 3) * L::kGateStride); };
-    LinWalker walker;
     LinItem it;
-    uint32_t gc = 0;  // chunks so far, the same count in every role
+    uint32_t gc = 0, taken = 0;  // chunks and items so far, the same counts in every role
+    auto next_item = [&]() {
+        const uint32_t s = taken & 1;
+        mbar_wait_short(&bar_item[s], (taken >> 1) & 1, abort_flag);
+        it = items[s];
+        ++taken;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar_itemfree[s]);
+        return it.chunks >= 0 && *static_cast<volatile int*>(abort_flag) == 0;
+    };
+    // registers of the CTA: 768 x 80; 8 warps at 104, 8 at 80, 8 at 56
+    static_assert(32 * (8 * 104 + 8 * 80 + 8 * 56) <= kThreads * 80, "register pool of the CTA");
 
     if (warp < 8) {
         // =============================================================== state warps
-        // registers of the CTA: 640 x 96; 8 warps at 112, 8 at 96, 4 at 56
-        static_assert(32 * (8 * 112 + 8 * 96 + 4 * 56) <= kThreads * 96, "register pool of the CTA");
-        reg_inc<112>();
+        reg_inc<104>();
         constexpr int kCols = DK / 2;  // of a thread
         const int lq = warp & 3, hf = warp >> 2;
         const uint32_t tm_lane = static_cast<uint32_t>(32 * lq) << 16;
-        float S[kCols];
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x) {
-            if (!walker.locate(p, i, it)) continue;
+        f2 S[kCols / 2];
+        if (lane == 0) mbar_arrive(&bar_dgo[0]);  // (there is no increment before the first)
+        while (next_item()) {
             const int row = it.dvt * 128 + 32 * lq + lane;
             const bool row_in = 32 * lq + lane < DV && row < p.dv;
             const int c0 = kCols * hf;
             // ---- the state that enters the segment
-            const bool from_seg = it.segment > 0;
-            if (from_seg) {
-                const float* src = p.seg_state + (i - static_cast<long long>(p.vh) * p.dv_tiles) * (DV * DK) + (32 * lq + lane) * DK + c0;
+            if (it.segment > 0) {
+                const float4* src = reinterpret_cast<const float4*>(p.seg_state + static_cast<long long>(it.index - p.vh * p.dv_tiles) * (128 * DK) + (32 * lq + lane) * DK + c0);
 #pragma unroll
                 for (int q = 0; q < kCols / 4; ++q) {
-                    const float4 v = 32 * lq + lane < DV ? __ldcg(reinterpret_cast<const float4*>(src) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    S[4 * q] = v.x; S[4 * q + 1] = v.y; S[4 * q + 2] = v.z; S[4 * q + 3] = v.w;
+                    const float4 v = __ldcg(src + q);
+                    S[2 * q] = pk(v.x, v.y);
+                    S[2 * q + 1] = pk(v.z, v.w);
                 }
             } else if (p.state_in && p.state_f32) {
                 const float* src = static_cast<const float*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0;
 #pragma unroll
                 for (int q = 0; q < kCols / 4; ++q) {
                     const float4 v = row_in && c0 + 4 * q < p.dk ? *(reinterpret_cast<const float4*>(src) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    S[4 * q] = v.x; S[4 * q + 1] = v.y; S[4 * q + 2] = v.z; S[4 * q + 3] = v.w;
+                    S[2 * q] = pk(v.x, v.y);
+                    S[2 * q + 1] = pk(v.z, v.w);
                 }
             } else if (p.state_in) {
                 const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0;
 #pragma unroll
                 for (int q = 0; q < kCols / 8; ++q) {
                     const uint4 v = row_in && c0 + 8 * q < p.dk ? *(reinterpret_cast<const uint4*>(src) + q) : make_uint4(0u, 0u, 0u, 0u);
-                    S[8 * q] = bf16_lo(v.x); S[8 * q + 1] = bf16_hi(v.x); S[8 * q + 2] = bf16_lo(v.y); S[8 * q + 3] = bf16_hi(v.y);
-                    S[8 * q + 4] = bf16_lo(v.z); S[8 * q + 5] = bf16_hi(v.z); S[8 * q + 6] = bf16_lo(v.w); S[8 * q + 7] = bf16_hi(v.w);
+                    S[4 * q] = pk(bf16_lo(v.x), bf16_hi(v.x));
+                    S[4 * q + 1] = pk(bf16_lo(v.y), bf16_hi(v.y));
+                    S[4 * q + 2] = pk(bf16_lo(v.z), bf16_hi(v.z));
+                    S[4 * q + 3] = pk(bf16_lo(v.w), bf16_hi(v.w));
                 }
             } else {
 #pragma unroll
-                for (int q = 0; q < kCols; ++q) S[q] = 0.f;
+                for (int q = 0; q < kCols / 2; ++q) S[q] = 0ull;
             }
-            // the bf16 copy that chunk `n` reads (rounded for the product only: the state itself stays in fp32)
-            auto publish = [&](uint32_t n) {
-                if (n > 0) mbar_wait(&bar_sq, (n - 1) & 1, abort_flag);  // the copy of the chunk before has been read
+            // Chunk by chunk: the bf16 copy that the chunk reads (rounded for the product only: the state itself stays in fp32), then its increment.
+#pragma unroll 1
+            for (int c = 0; c < it.chunks; ++c, ++gc) {
+                if (gc > 0) mbar_wait_short(bar_sq, (gc - 1) & 1, abort_flag);  // the copy of the chunk before has been read
                 tc_fence_after_sync();
 #pragma unroll
                 for (int q = 0; q < kCols / 32; ++q) {
                     uint32_t w[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e] = pack_bf16(S[q * 32 + 2 * e], S[q * 32 + 2 * e + 1]);
+                    for (int e = 0; e < 16; ++e) w[e] = pack2(S[q * 16 + e]);
                     tmem_st16(tmem + kTmS + tm_lane + kCols / 2 * hf + 16 * q, w);
                 }
                 tmem_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_s);
-            };
-            if (it.chunks > 0) publish(gc);
-            for (int c = 0; c < it.chunks; ++c, ++gc) {
-                mbar_wait(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                const float eg = gate_buf(gc)[192];
+                if (lane == 0) mbar_arrive(&bar_sgo[gc & 1]);
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
+                const float eg = gate_buf(gc)[256];
+                const f2 eg2 = pk(eg, eg);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
-                mbar_wait(bar_d, gc & 1, abort_flag);
+                mbar_wait_short(bar_d, gc & 1, abort_flag);
                 tc_fence_after_sync();
 #pragma unroll
-                for (int q = 0; q < kCols / 32; ++q) {
-                    uint32_t r[32];
-                    tmem_ld32(tmem + kTmD + tm_lane + kCols * hf + 32 * q, r);
+                for (int q = 0; q < kCols / 16; ++q) {  // (16 columns at a time: with 32 the state would not fit the registers)
+                    uint32_t r[16];
+                    tmem_ld16(tmem + kTmD + tm_lane + kCols * hf + 16 * q, r);
                     tmem_wait_ld();
-                    if (q == kCols / 32 - 1) {
+                    if (q == kCols / 16 - 1) {
                         tc_fence_before_sync();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(bar_dfree);
+                        if (lane == 0) mbar_arrive(&bar_dgo[(gc + 1) & 1]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) S[32 * q + e] = fmaf(S[32 * q + e], eg, __uint_as_float(r[e]));
+                    for (int e = 0; e < 8; ++e) S[8 * q + e] = fma2(S[8 * q + e], eg2, pk(r[2 * e], r[2 * e + 1]));
                 }
-                if (c + 1 < it.chunks) publish(gc + 1);
             }
             // ---- the state behind the sequence
-            if (it.segment == it.segments - 1 && p.state_out && row_in && *abort_flag == 0) {
+            if (it.segment == it.segments - 1 && p.state_out && row_in && *static_cast<volatile int*>(abort_flag) == 0) {
                 const long long at = it.seq * p.so_ss + it.head * p.so_sh + static_cast<long long>(row) * p.dk + c0;
                 if (p.state_f32) {
                     float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.state_out) + at);
 #pragma unroll
-                    for (int q = 0; q < kCols / 4; ++q)
-                        if (c0 + 4 * q < p.dk) dst[q] = make_float4(S[4 * q], S[4 * q + 1], S[4 * q + 2], S[4 * q + 3]);
+                    for (int q = 0; q < kCols / 4; ++q) {
+                        float4 v;
+                        unpk(S[2 * q], v.x, v.y);
+                        unpk(S[2 * q + 1], v.z, v.w);
+                        if (c0 + 4 * q < p.dk) dst[q] = v;
+                    }
                 } else {
                     uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.state_out) + at);
 #pragma unroll
                     for (int q = 0; q < kCols / 8; ++q)
-                        if (c0 + 8 * q < p.dk)
-                            dst[q] = make_uint4(pack_bf16(S[8 * q], S[8 * q + 1]), pack_bf16(S[8 * q + 2], S[8 * q + 3]),
-                                                pack_bf16(S[8 * q + 4], S[8 * q + 5]), pack_bf16(S[8 * q + 6], S[8 * q + 7]));
+                        if (c0 + 8 * q < p.dk) dst[q] = make_uint4(pack2(S[4 * q]), pack2(S[4 * q + 1]), pack2(S[4 * q + 2]), pack2(S[4 * q + 3]));
                 }
             }
         }
@@ -349,22 +392,26 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         const bool packed = p.cu_seqlens != nullptr;
         uint8_t* const sO = smem + L::kOffO;
         const uint32_t sOa = smem_u32(sO);
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x) {
-            if (!walker.locate(p, i, it)) continue;
+        if (lane < 2) {  // (no accumulators before the first two)
+            mbar_arrive(&bar_sgo[lane]);
+            mbar_arrive(&bar_p[lane]);
+        }
+        while (next_item()) {
+#pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                const int n = static_cast<int>(min(it.tokens - static_cast<long long>(c) * kChunk, static_cast<long long>(kChunk)));
-                const float* gb = gate_buf(gc) + 128;
+                const int n = min(it.tokens - c * kChunk, kChunk);
+                const float* gb = gate_buf(gc) + 192;
                 const uint32_t tO1 = tmem + kTmO1 + 64 * (gc & 1) + tm_lane, tO2 = tmem + kTmO2 + 64 * (gc & 1) + tm_lane;
-                mbar_wait(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                mbar_wait(&bar_o[gc & 1], (gc >> 1) & 1, abort_flag);
-                tc_fence_after_sync();
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 if (otid == 0) bulk_wait_read<0>();  // the store before has finished reading the staging tile
+                mbar_wait_short(&bar_o[gc & 1], (gc >> 1) & 1, abort_flag);
+                tc_fence_after_sync();
                 named_bar_sync(1, 128);
-#pragma unroll
+#pragma unroll 1
                 for (int b = 0; b < 2; ++b) {  // 32 tokens
-                    float2 gv[4];
+                    f2 gv[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const float2*>(gb + 32 * b + 8 * j + 2 * (lane & 3));
+                    for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const f2*>(gb + 32 * b + 8 * j + 2 * (lane & 3));
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {  // 16 rows
                         uint32_t r1[16], r2[16], w[8];
@@ -372,18 +419,8 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         tmem_ld_frag32(tO1 + at, r1);
                         tmem_ld_frag32(tO2 + at, r2);
                         tmem_wait_ld();
-                        if (b == 1 && h == 1) {
-                            tc_fence_before_sync();
-                            __syncwarp();
-                            if (lane == 0) {
-                                mbar_arrive(&bar_ofree[gc & 1]);
-                                mbar_arrive(&bar_gfree[gc & 3]);
-                            }
-                        }
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            w[j] = pack_bf16(fmaf(gv[j >> 1].x, __uint_as_float(r1[2 * j]), p.scale * __uint_as_float(r2[2 * j])),
-                                             fmaf(gv[j >> 1].y, __uint_as_float(r1[2 * j + 1]), p.scale * __uint_as_float(r2[2 * j + 1])));
+                        for (int j = 0; j < 8; ++j) w[j] = pack2(fma2(gv[j >> 1], pk(r1[2 * j], r1[2 * j + 1]), pk(r2[2 * j], r2[2 * j + 1])));
                         if (DV == 128 || lq < 2) {
                             const uint32_t so = sOa + (h ? osw1 : osw0) + 4096 * b;
                             stmatrix_x4_trans(so, w[0], w[1], w[2], w[3]);
@@ -391,22 +428,30 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         }
                     }
                 }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&bar_sgo[gc & 1]);
+                    mbar_arrive(&bar_p[gc & 1]);
+                    mbar_arrive(&bar_gfree[gc & 3]);
+                }
                 fence_proxy_async_smem();
                 named_bar_sync(1, 128);
-                const long long tok0 = it.tok0 + static_cast<long long>(c) * kChunk;
+                const int tok0 = it.tok0 + c * kChunk;
                 const int left = p.dv - it.dvt * 128;  // columns from this tile on
-                if (*abort_flag != 0) {
+                if (*static_cast<volatile int*>(abort_flag) != 0) {
                     // a wait has given up: the tile is garbage and stays on chip
                 } else if (!packed || n == kChunk) {
                     if (otid == 0) {
 #pragma unroll
                         for (int a = 0; a < DV / 64; ++a)  // columns past dv and tokens past the end are clipped
-                            if (64 * a < left) tma_store_4d(&tmO, sO + 8192 * a, it.dvt * 128 + 64 * a, it.head, static_cast<int>(tok0), it.batch);
+                            if (64 * a < left) tma_store_4d(&tmO, sO + 8192 * a, it.dvt * 128 + 64 * a, it.head, tok0, it.batch);
                         bulk_commit();
                     }
                 } else {  // a whole box would reach into the next sequence
                     __nv_bfloat16* base = p.out.ptr + it.batch * p.out.sb + tok0 * p.out.st + static_cast<long long>(it.head) * p.out.sh + it.dvt * 128;
                     const int pieces = min(left, DV) >> 3;
+#pragma unroll 1
                     for (int idx = otid; idx < n * 16; idx += 128) {
                         const int row = idx >> 4, c16 = idx & 15;
                         if (c16 < pieces) *reinterpret_cast<uint4*>(base + row * p.out.st + c16 * 8) = *reinterpret_cast<const uint4*>(sO + tile_off(row, c16));
@@ -417,63 +462,45 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         if (otid == 0) bulk_wait_read<0>();
     } else if (warp < 16) {
         // =============================================================== score warps
-        const int lq = warp & 3, stid = tid - 384;
-        const bool packed = p.cu_seqlens != nullptr;
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x) {
-            if (!walker.locate(p, i, it)) continue;
+        // Row i = 16 lq + l/4 (+ 8), eight columns at a time.  Left of the diagonal blocks the decay is a product of two factors, both at most
+        // one: e^{G_i - G_r} (one per row and block; the scale goes with it) and e^{G_r - G_j} (one per column), r the block's last token.
+        const int lq = warp & 3;
+        const int i0 = 16 * lq + (lane >> 2);
+        while (next_item()) {
+#pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                const int n = static_cast<int>(min(it.tokens - static_cast<long long>(c) * kChunk, static_cast<long long>(kChunk)));
-                const uint32_t s = gc % kStages, sp = (gc / kStages) & 1;
-                uint8_t* stage = smem + s * L::kStage;
                 const float* gb = gate_buf(gc);
-                mbar_wait(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                mbar_wait(&bar_qk[s], sp, abort_flag);
-                // ---- decayed K (rounded to bf16 as an operand)
-                mbar_wait(&bar_ktfree[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
-                uint8_t* kt = smem + L::kOffKT + (gc & 1) * L::kTileK;
-#pragma unroll
-                for (int u = 0; u < L::kTileK / 16 / 128; ++u) {
-                    const int at = stid + 128 * u, row = (at & 511) >> 3;
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + L::kOffK + at * 16);
-                    *reinterpret_cast<uint4*>(kt + at * 16) = row < n ? scale8(v, gb[64 + row]) : make_uint4(0u, 0u, 0u, 0u);
-                }
-                if (packed && n < kChunk) {  // rows of the next sequence meet zeros, but zero times its NaN is one
-                    mbar_wait(&bar_v[s], sp, abort_flag);
-                    for (int at = n * (DV / 8) + stid; at < kChunk * (DV / 8); at += 128)
-                        *reinterpret_cast<uint4*>(stage + L::kOffV + (at % (DV / 64)) * 8192 + at / (DV / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_kt[gc & 1]);
-                // ---- scores with their decay, row i = 16 lq + l/4 (+ 8), columns j
-                float2 gj[8];
-                const int i0 = 16 * lq + (lane >> 2);
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 const float g0 = gb[i0], g1 = gb[i0 + 8];
-                mbar_wait(&bar_score[gc & 1], (gc >> 1) & 1, abort_flag);
+                mbar_wait_short(&bar_score[gc & 1], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t tP = tmem + kTmP + (static_cast<uint32_t>(32 * lq + ((gc & 1) ? 16 : 0)) << 16);
-                const uint32_t sP = smem_u32(smem + L::kOffP + (gc & 1) * 8192);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {  // 32 columns
+                const uint32_t sP = smem_u32(smem + L::kOffP + (gc & 1) * 8192) + (16 * lq + (lane & 7)) * 128;
+#pragma unroll 1
+                for (int h = 0; h <= lq >> 1; ++h) {  // 32 columns
                     uint32_t r[16], w[8];
                     tmem_ld_frag32(tP + 32 * h, r);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) gj[j] = *reinterpret_cast<const float2*>(gb + 32 * h + 8 * j + 2 * (lane & 3));
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const int col = 32 * h + 8 * j + 2 * (lane & 3);
-                        // (chosen, not multiplied by zero: what lies above the diagonal may be anything)
-                        w[j] = pack_bf16(col <= i0 ? __uint_as_float(r[4 * j]) * ex2(g0 - gj[j].x) : 0.f,
-                                         col + 1 <= i0 ? __uint_as_float(r[4 * j + 1]) * ex2(g0 - gj[j].y) : 0.f);
-                        w[4 + j] = pack_bf16(col <= i0 + 8 ? __uint_as_float(r[4 * j + 2]) * ex2(g1 - gj[j].x) : 0.f,
-                                             col + 1 <= i0 + 8 ? __uint_as_float(r[4 * j + 3]) * ex2(g1 - gj[j].y) : 0.f);
+                        const int block = 4 * h + j, col = 8 * block + 2 * (lane & 3);
+                        if (block < 2 * lq) {
+                            const float gr = gb[8 * block + 7];
+                            const float a0 = p.scale * ex2(g0 - gr), a1 = p.scale * ex2(g1 - gr);
+                            const f2 bj = *reinterpret_cast<const f2*>(gb + 64 + col);
+                            w[j] = pack2(mul2(mul2(pk(r[4 * j], r[4 * j + 1]), bj), pk(a0, a0)));
+                            w[4 + j] = pack2(mul2(mul2(pk(r[4 * j + 2], r[4 * j + 3]), bj), pk(a1, a1)));
+                        } else {  // (chosen, not multiplied by zero: what lies above the diagonal may be anything)
+                            const float2 gj = *reinterpret_cast<const float2*>(gb + col);
+                            w[j] = pack_bf16(col <= i0 ? p.scale * __uint_as_float(r[4 * j]) * ex2(g0 - gj.x) : 0.f,
+                                             col + 1 <= i0 ? p.scale * __uint_as_float(r[4 * j + 1]) * ex2(g0 - gj.y) : 0.f);
+                            w[4 + j] = pack_bf16(col <= i0 + 8 ? p.scale * __uint_as_float(r[4 * j + 2]) * ex2(g1 - gj.x) : 0.f,
+                                                 col + 1 <= i0 + 8 ? p.scale * __uint_as_float(r[4 * j + 3]) * ex2(g1 - gj.y) : 0.f);
+                        }
                     }
-#pragma unroll
-                    for (int a = 0; a < 2; ++a) {  // 8 rows; lane 8m + r: row r, columns 8 (4 h + m)
-                        const int row = 16 * lq + 8 * a + (lane & 7);
-                        stmatrix_x4(sP + row * 128 + (((4 * h + (lane >> 3)) ^ (row & 7)) << 4), w[4 * a], w[4 * a + 1], w[4 * a + 2], w[4 * a + 3]);
-                    }
+                    const uint32_t to = sP + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4);  // lane 8m + r: row r (of 8), columns 8 (4 h + m)
+                    stmatrix_x4(to, w[0], w[1], w[2], w[3]);
+                    stmatrix_x4(to + 1024, w[4], w[5], w[6], w[7]);
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
@@ -481,117 +508,203 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 if (lane == 0) mbar_arrive(&bar_p[gc & 1]);
             }
         }
+    } else if (warp < 20) {
+        // =============================================================== key warps
+        reg_dec<56>();
+        const int ktid = tid - 512;
+        const bool packed = p.cu_seqlens != nullptr;
+        while (next_item()) {
+#pragma unroll 1
+            for (int c = 0; c < it.chunks; ++c, ++gc) {
+                const int n = min(it.tokens - c * kChunk, kChunk);
+                const uint32_t s = gc % kStages;
+                uint8_t* stage = smem + s * L::kStage;
+                uint8_t* kt = smem + L::kOffKT + (gc & 1) * L::kTileK;
+                const float* w = gate_buf(gc) + 128;
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
+                mbar_wait_short(&bar_ktfree[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
+                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+#pragma unroll 4
+                for (int u = 0; u < L::kTileK / 16 / 128; ++u) {
+                    const int at = ktid + 128 * u, row = (at & 511) >> 3;
+                    const uint4 v = *reinterpret_cast<const uint4*>(stage + L::kOffK + at * 16);
+                    *reinterpret_cast<uint4*>(kt + at * 16) = scale8(v, w[row]);
+                }
+                if (packed && n < kChunk) {  // rows of the next sequence: their products are cleared, not multiplied by zero (they may be NaN)
+                    named_bar_sync(2, 128);
+#pragma unroll 1
+                    for (int at = n * (DK / 8) + ktid; at < kChunk * (DK / 8); at += 128)
+                        *reinterpret_cast<uint4*>(kt + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+                    for (int at = n * (DV / 8) + ktid; at < kChunk * (DV / 8); at += 128)
+                        *reinterpret_cast<uint4*>(stage + L::kOffV + (at % (DV / 64)) * 8192 + at / (DV / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_dgo[gc & 1]);
+            }
+        }
     } else {
         reg_dec<56>();
     }
-    if (warp == 16) {
+    if (warp == 20) {
         // =============================================================== producer
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x) {
-            if (!walker.locate(p, i, it)) continue;
-            const int khead = it.head / (p.vh / p.kh);
+        while (next_item()) {
+#pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages;
-                mbar_wait(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
+                mbar_wait_short(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
                 uint8_t* st = smem + s * L::kStage;
-                const int tok = static_cast<int>(it.tok0 + static_cast<long long>(c) * kChunk);
-                mbar_arrive_expect_tx_w(&bar_qk[s], 2 * L::kTileK);
+                const int tok = it.tok0 + c * kChunk;
+                mbar_arrive_expect_tx_w(&bar_full[s], L::kStage);
 #pragma unroll
                 for (int a = 0; a < DK / 64; ++a) {
-                    tma_load_4d_w(st + L::kOffK + a * 8192, &tmK, &bar_qk[s], a * 64, khead, tok, it.batch);
-                    tma_load_4d_w(st + L::kOffQ + a * 8192, &tmQ, &bar_qk[s], a * 64, khead, tok, it.batch);
+                    tma_load_4d_w(st + L::kOffK + a * 8192, &tmK, &bar_full[s], a * 64, it.khead, tok, it.batch);
+                    tma_load_4d_w(st + L::kOffQ + a * 8192, &tmQ, &bar_full[s], a * 64, it.khead, tok, it.batch);
                 }
-                mbar_arrive_expect_tx_w(&bar_v[s], L::kTileV);
 #pragma unroll
-                for (int a = 0; a < DV / 64; ++a) tma_load_4d_w(st + L::kOffV + a * 8192, &tmV, &bar_v[s], it.dvt * 128 + a * 64, it.head, tok, it.batch);
+                for (int a = 0; a < DV / 64; ++a) tma_load_4d_w(st + L::kOffV + a * 8192, &tmV, &bar_full[s], it.dvt * 128 + a * 64, it.head, tok, it.batch);
+                // a stage's loads are issued two chunks before their use, sooner than DRAM under load answers: L2 has them by then
+                constexpr int kLead = 4;
+                if (c + kLead < it.chunks && lane == 0) {
+                    const int ahead = tok + kLead * kChunk;
+#pragma unroll
+                    for (int a = 0; a < DK / 64; ++a) {
+                        tma_prefetch_4d(&tmK, a * 64, it.khead, ahead, it.batch);
+                        tma_prefetch_4d(&tmQ, a * 64, it.khead, ahead, it.batch);
+                    }
+#pragma unroll
+                    for (int a = 0; a < DV / 64; ++a) tma_prefetch_4d(&tmV, it.dvt * 128 + a * 64, it.head, ahead, it.batch);
+                }
+                __syncwarp();
             }
         }
-    } else if (warp == 17) {
-        // =============================================================== MMA issuer
-        constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
-        constexpr uint32_t id_d = make_idesc_bf16(128, DK, true, true);
-        constexpr uint32_t id_sq = make_idesc_bf16(128, 64, false, false);
-        constexpr uint32_t id_vp = make_idesc_bf16(128, 64, true, false);
-        // dv rows 64 .. 127 of V^T: the second atom; where a head has none the first one again (those lanes are not looked at)
-        constexpr uint32_t kLboV = DV == 128 ? 8192 : 0;
-        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
-        const uint64_t dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), kLboV, 1024);
-        const uint64_t dKT = make_smem_desc_sw128(smem_u32(smem + L::kOffKT), 8192, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
-        // Q K^T of chunk n, which the scores of the chunk wait for, goes out a chunk ahead
-        auto issue_qk = [&](uint32_t n) {
-            const uint32_t s = n % kStages;
-            mbar_wait(&bar_qk[s], (n / kStages) & 1, abort_flag);
-            tc_fence_after_sync();
-            const uint32_t tP = tmem + kTmP + ((n & 1) ? (16u << 16) : 0u);
-            const uint64_t q = desc_advance(dQ, s * L::kStage), k = desc_advance(dK, s * L::kStage);
-            mma_ss_w<false>(tP, q, k, id_qk);
-#pragma unroll
-            for (int ks = 1; ks < DK / 16; ++ks) mma_ss_w<true>(tP, desc_advance(q, kmajor_step(ks, 8192)), desc_advance(k, kmajor_step(ks, 8192)), id_qk);
-            mma_commit_w(&bar_score[n & 1]);
-        };
-        long long total = 0;  // chunks of this CTA
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x)
-            if (walker.locate(p, i, it)) total += it.chunks;
-        if (total > 0) issue_qk(0);
-        for (long long left = total; left > 0; --left, ++gc) {
-            const uint32_t s = gc % kStages, b = gc & 1;
-            // (the accumulator of chunk gc + 1 is that of gc - 1, whose scores have been written: its second product is issued)
-            if (left > 1) issue_qk(gc + 1);
-            const uint64_t v = desc_advance(dV, s * L::kStage), kt = desc_advance(dKT, b * L::kTileK), pp = desc_advance(dP, b * 8192), q = desc_advance(dQ, s * L::kStage);
-            // D = V^T (decayed K)
-            mbar_wait(&bar_v[s], (gc / kStages) & 1, abort_flag);
-            mbar_wait(&bar_kt[b], (gc >> 1) & 1, abort_flag);
-            if (gc > 0) mbar_wait(bar_dfree, (gc - 1) & 1, abort_flag);
-            tc_fence_after_sync();
-            mma_ss_w<false>(tmem + kTmD, v, kt, id_d);
-#pragma unroll
-            for (int ks = 1; ks < 4; ++ks) mma_ss_w<true>(tmem + kTmD, desc_advance(v, ks * 2048), desc_advance(kt, ks * 2048), id_d);
-            mma_commit_w(bar_d);
-            mma_commit_w(&bar_ktfree[b]);
-            // S Q^T
-            mbar_wait(bar_s, gc & 1, abort_flag);
-            if (gc > 1) mbar_wait(&bar_ofree[b], ((gc >> 1) + 1) & 1, abort_flag);
-            tc_fence_after_sync();
-            if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO1 + 64 * b, tmem + kTmS, q, id_sq);
-            else mma_ts_k64_w<false, 2>(tmem + kTmO1 + 64 * b, tmem + kTmS, q, id_sq);
-            mma_commit_w(&bar_sq);
-            // V^T P^T
-            mbar_wait(&bar_p[b], (gc >> 1) & 1, abort_flag);
-            tc_fence_after_sync();
-            mma_ss_w<false>(tmem + kTmO2 + 64 * b, v, pp, id_vp);
-#pragma unroll
-            for (int ks = 1; ks < 4; ++ks) mma_ss_w<true>(tmem + kTmO2 + 64 * b, desc_advance(v, ks * 2048), desc_advance(pp, ks * 32), id_vp);
-            mma_commit_w(&bar_o[b]);
-            mma_commit_w(&bar_empty[s]);
+        if (*static_cast<volatile int*>(abort_flag) != 0) {  // a wait has given up: the copies in flight land before the CTA goes
+            for (uint32_t n = gc > kStages ? gc - kStages : 0; n < gc; ++n) {
+                int none = 0;
+                mbar_wait_limit(&bar_full[n % kStages], (n / kStages) & 1, &none, 1ll << 28);
+            }
         }
-    } else if (warp == 18) {
-        // =============================================================== gates
-        for (long long i = blockIdx.x; i < p.num_items; i += gridDim.x) {
-            if (!walker.locate(p, i, it)) continue;
-            auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
-                const long long t = static_cast<long long>(c) * kChunk + lane;
-                a0 = p.gate.ptr && t < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t, it.head) : 0u;
-                a1 = p.gate.ptr && t + 32 < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t + 32, it.head) : 0u;
-            };
+    } else if (warp == 21 || warp == 22) {
+        // =============================================================== MMA issuers
+        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024);
+        // dv rows 64 .. 127 of V^T: the second atom; where a head has none the first one again (those lanes are not looked at)
+        const uint64_t dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), DV == 128 ? 8192 : 0, 1024);
+        // the chunks left of the item at hand, then of the next one that has any
+        auto more = [&](int left) {
+            while (left == 0) {
+                if (!next_item()) return 0;
+                left = it.chunks;
+            }
+            return left;
+        };
+        int left = more(0);
+        if (warp == 21) {
+            constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
+            constexpr uint32_t id_vp = make_idesc_bf16(128, 64, true, false);
+            const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
+            // Q K^T of a chunk goes out ahead of V^T P^T of the chunk before.  (Its accumulator is that of two chunks before, whose scores
+            // have been written: their product is issued.  So is the scores' tile then free when it is done.)
+            bool first = true;
+            uint32_t n = 0;  // chunk of the next Q K^T
+#pragma unroll 1
+            while (left > 0) {
+                const uint32_t s = n % kStages;
+                mbar_wait_short(&bar_full[s], (n / kStages) & 1, abort_flag);
+                tc_fence_after_sync();
+                const uint32_t tP = tmem + kTmP + ((n & 1) ? (16u << 16) : 0u);
+                const uint64_t q = desc_advance(dQ, s * L::kStage), k = desc_advance(dK, s * L::kStage);
+                mma_ss_k64_w<false, 2, 2>(tP, q, k, id_qk);
+                if (DK == 128) mma_ss_k64_w<true, 2, 2>(tP, desc_advance(q, 8192), desc_advance(k, 8192), id_qk);
+                mma_commit_w(&bar_score[n & 1]);
+                ++n;
+                left = more(left - 1);
+                if (first && left > 0) {
+                    first = false;
+                    continue;
+                }
+                do {  // (twice behind the last Q K^T)
+                    const uint32_t sv = gc % kStages, b = gc & 1;
+                    mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
+                    tc_fence_after_sync();
+                    mma_ss_k64_w<false, 128, 2>(tmem + kTmO2 + 64 * b, desc_advance(dV, sv * L::kStage), desc_advance(dP, b * 8192), id_vp);
+                    mma_commit_w(&bar_o[b]);
+                    mma_commit_w(&bar_empty[sv]);
+                    ++gc;
+                } while (left == 0 && gc < n);
+            }
+        } else {
+            constexpr uint32_t id_d = make_idesc_bf16(128, DK, true, true);
+            constexpr uint32_t id_sq = make_idesc_bf16(128, 64, false, false);
+            const uint64_t dKT = make_smem_desc_sw128(smem_u32(smem + L::kOffKT), 8192, 1024);
+#pragma unroll 1
+            while (left > 0) {
+                const uint32_t s = gc % kStages, b = gc & 1;
+                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
+                tc_fence_after_sync();
+                mma_ss_k64_w<false, 128, 128>(tmem + kTmD, desc_advance(dV, s * L::kStage), desc_advance(dKT, b * L::kTileK), id_d);
+                mma_commit_w(bar_d);
+                mma_commit_w(&bar_ktfree[b]);
+                mbar_wait_short(&bar_sgo[b], (gc >> 1) & 1, abort_flag);
+                tc_fence_after_sync();
+                if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO1 + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_sq);
+                else mma_ts_k64_w<false, 2>(tmem + kTmO1 + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_sq);
+                mma_commit_w(bar_sq);
+                mma_commit_w(&bar_o[b]);
+                mma_commit_w(&bar_empty[s]);
+                ++gc;
+                left = more(left - 1);
+            }
+        }
+    } else if (warp == 23) {
+        // =============================================================== items and gates
+        LinWalker walker;
+        uint32_t n = 0;
+        auto hand_out = [&]() {
+            mbar_wait_short(&bar_itemfree[n & 1], ((n >> 1) + 1) & 1, abort_flag);
+            if (lane == 0) {
+                items[n & 1] = it;
+                mbar_arrive(&bar_item[n & 1]);
+            }
+            __syncwarp();
+            ++n;
+        };
+        auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
+            const int t = c * kChunk + lane;
+            a0 = p.gate.ptr && t < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t, it.head) : 0u;
+            a1 = p.gate.ptr && t + 32 < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t + 32, it.head) : 0u;
+        };
+#pragma unroll 1
+        for (int i = blockIdx.x; i < p.num_items; i += gridDim.x) {
+            if (!walker.locate(p, i, it)) break;  // (surplus items are the last ones)
+            hand_out();
             uint32_t a0, a1;
             load(0, a0, a1);
+#pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 float g0 = lin_gate_log2(p.gate.value(a0)), g1 = lin_gate_log2(p.gate.value(a1));
                 load(c + 1, a0, a1);
                 scan64(g0, g1, lane);  // (tokens past the end have no decay: they carry the last one's sum)
                 const float last = __shfl_sync(0xffffffffu, g1, 31);
-                mbar_wait(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
+                const float r0 = __shfl_sync(0xffffffffu, g0, lane | 7), r1 = __shfl_sync(0xffffffffu, g1, lane | 7);
+                mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
                 gb[lane] = g0;
                 gb[lane + 32] = g1;
-                gb[64 + lane] = ex2(last - g0);
-                gb[96 + lane] = ex2(last - g1);
-                gb[128 + lane] = p.scale * ex2(g0);
-                gb[160 + lane] = p.scale * ex2(g1);
-                if (lane == 0) gb[192] = ex2(last);
+                gb[64 + lane] = ex2(r0 - g0);
+                gb[96 + lane] = ex2(r1 - g1);
+                gb[128 + lane] = ex2(last - g0);
+                gb[160 + lane] = ex2(last - g1);
+                gb[192 + lane] = p.scale * ex2(g0);
+                gb[224 + lane] = p.scale * ex2(g1);
+                if (lane == 0) gb[256] = ex2(last);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gate[gc & 3]);
             }
         }
+        it.chunks = -1;
+        hand_out();
     }
     tc_fence_before_sync();
     __syncthreads();

@@ -98,6 +98,20 @@ GDN_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_fl
     return mbar_wait_limit(bar, parity, abort_flag, kWaitLimitCycles);
 }
 
+// The same in a few instructions, for kernels of many roles whose waits would not all fit the instruction cache: the limit is a number of
+// polls (each takes tens of cycles at least: half a second and more).
+GDN_DEVICE bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    int left = 1 << 24;
+#pragma unroll 1
+    while (!mbar_try_wait(bar, parity)) {
+        if (*abort_flag != 0 || --left == 0) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
 // The same wait for warps that are not on a critical path: sleeps `kSleepNs` between polls so
 // that the polling does not take issue slots and shared-memory queue entries from the warps
 // that are.
@@ -569,6 +583,25 @@ GDN_DEVICE void mma_ts_k64_w(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, 
         "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], [ta], bd, %3, pt;\n\t}\n" ::"r"(d_tmem),
         "r"(a_tmem), "l"(b_desc), "r"(idesc), "n"(kAccumulateFirst ? 1 : 0), "n"(kStep16), "n"(2 * kStep16),
         "n"(3 * kStep16)
+        : "memory");
+}
+// Four K-steps (K = 64) with both operands in shared memory, descriptors advancing by `kStepA`, `kStepB` 16-byte units per step.
+template <bool kAccumulateFirst, int kStepA, int kStepB>
+GDN_DEVICE void mma_ss_k64_w(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred pe;\n\t.reg .pred pa;\n\t.reg .pred pt;\n\t.reg .b64 ad;\n\t.reg .b64 bd;\n\t"
+        "elect.sync _|pe, 0xffffffff;\n\t"
+        "setp.ne.b32 pa, %4, 0;\n\t"
+        "setp.eq.b32 pt, 0, 0;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, pa;\n\t"
+        "add.u64 ad, %1, %5;\n\tadd.u64 bd, %2, %8;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, pt;\n\t"
+        "add.u64 ad, %1, %6;\n\tadd.u64 bd, %2, %9;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, pt;\n\t"
+        "add.u64 ad, %1, %7;\n\tadd.u64 bd, %2, %10;\n\t"
+        "@pe tcgen05.mma.cta_group::1.kind::f16 [%0], ad, bd, %3, pt;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "n"(kAccumulateFirst ? 1 : 0), "n"(kStepA), "n"(2 * kStepA), "n"(3 * kStepA), "n"(kStepB),
+        "n"(2 * kStepB), "n"(3 * kStepB)
         : "memory");
 }
 GDN_DEVICE void mma_commit_w(uint64_t* bar) {
