@@ -1,25 +1,33 @@
 // Linear attention with decay over whole prompts, 64 tokens at a time.  With G the running sum of a chunk's log-decays and S the
 // state that enters it (dv x dk),
 //     O = scale * ( e^{G_i} Q S^T  +  (Q K^T .* e^{G_i - G_j}, j <= i) V )
-//     S <- e^{G_L} S + V^T (e^{G_L - G_j} K) .
-// The increment of the state does not depend on the state, so nothing but a multiplication and an addition per element
-// runs from chunk to chunk, and all products of a chunk can be issued ahead of it.
+//     S <- e^{G_L} S + (e^{G_L - G_j} V)^T K .
+// The state's increment does not depend on the state, so all products of a chunk can be issued ahead of it.  Where no decay of the chunk is
+// below 2^-64 it is a factor of the values alone,
+//     V' = e^{-G_j} V ,   O = scale e^{G_i} * ( Q S^T + (Q K^T, j <= i) V' ) ,   S <- e^{G_L} (S + V'^T K) ,
+// so that the scores only have to be cut off above the diagonal and both parts of O are one accumulation ("plain" chunks).  The factor
+// e^{G_L} is not applied either but kept as an exponent c of the whole state, which joins the factors of the chunks that follow,
+//     S = 2^c S' ,   V' = e^{-G_j} 2^{-c} V ,   O = scale e^{G_i} 2^c * ( ... ) ,
+// until it leaves 2^-64 too: S' is an accumulator in tensor memory that the increments are added to by the products themselves.  (2^64 leaves
+// 2^60 for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: it goes into the
+// scores, the rows of Q are scaled where they lie, the values come twice and the state is scaled between its read and its increment.
 //
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
 // items and chunks, handing tiles on through mbarriers:
-//   warps 0-7   state warps: the fp32 state in registers (lane = dv row, half of the columns each), its bf16 copy into tensor memory
-//   warps 8-11  output warps: both parts of O added, transposed through shared memory, stored
-//   warps 12-15 score warps: the scores with their decay as bf16 tile
-//   warps 16-19 key warps: K times e^{G_L - G_j} as bf16 tile
+//   warps 0-7   state warps: a bf16 copy of the fp32 state for the products with Q (lane = dv row, half of the columns each); its scaling
+//   warps 8-11  output warps: O scaled, transposed through shared memory, stored
+//   warps 12-15 score warps: the scores as bf16 tile
+//   warps 16-19 value warps: V^T times its factors into tensor memory
 //   warp 20     producer: tensor copies of Q, K, V into a ring of stages
-//   warp 21     issues Q K^T and V^T P^T
-//   warp 22     issues the state's products, D = V^T (decayed K) and S Q^T
+//   warp 21     issues the products of the output, V'^T P^T and S Q^T
+//   warp 22     issues the scores Q K^T and the state's increment V'^T K
 //   warp 23     finds the items; the gates' running sums and the factors made of them
-// What bounds a chunk is not the tensor pipe (900 cycles of products) but what a warp of each role needs for its part, a few hundred
-// instructions one behind the other, and how much of the roles' code the instruction cache holds: the waits are the short form and the
-// item search is one warp's (104 KB of code took 5200 cycles a chunk with both SMs of a pair at work, 2900 with one).
-// All accumulators that feed the output are transposed (128 dv rows = M): S is an A operand in tensor memory, V one read MN-major
-// from the tile as it was copied, Q and the scores are B operands.
+// All products that feed output and state are transposed (128 dv rows = M): S and V' are A operands in tensor memory; Q, K and the scores
+// are B operands.
+// What bounds a chunk is shared memory (176 KB of copies, operands and tiles at 128 bytes a cycle: 1400 cycles) and what a warp of each role
+// needs for its part, a few hundred instructions one behind the other, not the tensor pipe (900 cycles of products); HBM allows 2750 at d = 128.  The instruction cache
+// counts: the waits are the short form and the item search is one warp's (104 KB of code took 5200 cycles a chunk with both SMs of a pair at work, 2900 with one).
+// The form with decays in keys and scores throughout (240 KB a chunk, two accumulators) took 118 us where this takes XX (4 x 4096 tokens, 32 v-heads).
 #pragma once
 #include <cuda.h>
 
@@ -123,11 +131,11 @@ struct LinSmem {
     static constexpr int kStages = 3;
     static constexpr int kTileK = kChunk * DK * 2, kTileV = kChunk * DV * 2;
     static constexpr int kOffQ = 0, kOffK = kTileK, kOffV = 2 * kTileK, kStage = 2 * kTileK + kTileV;
-    static constexpr int kOffKT = kStages * kStage;    // 2 x decayed K
-    static constexpr int kOffP = kOffKT + 2 * kTileK;  // 2 x scores, 64 x 64
-    static constexpr int kOffO = kOffP + 2 * 8192;     // output staging
-    // 4 x gate factors, fp32: G[64] (log2); e^{G_r - G_j}[64], r the last token of j's eight; e^{G_L - G_j}[64]; scale e^{G_i}[64]; e^{G_L}
-    static constexpr int kOffGate = kOffO + kTileV;
+    static constexpr int kOffP = kStages * kStage;  // 2 x scores, 64 x 64
+    static constexpr int kOffO = kOffP + 2 * 8192;  // 2 x output staging
+    // 4 x gate factors, fp32: of the values [64]; of the output [64]; not plain: G[64] (log2), e^{G_i}[64]; of the state in front of its copy
+    // and behind it; 2^c behind the chunk; plain or not
+    static constexpr int kOffGate = kOffO + 2 * kTileV;
     static constexpr int kGateStride = (4 * 64 + 4) * 4;
     static constexpr int kOffBar = kOffGate + 4 * kGateStride;
     static constexpr int kBytes = kOffBar + 512 + 1024;
@@ -135,15 +143,13 @@ struct LinSmem {
 
 namespace lin {
 constexpr int kThreads = 768;  // 6 warpgroups: 2 x state, output, scores, keys, the rest
-constexpr uint32_t kTmS = 0;     // bf16 state, 64 columns
+constexpr uint32_t kTmS = 0;     // its bf16 copy, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
-constexpr uint32_t kTmD = 128;   // fp32 state increment, 128 columns
-constexpr uint32_t kTmO1 = 256;  // 2 x fp32 S Q^T, 64 columns
-constexpr uint32_t kTmO2 = 384;  // 2 x fp32 V^T P^T, 64 columns
-template <int N>
-__device__ __forceinline__ void reg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void reg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr uint32_t kTmF = 128;   // fp32 state, 128 columns
+constexpr uint32_t kTmO = 256;   // 2 x fp32 V'^T P^T + S Q^T, 64 columns
+constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: V^T), 32 columns
+constexpr uint32_t kTmVd = 448;  // 2 x bf16 (e^{G_L - G_j} V)^T of chunks that are not plain, 32 columns
+constexpr float kPlainLog2 = 64.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -214,21 +220,19 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     uint64_t* bar_full = bars;                  // [stages] Q, K, V of a stage have arrived
     uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done (both issuers)
     uint64_t* bar_gate = bar_empty + kStages;   // [4] gate factors of a chunk
-    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps
+    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps and the increments' issuer
     uint64_t* bar_score = bar_gfree + 4;        // [2] Q K^T done
-    uint64_t* bar_p = bar_score + 2;            // [2] scores written, and the accumulator of V^T P^T read two chunks before
-    uint64_t* bar_dgo = bar_p + 2;              // [2] decayed K written (rows of V past the end cleared), and the increment before read
-    uint64_t* bar_ktfree = bar_dgo + 2;         // [2] decayed K read
-    uint64_t* bar_sgo = bar_ktfree + 2;         // [2] the state is in tensor memory, and the accumulator of S Q^T read two chunks before
-    uint64_t* bar_o = bar_sgo + 2;              // [2] both parts of O done
-    uint64_t* bar_d = bar_o + 2;                // state increment done
-    uint64_t* bar_sq = bar_d + 1;               // the bf16 state has been read
-    uint64_t* bar_item = bar_sq + 1;            // [2] an item is there
+    uint64_t* bar_p = bar_score + 2;            // [2] scores and values written, and the output's accumulator read two chunks before
+    uint64_t* bar_dgo = bar_p + 2;              // [2] values written, and the state copied
+    uint64_t* bar_o = bar_dgo + 2;              // [2] O done: scores, state and values read
+    uint64_t* bar_d = bar_o + 2;                // [2] increment added: values read
+    uint64_t* bar_sgo = bar_d + 2;              // the state's copy is there
+    uint64_t* bar_item = bar_sgo + 1;           // [2] an item is there
     uint64_t* bar_itemfree = bar_item + 2;      // [2] and every warp has it
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_itemfree + 2);
     int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
     LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
-    static_assert((2 * kStages + 26) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
+    static_assert((2 * kStages + 23) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -239,20 +243,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar_gate[i], 1);
-            mbar_init(&bar_gfree[i], 12);
+            mbar_init(&bar_gfree[i], 13);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_score[i], 1);
-            mbar_init(&bar_p[i], 8);
+            mbar_init(&bar_p[i], 12);
             mbar_init(&bar_dgo[i], 12);
-            mbar_init(&bar_ktfree[i], 1);
-            mbar_init(&bar_sgo[i], 12);
-            mbar_init(&bar_o[i], 2);
+            mbar_init(&bar_o[i], 1);
+            mbar_init(&bar_d[i], 1);
             mbar_init(&bar_item[i], 1);
             mbar_init(&bar_itemfree[i], 23);
         }
-        mbar_init(bar_d, 1);
-        mbar_init(bar_sq, 1);
+        mbar_init(bar_sgo, 8);
         mbar_fence_init();
     }
     // the scores' blocks above the diagonal stay zero: nobody writes them
@@ -278,106 +280,114 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         if (lane == 0) mbar_arrive(&bar_itemfree[s]);
         return it.chunks >= 0 && *static_cast<volatile int*>(abort_flag) == 0;
     };
-    // registers of the CTA: 768 x 80; 8 warps at 104, 8 at 80, 8 at 56
-    static_assert(32 * (8 * 104 + 8 * 80 + 8 * 56) <= kThreads * 80, "register pool of the CTA");
-
     if (warp < 8) {
         // =============================================================== state warps
-        reg_inc<104>();
-        constexpr int kCols = DK / 2;  // of a thread
         const int lq = warp & 3, hf = warp >> 2;
+        constexpr int kCols = DK / 2;  // of a thread
+        const int c0 = kCols * hf;
         const uint32_t tm_lane = static_cast<uint32_t>(32 * lq) << 16;
-        f2 S[kCols / 2];
-        if (lane == 0) mbar_arrive(&bar_dgo[0]);  // (there is no increment before the first)
+        const uint32_t tF = tmem + kTmF + tm_lane + c0, tS = tmem + kTmS + tm_lane + c0 / 2;
         while (next_item()) {
             const int row = it.dvt * 128 + 32 * lq + lane;
             const bool row_in = 32 * lq + lane < DV && row < p.dv;
-            const int c0 = kCols * hf;
-            // ---- the state that enters the segment
-            if (it.segment > 0) {
-                const float4* src = reinterpret_cast<const float4*>(p.seg_state + static_cast<long long>(it.index - p.vh * p.dv_tiles) * (128 * DK) + (32 * lq + lane) * DK + c0);
+            // ---- the state that enters the segment (the increments of the item before have been read at its end)
+#pragma unroll 1
+            for (int q = 0; q < kCols; q += 16) {
+                uint32_t r[16];
+                const int cols = row_in ? p.dk - c0 - q : 0;  // columns that are there from this one on
+                if (it.segment > 0) {
+                    const uint4* src = reinterpret_cast<const uint4*>(p.seg_state + static_cast<long long>(it.index - p.vh * p.dv_tiles) * (128 * DK) + (32 * lq + lane) * DK + c0 + q);
 #pragma unroll
-                for (int q = 0; q < kCols / 4; ++q) {
-                    const float4 v = __ldcg(src + q);
-                    S[2 * q] = pk(v.x, v.y);
-                    S[2 * q + 1] = pk(v.z, v.w);
+                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = __ldcg(src + e);
+                } else if (p.state_in && p.state_f32) {
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0 + q);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = 4 * e < cols ? src[e] : make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0 + q);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint4 v = p.state_in && 8 * e < cols ? src[e] : make_uint4(0u, 0u, 0u, 0u);
+                        r[8 * e] = v.x << 16; r[8 * e + 1] = v.x & 0xFFFF0000u;
+                        r[8 * e + 2] = v.y << 16; r[8 * e + 3] = v.y & 0xFFFF0000u;
+                        r[8 * e + 4] = v.z << 16; r[8 * e + 5] = v.z & 0xFFFF0000u;
+                        r[8 * e + 6] = v.w << 16; r[8 * e + 7] = v.w & 0xFFFF0000u;
+                    }
                 }
-            } else if (p.state_in && p.state_f32) {
-                const float* src = static_cast<const float*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0;
-#pragma unroll
-                for (int q = 0; q < kCols / 4; ++q) {
-                    const float4 v = row_in && c0 + 4 * q < p.dk ? *(reinterpret_cast<const float4*>(src) + q) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    S[2 * q] = pk(v.x, v.y);
-                    S[2 * q + 1] = pk(v.z, v.w);
-                }
-            } else if (p.state_in) {
-                const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0;
-#pragma unroll
-                for (int q = 0; q < kCols / 8; ++q) {
-                    const uint4 v = row_in && c0 + 8 * q < p.dk ? *(reinterpret_cast<const uint4*>(src) + q) : make_uint4(0u, 0u, 0u, 0u);
-                    S[4 * q] = pk(bf16_lo(v.x), bf16_hi(v.x));
-                    S[4 * q + 1] = pk(bf16_lo(v.y), bf16_hi(v.y));
-                    S[4 * q + 2] = pk(bf16_lo(v.z), bf16_hi(v.z));
-                    S[4 * q + 3] = pk(bf16_lo(v.w), bf16_hi(v.w));
-                }
-            } else {
-#pragma unroll
-                for (int q = 0; q < kCols / 2; ++q) S[q] = 0ull;
+                tmem_st16(tF + q, r);
             }
-            // Chunk by chunk: the bf16 copy that the chunk reads (rounded for the product only: the state itself stays in fp32), then its increment.
+            tmem_wait_st();
+            float pow_c = 1.f;  // 2^c
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                if (gc > 0) mbar_wait_short(bar_sq, (gc - 1) & 1, abort_flag);  // the copy of the chunk before has been read
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
+                const float before = gate_buf(gc)[256], behind = gate_buf(gc)[257];
+                pow_c = gate_buf(gc)[258];
+                const bool scaled = before != 1.f || behind != 1.f;  // (a NaN is)
+                const f2 before2 = pk(before, before), behind2 = pk(behind, behind);
+                if (gc > 0) {  // the copy of the chunk before has been read, its increment added
+                    mbar_wait_short(&bar_o[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
+                    mbar_wait_short(&bar_d[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
+                }
                 tc_fence_after_sync();
+#pragma unroll 1
+                for (int q = 0; q < kCols; q += 32) {
+                    uint32_t r[32], w[16];
+                    tmem_ld32(tF + q, r);
+                    tmem_wait_ld();
+                    if (scaled) {
 #pragma unroll
-                for (int q = 0; q < kCols / 32; ++q) {
-                    uint32_t w[16];
+                        for (int e = 0; e < 16; ++e) {
+                            float x, y;
+                            const f2 v = mul2(pk(r[2 * e], r[2 * e + 1]), before2);
+                            w[e] = pack2(v);
+                            unpk(mul2(v, behind2), x, y);
+                            r[2 * e] = __float_as_uint(x);
+                            r[2 * e + 1] = __float_as_uint(y);
+                        }
+                        tmem_st16(tF + q, r);
+                        tmem_st16(tF + q + 16, r + 16);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) w[e] = pack2(S[q * 16 + e]);
-                    tmem_st16(tmem + kTmS + tm_lane + kCols / 2 * hf + 16 * q, w);
+                        for (int e = 0; e < 16; ++e) w[e] = pack2(pk(r[2 * e], r[2 * e + 1]));
+                    }
+                    tmem_st16(tS + q / 2, w);  // (rounded to bf16 as an operand: the state itself stays in fp32)
                 }
                 tmem_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_sgo[gc & 1]);
-                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                const float eg = gate_buf(gc)[256];
-                const f2 eg2 = pk(eg, eg);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
-                mbar_wait_short(bar_d, gc & 1, abort_flag);
-                tc_fence_after_sync();
-#pragma unroll
-                for (int q = 0; q < kCols / 16; ++q) {  // (16 columns at a time: with 32 the state would not fit the registers)
-                    uint32_t r[16];
-                    tmem_ld16(tmem + kTmD + tm_lane + kCols * hf + 16 * q, r);
-                    tmem_wait_ld();
-                    if (q == kCols / 16 - 1) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&bar_dgo[(gc + 1) & 1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) S[8 * q + e] = fma2(S[8 * q + e], eg2, pk(r[2 * e], r[2 * e + 1]));
+                if (lane == 0) {
+                    mbar_arrive(bar_sgo);
+                    mbar_arrive(&bar_dgo[gc & 1]);
+                    mbar_arrive(&bar_gfree[gc & 3]);
                 }
             }
             // ---- the state behind the sequence
-            if (it.segment == it.segments - 1 && p.state_out && row_in && *static_cast<volatile int*>(abort_flag) == 0) {
+            if (it.chunks > 0) mbar_wait_short(&bar_d[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
+            tc_fence_after_sync();
+            if (it.segment == it.segments - 1 && p.state_out && *static_cast<volatile int*>(abort_flag) == 0) {
                 const long long at = it.seq * p.so_ss + it.head * p.so_sh + static_cast<long long>(row) * p.dk + c0;
-                if (p.state_f32) {
-                    float4* dst = reinterpret_cast<float4*>(static_cast<float*>(p.state_out) + at);
+#pragma unroll 1
+                for (int q = 0; q < kCols; q += 16) {
+                    uint32_t r[16];
+                    tmem_ld16(tF + q, r);
+                    tmem_wait_ld();
+                    const int cols = row_in ? p.dk - c0 - q : 0;
 #pragma unroll
-                    for (int q = 0; q < kCols / 4; ++q) {
-                        float4 v;
-                        unpk(S[2 * q], v.x, v.y);
-                        unpk(S[2 * q + 1], v.z, v.w);
-                        if (c0 + 4 * q < p.dk) dst[q] = v;
+                    for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * pow_c);
+                    if (p.state_f32) {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.state_out) + at + q);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (4 * e < cols) dst[e] = *reinterpret_cast<const uint4*>(r + 4 * e);
+                    } else {
+                        uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.state_out) + at + q);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (8 * e < cols)
+                                dst[e] = make_uint4(pack2(pk(r[8 * e], r[8 * e + 1])), pack2(pk(r[8 * e + 2], r[8 * e + 3])),
+                                                    pack2(pk(r[8 * e + 4], r[8 * e + 5])), pack2(pk(r[8 * e + 6], r[8 * e + 7])));
                     }
-                } else {
-                    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.state_out) + at);
-#pragma unroll
-                    for (int q = 0; q < kCols / 8; ++q)
-                        if (c0 + 8 * q < p.dk) dst[q] = make_uint4(pack2(S[4 * q]), pack2(S[4 * q + 1]), pack2(S[4 * q + 2]), pack2(S[4 * q + 3]));
                 }
             }
         }
@@ -390,52 +400,43 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         const uint32_t ochunk = static_cast<uint32_t>(4 * (lq & 1) + ((lane >> 3) & 1));
         const uint32_t osw0 = olane + ((ochunk ^ (lane & 7)) << 4), osw1 = olane + (((ochunk + 2) ^ (lane & 7)) << 4);
         const bool packed = p.cu_seqlens != nullptr;
-        uint8_t* const sO = smem + L::kOffO;
-        const uint32_t sOa = smem_u32(sO);
-        if (lane < 2) {  // (no accumulators before the first two)
-            mbar_arrive(&bar_sgo[lane]);
-            mbar_arrive(&bar_p[lane]);
-        }
+        if (lane < 2) mbar_arrive(&bar_p[lane]);  // (no accumulators before the first two)
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const int n = min(it.tokens - c * kChunk, kChunk);
-                const float* gb = gate_buf(gc) + 192;
-                const uint32_t tO1 = tmem + kTmO1 + 64 * (gc & 1) + tm_lane, tO2 = tmem + kTmO2 + 64 * (gc & 1) + tm_lane;
+                const float* gb = gate_buf(gc) + 64;
+                uint8_t* const sO = smem + L::kOffO + (gc & 1) * L::kTileV;
+                const uint32_t sOa = smem_u32(sO), tO = tmem + kTmO + 64 * (gc & 1) + tm_lane;
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                if (otid == 0) bulk_wait_read<0>();  // the store before has finished reading the staging tile
                 mbar_wait_short(&bar_o[gc & 1], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-                named_bar_sync(1, 128);
 #pragma unroll 1
-                for (int b = 0; b < 2; ++b) {  // 32 tokens
+                for (int i = 0; i < 4; ++i) {  // 16 rows, 32 tokens
+                    const int h = i & 1, b = i >> 1;
+                    uint32_t r[16], w[8];
+                    tmem_ld_frag32(tO + (static_cast<uint32_t>(16 * h) << 16) + 32 * b, r);
                     f2 gv[4];
 #pragma unroll
                     for (int j = 0; j < 4; ++j) gv[j] = *reinterpret_cast<const f2*>(gb + 32 * b + 8 * j + 2 * (lane & 3));
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {  // 16 rows
-                        uint32_t r1[16], r2[16], w[8];
-                        const uint32_t at = (static_cast<uint32_t>(16 * h) << 16) + 32 * b;
-                        tmem_ld_frag32(tO1 + at, r1);
-                        tmem_ld_frag32(tO2 + at, r2);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) w[j] = pack2(fma2(gv[j >> 1], pk(r1[2 * j], r1[2 * j + 1]), pk(r2[2 * j], r2[2 * j + 1])));
-                        if (DV == 128 || lq < 2) {
-                            const uint32_t so = sOa + (h ? osw1 : osw0) + 4096 * b;
-                            stmatrix_x4_trans(so, w[0], w[1], w[2], w[3]);
-                            stmatrix_x4_trans(so + 2048, w[4], w[5], w[6], w[7]);
-                        }
+                    for (int j = 0; j < 8; ++j) w[j] = pack2(mul2(gv[j >> 1], pk(r[2 * j], r[2 * j + 1])));
+                    if (DV == 128 || lq < 2) {
+                        const uint32_t so = sOa + (h ? osw1 : osw0) + 4096 * b;
+                        stmatrix_x4_trans(so, w[0], w[1], w[2], w[3]);
+                        stmatrix_x4_trans(so + 2048, w[4], w[5], w[6], w[7]);
                     }
                 }
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&bar_sgo[gc & 1]);
                     mbar_arrive(&bar_p[gc & 1]);
                     mbar_arrive(&bar_gfree[gc & 3]);
                 }
                 fence_proxy_async_smem();
+                // (a tile is written again two chunks on: the store between the two has been waited for here by then)
+                if (otid == 0) bulk_wait_read<0>();
                 named_bar_sync(1, 128);
                 const int tok0 = it.tok0 + c * kChunk;
                 const int left = p.dv - it.dvt * 128;  // columns from this tile on
@@ -462,45 +463,65 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         if (otid == 0) bulk_wait_read<0>();
     } else if (warp < 16) {
         // =============================================================== score warps
-        // Row i = 16 lq + l/4 (+ 8), eight columns at a time.  Left of the diagonal blocks the decay is a product of two factors, both at most
-        // one: e^{G_i - G_r} (one per row and block; the scale goes with it) and e^{G_r - G_j} (one per column), r the block's last token.
-        const int lq = warp & 3;
+        // Rows i = 16 lq + l/4 and + 8; columns up to the diagonal blocks, 32 at a time.
+        const int lq = warp & 3, stid = tid - 384;
         const int i0 = 16 * lq + (lane >> 2);
+        // the columns 2 (l%4), + 1 of an 8 x 8 block on the diagonal that row l/4 keeps (cut off as bits: what lies above may be anything)
+        const uint32_t keep = (2 * (lane & 3) <= (lane >> 2) ? 0xFFFFu : 0u) | (2 * (lane & 3) + 1 <= (lane >> 2) ? 0xFFFF0000u : 0u);
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                const float g0 = gb[i0], g1 = gb[i0 + 8];
+                const bool plain = gb[259] != 0.f;
+                if (gc > 1) mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the tile of two chunks before has been read
                 mbar_wait_short(&bar_score[gc & 1], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t tP = tmem + kTmP + (static_cast<uint32_t>(32 * lq + ((gc & 1) ? 16 : 0)) << 16);
                 const uint32_t sP = smem_u32(smem + L::kOffP + (gc & 1) * 8192) + (16 * lq + (lane & 7)) * 128;
 #pragma unroll 1
-                for (int h = 0; h <= lq >> 1; ++h) {  // 32 columns
+                for (int h = 0; h <= lq >> 1; ++h) {
                     uint32_t r[16], w[8];
                     tmem_ld_frag32(tP + 32 * h, r);
                     tmem_wait_ld();
+                    if (!plain) {
+                        const float g0 = gb[128 + i0], g1 = gb[128 + i0 + 8];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int block = 4 * h + j, col = 8 * block + 2 * (lane & 3);
-                        if (block < 2 * lq) {
-                            const float gr = gb[8 * block + 7];
-                            const float a0 = p.scale * ex2(g0 - gr), a1 = p.scale * ex2(g1 - gr);
-                            const f2 bj = *reinterpret_cast<const f2*>(gb + 64 + col);
-                            w[j] = pack2(mul2(mul2(pk(r[4 * j], r[4 * j + 1]), bj), pk(a0, a0)));
-                            w[4 + j] = pack2(mul2(mul2(pk(r[4 * j + 2], r[4 * j + 3]), bj), pk(a1, a1)));
-                        } else {  // (chosen, not multiplied by zero: what lies above the diagonal may be anything)
-                            const float2 gj = *reinterpret_cast<const float2*>(gb + col);
-                            w[j] = pack_bf16(col <= i0 ? p.scale * __uint_as_float(r[4 * j]) * ex2(g0 - gj.x) : 0.f,
-                                             col + 1 <= i0 ? p.scale * __uint_as_float(r[4 * j + 1]) * ex2(g0 - gj.y) : 0.f);
-                            w[4 + j] = pack_bf16(col <= i0 + 8 ? p.scale * __uint_as_float(r[4 * j + 2]) * ex2(g1 - gj.x) : 0.f,
-                                                 col + 1 <= i0 + 8 ? p.scale * __uint_as_float(r[4 * j + 3]) * ex2(g1 - gj.y) : 0.f);
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 gj = *reinterpret_cast<const float2*>(gb + 128 + 32 * h + 8 * j + 2 * (lane & 3));
+                            r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) * ex2(g0 - gj.x));
+                            r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) * ex2(g0 - gj.y));
+                            r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) * ex2(g1 - gj.x));
+                            r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) * ex2(g1 - gj.y));
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {  // (rounded to bf16 as an operand)
+                        w[j] = pack2(pk(r[4 * j], r[4 * j + 1]));
+                        w[4 + j] = pack2(pk(r[4 * j + 2], r[4 * j + 3]));
+                    }
+                    if (h == lq >> 1) {  // the diagonal blocks and what is above them
+                        if (lq & 1) {
+                            w[2] &= keep;
+                            w[3] = 0u;
+                            w[7] &= keep;
+                        } else {
+                            w[0] &= keep;
+                            w[5] &= keep;
+                            w[1] = w[2] = w[3] = w[6] = w[7] = 0u;
                         }
                     }
                     const uint32_t to = sP + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4);  // lane 8m + r: row r (of 8), columns 8 (4 h + m)
                     stmatrix_x4(to, w[0], w[1], w[2], w[3]);
                     stmatrix_x4(to + 1024, w[4], w[5], w[6], w[7]);
+                }
+                if (!plain) {  // Q, which Q K^T has been through with, takes its decay where it lies
+                    const uint32_t s = gc % kStages;
+                    mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                    uint8_t* q = smem + s * L::kStage + L::kOffQ;
+#pragma unroll 1
+                    for (int at = stid; at < L::kTileK / 16; at += 128)
+                        *reinterpret_cast<uint4*>(q + at * 16) = scale8(*reinterpret_cast<const uint4*>(q + at * 16), gb[192 + ((at & 511) >> 3)]);
                 }
                 fence_proxy_async_smem();
                 tc_fence_before_sync();
@@ -509,9 +530,14 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             }
         }
     } else if (warp < 20) {
-        // =============================================================== key warps
-        reg_dec<56>();
-        const int ktid = tid - 512;
+        // =============================================================== value warps
+        // V^T comes by transposing matrix loads: lane 8m + r addresses token r of block m (8 rows x 8 tokens), block m = rows 8 (m & 1) ..
+        // of 16, tokens 8 (m >> 1) .. of 16.
+        const int lq = warp & 3, vtid = tid - 512;
+        const uint32_t tm_lane = static_cast<uint32_t>(32 * lq) << 16;
+        const uint32_t vlane = static_cast<uint32_t>((lq >> 1) * 8192 + (8 * (lane >> 4) + (lane & 7)) * 128);
+        const uint32_t vchunk = static_cast<uint32_t>(4 * (lq & 1) + ((lane >> 3) & 1));  // 16-byte piece of the first 16 rows
+        const uint32_t vsw0 = vlane + ((vchunk ^ (lane & 7)) << 4), vsw1 = vlane + (((vchunk + 2) ^ (lane & 7)) << 4);
         const bool packed = p.cu_seqlens != nullptr;
         while (next_item()) {
 #pragma unroll 1
@@ -519,35 +545,72 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 const int n = min(it.tokens - c * kChunk, kChunk);
                 const uint32_t s = gc % kStages;
                 uint8_t* stage = smem + s * L::kStage;
-                uint8_t* kt = smem + L::kOffKT + (gc & 1) * L::kTileK;
-                const float* w = gate_buf(gc) + 128;
+                const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                mbar_wait_short(&bar_ktfree[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
+                if (gc > 1) {
+                    mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
+                    mbar_wait_short(&bar_d[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
+                }
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
-#pragma unroll 4
-                for (int u = 0; u < L::kTileK / 16 / 128; ++u) {
-                    const int at = ktid + 128 * u, row = (at & 511) >> 3;
-                    const uint4 v = *reinterpret_cast<const uint4*>(stage + L::kOffK + at * 16);
-                    *reinterpret_cast<uint4*>(kt + at * 16) = scale8(v, w[row]);
-                }
-                if (packed && n < kChunk) {  // rows of the next sequence: their products are cleared, not multiplied by zero (they may be NaN)
-                    named_bar_sync(2, 128);
+                tc_fence_after_sync();
+                const bool plain = gb[259] != 0.f;
+                const uint32_t sV = smem_u32(stage + L::kOffV);
+                if (DV == 128 || lq < 2) {
 #pragma unroll 1
-                    for (int at = n * (DK / 8) + ktid; at < kChunk * (DK / 8); at += 128)
-                        *reinterpret_cast<uint4*>(kt + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 1
-                    for (int at = n * (DV / 8) + ktid; at < kChunk * (DV / 8); at += 128)
-                        *reinterpret_cast<uint4*>(stage + L::kOffV + (at % (DV / 64)) * 8192 + at / (DV / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    for (int hf = 0; hf < 2; ++hf) {  // 32 tokens
+                        const int t0 = 32 * hf + 2 * (lane & 3);  // first token of this lane's first pair; the others are 8 further on each
+                        uint32_t v[2][2][4];  // [16 rows][16 tokens][block]
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            ldmatrix_x4_trans(sV + vsw0 + 4096 * hf + 2048 * j, v[0][j]);
+                            ldmatrix_x4_trans(sV + vsw1 + 4096 * hf + 2048 * j, v[1][j]);
+                        }
+                        if (n < kChunk) {  // tokens past the end (of the next sequence, maybe)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t keep = (t0 + 8 * i < n ? 0xFFFFu : 0u) | (t0 + 8 * i + 1 < n ? 0xFFFF0000u : 0u);
+#pragma unroll
+                                for (int a = 0; a < 2; ++a) {
+                                    v[0][i >> 1][2 * (i & 1) + a] &= keep;
+                                    v[1][i >> 1][2 * (i & 1) + a] &= keep;
+                                }
+                            }
+                        }
+                        const uint32_t to = tmem + tm_lane + 32 * (gc & 1) + 16 * hf;
+                        if (!plain) {
+                            tmem_st_frag16(to + kTmV, v[0][0]);
+                            tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f2 f = *reinterpret_cast<const f2*>(gb + t0 + 8 * i);
+#pragma unroll
+                            for (int a = 0; a < 2; ++a) {
+                                uint32_t &x = v[0][i >> 1][2 * (i & 1) + a], &y = v[1][i >> 1][2 * (i & 1) + a];
+                                x = pack2(mul2(pk(bf16_lo(x), bf16_hi(x)), f));  // (rounded to bf16 as an operand)
+                                y = pack2(mul2(pk(bf16_lo(y), bf16_hi(y)), f));
+                            }
+                        }
+                        tmem_st_frag16(to + (plain ? kTmV : kTmVd), v[0][0]);
+                        tmem_st_frag16(to + (plain ? kTmV : kTmVd) + (16u << 16), v[1][0]);
+                    }
                 }
-                fence_proxy_async_smem();
+                if (packed && n < kChunk) {  // keys of the next sequence meet zero values, but zero times their NaN is one
+#pragma unroll 1
+                    for (int at = n * (DK / 8) + vtid; at < kChunk * (DK / 8); at += 128)
+                        *reinterpret_cast<uint4*>(stage + L::kOffK + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    fence_proxy_async_smem();
+                }
+                tmem_wait_st();
+                tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bar_dgo[gc & 1]);
+                if (lane == 0) {
+                    mbar_arrive(&bar_dgo[gc & 1]);
+                    mbar_arrive(&bar_p[gc & 1]);
+                }
             }
         }
-    } else {
-        reg_dec<56>();
-    }
-    if (warp == 20) {
+    } else if (warp == 20) {
         // =============================================================== producer
         while (next_item()) {
 #pragma unroll 1
@@ -587,9 +650,6 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
     } else if (warp == 21 || warp == 22) {
         // =============================================================== MMA issuers
-        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024);
-        // dv rows 64 .. 127 of V^T: the second atom; where a head has none the first one again (those lanes are not looked at)
-        const uint64_t dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), DV == 128 ? 8192 : 0, 1024);
         // the chunks left of the item at hand, then of the next one that has any
         auto more = [&](int left) {
             while (left == 0) {
@@ -600,23 +660,42 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         };
         int left = more(0);
         if (warp == 21) {
-            constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
-            constexpr uint32_t id_vp = make_idesc_bf16(128, 64, true, false);
-            const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
-            // Q K^T of a chunk goes out ahead of V^T P^T of the chunk before.  (Its accumulator is that of two chunks before, whose scores
-            // have been written: their product is issued.  So is the scores' tile then free when it is done.)
-            bool first = true;
-            uint32_t n = 0;  // chunk of the next Q K^T
+            constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, false);
+            const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
 #pragma unroll 1
             while (left > 0) {
-                const uint32_t s = n % kStages;
-                mbar_wait_short(&bar_full[s], (n / kStages) & 1, abort_flag);
+                const uint32_t s = gc % kStages, b = gc & 1;
+                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-                const uint32_t tP = tmem + kTmP + ((n & 1) ? (16u << 16) : 0u);
+                mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmV + 32 * b, desc_advance(dP, b * 8192), id_o);
+                mbar_wait_short(bar_sgo, gc & 1, abort_flag);
+                tc_fence_after_sync();
+                if (DK == 128) mma_ts_k128_w<true>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
+                else mma_ts_k64_w<true, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
+                mma_commit_w(&bar_o[b]);
+                mma_commit_w(&bar_empty[s]);
+                ++gc;
+                left = more(left - 1);
+            }
+        } else {
+            constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
+            constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true);
+            const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
+            const uint64_t dKm = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024);  // read MN-major
+            bool first = true;
+            uint32_t n = 0;  // chunk of the next Q K^T, which goes out ahead of the increment of the chunk before
+#pragma unroll 1
+            while (left > 0) {
+                const uint32_t s = n % kStages, bn = n & 1;
+                mbar_wait_short(&bar_full[s], (n / kStages) & 1, abort_flag);
+                if (n > 1) mbar_wait_short(&bar_p[bn], ((n >> 1) + 1) & 1, abort_flag);  // the scores of two chunks before have been read
+                tc_fence_after_sync();
+                const uint32_t tP = tmem + kTmP + (bn ? (16u << 16) : 0u);
                 const uint64_t q = desc_advance(dQ, s * L::kStage), k = desc_advance(dK, s * L::kStage);
                 mma_ss_k64_w<false, 2, 2>(tP, q, k, id_qk);
                 if (DK == 128) mma_ss_k64_w<true, 2, 2>(tP, desc_advance(q, 8192), desc_advance(k, 8192), id_qk);
-                mma_commit_w(&bar_score[n & 1]);
+                mma_commit_w(&bar_score[bn]);
                 ++n;
                 left = more(left - 1);
                 if (first && left > 0) {
@@ -624,37 +703,17 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     continue;
                 }
                 do {  // (twice behind the last Q K^T)
-                    const uint32_t sv = gc % kStages, b = gc & 1;
-                    mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
+                    const uint32_t sd = gc % kStages, b = gc & 1;
+                    mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
                     tc_fence_after_sync();
-                    mma_ss_k64_w<false, 128, 2>(tmem + kTmO2 + 64 * b, desc_advance(dV, sv * L::kStage), desc_advance(dP, b * 8192), id_vp);
-                    mma_commit_w(&bar_o[b]);
-                    mma_commit_w(&bar_empty[sv]);
+                    const bool plain = gate_buf(gc)[259] != 0.f;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
+                    mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + (plain ? kTmV : kTmVd) + 32 * b, desc_advance(dKm, sd * L::kStage), id_d);
+                    mma_commit_w(&bar_d[b]);
+                    mma_commit_w(&bar_empty[sd]);
                     ++gc;
                 } while (left == 0 && gc < n);
-            }
-        } else {
-            constexpr uint32_t id_d = make_idesc_bf16(128, DK, true, true);
-            constexpr uint32_t id_sq = make_idesc_bf16(128, 64, false, false);
-            const uint64_t dKT = make_smem_desc_sw128(smem_u32(smem + L::kOffKT), 8192, 1024);
-#pragma unroll 1
-            while (left > 0) {
-                const uint32_t s = gc % kStages, b = gc & 1;
-                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
-                mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
-                tc_fence_after_sync();
-                mma_ss_k64_w<false, 128, 128>(tmem + kTmD, desc_advance(dV, s * L::kStage), desc_advance(dKT, b * L::kTileK), id_d);
-                mma_commit_w(bar_d);
-                mma_commit_w(&bar_ktfree[b]);
-                mbar_wait_short(&bar_sgo[b], (gc >> 1) & 1, abort_flag);
-                tc_fence_after_sync();
-                if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO1 + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_sq);
-                else mma_ts_k64_w<false, 2>(tmem + kTmO1 + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_sq);
-                mma_commit_w(bar_sq);
-                mma_commit_w(&bar_o[b]);
-                mma_commit_w(&bar_empty[s]);
-                ++gc;
-                left = more(left - 1);
             }
         }
     } else if (warp == 23) {
@@ -680,6 +739,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             if (!walker.locate(p, i, it)) break;  // (surplus items are the last ones)
             hand_out();
             uint32_t a0, a1;
+            float expo = 0.f;  // c
             load(0, a0, a1);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
@@ -687,18 +747,36 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 load(c + 1, a0, a1);
                 scan64(g0, g1, lane);  // (tokens past the end have no decay: they carry the last one's sum)
                 const float last = __shfl_sync(0xffffffffu, g1, 31);
-                const float r0 = __shfl_sync(0xffffffffu, g0, lane | 7), r1 = __shfl_sync(0xffffffffu, g1, lane | 7);
+                // (a NaN is not plain, neither are gates that grow)
+                auto within = [&](float c) { return __all_sync(0xffffffffu, fabsf(g0 + c) <= kPlainLog2 && fabsf(g1 + c) <= kPlainLog2); };
+                float before = 1.f, behind = 1.f;
+                bool plain = within(expo);
+                if (!plain) {  // the state takes its exponent
+                    before = ex2(expo);
+                    expo = 0.f;
+                    plain = within(0.f);
+                }
                 mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
-                gb[lane] = g0;
-                gb[lane + 32] = g1;
-                gb[64 + lane] = ex2(r0 - g0);
-                gb[96 + lane] = ex2(r1 - g1);
-                gb[128 + lane] = ex2(last - g0);
-                gb[160 + lane] = ex2(last - g1);
-                gb[192 + lane] = p.scale * ex2(g0);
-                gb[224 + lane] = p.scale * ex2(g1);
-                if (lane == 0) gb[256] = ex2(last);
+                if (plain) {
+                    g0 += expo;
+                    g1 += expo;
+                    gb[lane] = ex2(-g0);
+                    gb[lane + 32] = ex2(-g1);
+                    gb[64 + lane] = p.scale * ex2(g0);
+                    gb[96 + lane] = p.scale * ex2(g1);
+                    expo += last;
+                } else {
+                    behind = ex2(last);
+                    gb[lane] = ex2(last - g0);
+                    gb[lane + 32] = ex2(last - g1);
+                    gb[64 + lane] = gb[96 + lane] = p.scale;
+                    gb[128 + lane] = g0;
+                    gb[160 + lane] = g1;
+                    gb[192 + lane] = ex2(g0);
+                    gb[224 + lane] = ex2(g1);
+                }
+                if (lane == 0) *reinterpret_cast<float4*>(gb + 256) = make_float4(before, behind, ex2(expo), plain ? 1.f : 0.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gate[gc & 3]);
             }

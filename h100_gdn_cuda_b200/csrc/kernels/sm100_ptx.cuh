@@ -98,12 +98,24 @@ GDN_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_fl
     return mbar_wait_limit(bar, parity, abort_flag, kWaitLimitCycles);
 }
 
-// The same in a few instructions, for kernels of many roles whose waits would not all fit the instruction cache: the limit is a number of
-// polls (each takes tens of cycles at least: half a second and more).
+// The same in a few instructions, for kernels of many roles whose waits would not all fit the instruction cache.  The hardware is asked to
+// keep the warp suspended for up to 4 us a poll: two dozen warps that poll in a loop take half of an SM's issue slots from the ones that work.  The
+// limit is a number of polls, four seconds where they last that long.
+GDN_DEVICE bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 4000;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 GDN_DEVICE bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    int left = 1 << 24;
+    int left = 1 << 20;
 #pragma unroll 1
-    while (!mbar_try_wait(bar, parity)) {
+    while (!mbar_try_wait_long(bar, parity)) {
         if (*abort_flag != 0 || --left == 0) {
             *abort_flag = 1;
             return false;
