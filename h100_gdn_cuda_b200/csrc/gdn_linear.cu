@@ -34,21 +34,36 @@ int launch_linear_recurrent(const LinRecurrentParams& p, cudaStream_t st) {
     return GDN_OK;
 }
 
-// Tensor map of a token tensor; an axis of one token or head may come with any stride, the map wants a positive one.
-int linear_map(CUtensorMap* out, GdnTokenTensor t, const GdnShape& s, int heads, int dim, const char* name) {
+// Tensor map of a token tensor; an axis of one token or head may come with any stride, the map wants a positive one.  `columns` > 0: of rank 5,
+// (64 columns, tokens, column blocks, heads, batch), for boxes of `columns` columns and 64 tokens; otherwise as make_token_map has it.
+int linear_map(CUtensorMap* out, GdnTokenTensor t, const GdnShape& s, int heads, int dim, const char* name, int columns = 0) {
     if (heads == 1) t.stride_head = dim;
     const int64_t tokens = s.cu_seqlens ? s.total_tokens : s.seq_len;
     if (tokens == 1) t.stride_token = std::max<int64_t>(t.stride_token, static_cast<int64_t>(heads) * t.stride_head);
-    return make_token_map(out, t, s, heads, name, dim);
+    if (columns == 0) return make_token_map(out, t, s, heads, name, dim);
+    const bool packed = s.cu_seqlens != nullptr;
+    const uint64_t batch = packed ? 1 : static_cast<uint64_t>(s.batch);
+    uint64_t sb = static_cast<uint64_t>(t.stride_batch) * 2;
+    if (packed || sb == 0) sb = std::max<uint64_t>(16, static_cast<uint64_t>(tokens * t.stride_token) * 2);
+    const uint64_t dims[5] = {64, static_cast<uint64_t>(tokens), static_cast<uint64_t>(dim / 64), static_cast<uint64_t>(heads), batch};
+    const uint64_t strides[4] = {static_cast<uint64_t>(t.stride_token) * 2, 128, static_cast<uint64_t>(t.stride_head) * 2, sb};
+    const uint32_t box[5] = {64, 64, static_cast<uint32_t>(columns / 64), 1, 1};
+    if (!make_tmap_bf16(out, t.ptr, 5, dims, strides, box, true)) return fail(GDN_ERR_CUDA, "could not encode the TMA descriptor of %s", name);
+    return GDN_OK;
 }
 
 bool wide_linear(const GdnShape& s) { return s.head_dim_k > 128; }
 
-template <int DK, int DV>
-int launch_linear_chunked(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const CUtensorMap& tmO, const LinChunkedParams& p,
-                          int sms, cudaStream_t st) {
+template <int DK, int DV, bool kWhole>
+int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, int sms, cudaStream_t st) {
     using L = LinSmem<DK, DV>;
-    if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV>>(L::kBytes)) return rc;
+    const GdnShape& s = a.shape;
+    CUtensorMap tmQ, tmK, tmV, tmO;
+    if (int rc = linear_map(&tmQ, a.q, s, s.num_k_heads, s.head_dim_k, "q", kWhole ? DK : 0)) return rc;
+    if (int rc = linear_map(&tmK, a.k, s, s.num_k_heads, s.head_dim_k, "k", kWhole ? DK : 0)) return rc;
+    if (int rc = linear_map(&tmV, a.v, s, s.num_v_heads, s.head_dim_v, "v", kWhole ? DV : 0)) return rc;
+    if (int rc = linear_map(&tmO, a.out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
+    if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV, kWhole>>(L::kBytes)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.num_items, sms)));
     cfg.blockDim = dim3(lin::kThreads);
@@ -59,7 +74,7 @@ int launch_linear_chunked(const CUtensorMap& tmQ, const CUtensorMap& tmK, const 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV>, tmQ, tmK, tmV, tmO, p));
+    GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV, kWhole>, tmQ, tmK, tmV, tmO, p));
     return GDN_OK;
 }
 
@@ -134,11 +149,6 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     GDN_REQUIRE(tokens < (1ll << 31) - kChunk, "gdn_linear_chunked: too many tokens");
     DeviceInfo* d = nullptr;
     if (int rc = get_device_info(&d)) return rc;
-    CUtensorMap tmQ, tmK, tmV, tmO;
-    if (int rc = linear_map(&tmQ, a->q, s, s.num_k_heads, s.head_dim_k, "q")) return rc;
-    if (int rc = linear_map(&tmK, a->k, s, s.num_k_heads, s.head_dim_k, "k")) return rc;
-    if (int rc = linear_map(&tmV, a->v, s, s.num_v_heads, s.head_dim_v, "v")) return rc;
-    if (int rc = linear_map(&tmO, a->out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
     LinChunkedParams p{};
     p.out = token_view(a->out);
     p.gate = scalar_view(a->gate);
@@ -157,9 +167,12 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     GDN_REQUIRE(items < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
     p.num_items = static_cast<int>(items);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.dk <= 64)
-        return p.dv <= 64 ? launch_linear_chunked<64, 64>(tmQ, tmK, tmV, tmO, p, d->sms, st) : launch_linear_chunked<64, 128>(tmQ, tmK, tmV, tmO, p, d->sms, st);
-    return p.dv <= 64 ? launch_linear_chunked<128, 64>(tmQ, tmK, tmV, tmO, p, d->sms, st) : launch_linear_chunked<128, 128>(tmQ, tmK, tmV, tmO, p, d->sms, st);
+    // (a single column block needs no rank 5: its map clips what is missing)
+    const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);
+    if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false>(*a, p, d->sms, st);
+    if (p.dk <= 64) return launch_linear_chunked<64, 128, false>(*a, p, d->sms, st);
+    if (p.dv <= 64) return launch_linear_chunked<128, 64, false>(*a, p, d->sms, st);
+    return whole ? launch_linear_chunked<128, 128, true>(*a, p, d->sms, st) : launch_linear_chunked<128, 128, false>(*a, p, d->sms, st);
 }
 
 }  // extern "C"

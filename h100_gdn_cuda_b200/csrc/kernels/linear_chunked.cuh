@@ -20,8 +20,9 @@
 //   warps 16-19 value warps: V^T times its factors into tensor memory
 //   warp 20     producer: tensor copies of Q, K, V into a ring of stages
 //   warp 21     issues the products of the output, V'^T P^T and S Q^T
-//   warp 22     issues the scores Q K^T and the state's increment V'^T K
+//   warp 22     issues the state's increment V'^T K
 //   warp 23     finds the items; the gates' running sums and the factors made of them
+//   warp 24     issues the scores Q K^T
 // All products that feed output and state are transposed (128 dv rows = M): S and V' are A operands in tensor memory; Q, K and the scores
 // are B operands.
 // What bounds a chunk is shared memory (176 KB of copies, operands and tiles at 128 bytes a cycle: 1400 cycles) and what a warp of each role
@@ -142,7 +143,7 @@ struct LinSmem {
 };
 
 namespace lin {
-constexpr int kThreads = 768;  // 6 warpgroups: 2 x state, output, scores, keys, the rest
+constexpr int kThreads = 800;  // 25 warps
 constexpr uint32_t kTmS = 0;     // its bf16 copy, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
 constexpr uint32_t kTmF = 128;   // fp32 state, 128 columns
@@ -204,7 +205,9 @@ __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
 }
 }  // namespace lin
 
-template <int DK, int DV>
+// kWhole: head dims are multiples of 64, so that one copy fetches all columns of a tile (maps of rank 5: 64 columns, tokens, column blocks, heads,
+// batch); otherwise every 64 columns are a copy of their own, which leaves out the columns that the next head begins with.
+template <int DK, int DV, bool kWhole>
 __global__ void __launch_bounds__(lin::kThreads, 1)
     gdn_linear_chunked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const LinChunkedParams p) {
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
     static_assert((2 * kStages + 23) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         *abort_flag = 0;
         for (int i = 0; i < kStages; ++i) {
@@ -252,7 +255,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             mbar_init(&bar_o[i], 1);
             mbar_init(&bar_d[i], 1);
             mbar_init(&bar_item[i], 1);
-            mbar_init(&bar_itemfree[i], 23);
+            mbar_init(&bar_itemfree[i], 24);
         }
         mbar_init(bar_sgo, 8);
         mbar_fence_init();
@@ -264,7 +267,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     grid_dep_wait();
     grid_dep_launch();
 
@@ -276,9 +279,11 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         mbar_wait_short(&bar_item[s], (taken >> 1) & 1, abort_flag);
         it = items[s];
         ++taken;
-        __syncwarp();
+        // (the count by way of a shuffle, so that the compiler knows it to be the same in all lanes: loop counters, addresses and descriptors
+        // made of it then live in uniform registers)
+        it.chunks = __shfl_sync(0xffffffffu, *static_cast<volatile int*>(abort_flag) == 0 ? it.chunks : -1, 0);
         if (lane == 0) mbar_arrive(&bar_itemfree[s]);
-        return it.chunks >= 0 && *static_cast<volatile int*>(abort_flag) == 0;
+        return it.chunks >= 0;
     };
     if (warp < 8) {
         // =============================================================== state warps
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     uint32_t r[32], w[16];
                     tmem_ld32(tF + q, r);
                     tmem_wait_ld();
-                    if (scaled) {
+                    if (__builtin_expect(scaled, 0)) {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             float x, y;
@@ -440,9 +445,9 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 named_bar_sync(1, 128);
                 const int tok0 = it.tok0 + c * kChunk;
                 const int left = p.dv - it.dvt * 128;  // columns from this tile on
-                if (*static_cast<volatile int*>(abort_flag) != 0) {
+                if (__builtin_expect(*static_cast<volatile int*>(abort_flag) != 0, 0)) {
                     // a wait has given up: the tile is garbage and stays on chip
-                } else if (!packed || n == kChunk) {
+                } else if (__builtin_expect(!packed || n == kChunk, 1)) {
                     if (otid == 0) {
 #pragma unroll
                         for (int a = 0; a < DV / 64; ++a)  // columns past dv and tokens past the end are clipped
@@ -484,7 +489,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     uint32_t r[16], w[8];
                     tmem_ld_frag32(tP + 32 * h, r);
                     tmem_wait_ld();
-                    if (!plain) {
+                    if (__builtin_expect(!plain, 0)) {
                         const float g0 = gb[128 + i0], g1 = gb[128 + i0 + 8];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
@@ -515,7 +520,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     stmatrix_x4(to, w[0], w[1], w[2], w[3]);
                     stmatrix_x4(to + 1024, w[4], w[5], w[6], w[7]);
                 }
-                if (!plain) {  // Q, which Q K^T has been through with, takes its decay where it lies
+                if (__builtin_expect(!plain, 0)) {  // Q, which Q K^T has been through with, takes its decay where it lies
                     const uint32_t s = gc % kStages;
                     mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                     uint8_t* q = smem + s * L::kStage + L::kOffQ;
@@ -565,7 +570,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             ldmatrix_x4_trans(sV + vsw0 + 4096 * hf + 2048 * j, v[0][j]);
                             ldmatrix_x4_trans(sV + vsw1 + 4096 * hf + 2048 * j, v[1][j]);
                         }
-                        if (n < kChunk) {  // tokens past the end (of the next sequence, maybe)
+                        if (__builtin_expect(n < kChunk, 0)) {  // tokens past the end (of the next sequence, maybe)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t keep = (t0 + 8 * i < n ? 0xFFFFu : 0u) | (t0 + 8 * i + 1 < n ? 0xFFFF0000u : 0u);
@@ -577,7 +582,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             }
                         }
                         const uint32_t to = tmem + tm_lane + 32 * (gc & 1) + 16 * hf;
-                        if (!plain) {
+                        if (__builtin_expect(!plain, 0)) {
                             tmem_st_frag16(to + kTmV, v[0][0]);
                             tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
                         }
@@ -595,7 +600,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         tmem_st_frag16(to + (plain ? kTmV : kTmVd) + (16u << 16), v[1][0]);
                     }
                 }
-                if (packed && n < kChunk) {  // keys of the next sequence meet zero values, but zero times their NaN is one
+                if (__builtin_expect(packed && n < kChunk, 0)) {  // keys of the next sequence meet zero values, but zero times their NaN is one
 #pragma unroll 1
                     for (int at = n * (DK / 8) + vtid; at < kChunk * (DK / 8); at += 128)
                         *reinterpret_cast<uint4*>(stage + L::kOffK + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -612,32 +617,45 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
     } else if (warp == 20) {
         // =============================================================== producer
+        // A stage's loads are issued two chunks before their use, sooner than DRAM under load answers: they are asked for kLead chunks ahead, so
+        // that L2 has them by then.
+        constexpr int kLead = 4;
         while (next_item()) {
+            const int khead = __shfl_sync(0xffffffffu, it.khead, 0), head = __shfl_sync(0xffffffffu, it.head, 0), batch = __shfl_sync(0xffffffffu, it.batch, 0);
+            const int tok0 = __shfl_sync(0xffffffffu, it.tok0, 0), dvt = __shfl_sync(0xffffffffu, it.dvt, 0);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages;
                 mbar_wait_short(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
                 uint8_t* st = smem + s * L::kStage;
-                const int tok = it.tok0 + c * kChunk;
-                mbar_arrive_expect_tx_w(&bar_full[s], L::kStage);
-#pragma unroll
-                for (int a = 0; a < DK / 64; ++a) {
-                    tma_load_4d_w(st + L::kOffK + a * 8192, &tmK, &bar_full[s], a * 64, it.khead, tok, it.batch);
-                    tma_load_4d_w(st + L::kOffQ + a * 8192, &tmQ, &bar_full[s], a * 64, it.khead, tok, it.batch);
-                }
-#pragma unroll
-                for (int a = 0; a < DV / 64; ++a) tma_load_4d_w(st + L::kOffV + a * 8192, &tmV, &bar_full[s], it.dvt * 128 + a * 64, it.head, tok, it.batch);
-                // a stage's loads are issued two chunks before their use, sooner than DRAM under load answers: L2 has them by then
-                constexpr int kLead = 4;
-                if (c + kLead < it.chunks && lane == 0) {
-                    const int ahead = tok + kLead * kChunk;
-#pragma unroll
-                    for (int a = 0; a < DK / 64; ++a) {
-                        tma_prefetch_4d(&tmK, a * 64, it.khead, ahead, it.batch);
-                        tma_prefetch_4d(&tmQ, a * 64, it.khead, ahead, it.batch);
+                const int tok = tok0 + c * kChunk, ahead = tok + kLead * kChunk;
+                if (elect_one()) {
+                    mbar_arrive_expect_tx(&bar_full[s], L::kStage);
+                    if (kWhole) {
+                        tma_load_5d(st + L::kOffK, &tmK, &bar_full[s], 0, tok, 0, khead, batch);
+                        tma_load_5d(st + L::kOffQ, &tmQ, &bar_full[s], 0, tok, 0, khead, batch);
+                        tma_load_5d(st + L::kOffV, &tmV, &bar_full[s], 0, tok, 2 * dvt, head, batch);
+                        if (c + kLead < it.chunks) {
+                            tma_prefetch_5d(&tmK, 0, ahead, 0, khead, batch);
+                            tma_prefetch_5d(&tmQ, 0, ahead, 0, khead, batch);
+                            tma_prefetch_5d(&tmV, 0, ahead, 2 * dvt, head, batch);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int a = 0; a < DK / 64; ++a) {
+                            tma_load_4d(st + L::kOffK + a * 8192, &tmK, &bar_full[s], a * 64, khead, tok, batch);
+                            tma_load_4d(st + L::kOffQ + a * 8192, &tmQ, &bar_full[s], a * 64, khead, tok, batch);
+                            if (c + kLead < it.chunks) {
+                                tma_prefetch_4d(&tmK, a * 64, khead, ahead, batch);
+                                tma_prefetch_4d(&tmQ, a * 64, khead, ahead, batch);
+                            }
+                        }
+#pragma unroll 1
+                        for (int a = 0; a < DV / 64; ++a) {
+                            tma_load_4d(st + L::kOffV + a * 8192, &tmV, &bar_full[s], dvt * 128 + a * 64, head, tok, batch);
+                            if (c + kLead < it.chunks) tma_prefetch_4d(&tmV, dvt * 128 + a * 64, head, ahead, batch);
+                        }
                     }
-#pragma unroll
-                    for (int a = 0; a < DV / 64; ++a) tma_prefetch_4d(&tmV, it.dvt * 128 + a * 64, it.head, ahead, it.batch);
                 }
                 __syncwarp();
             }
@@ -648,22 +666,13 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 mbar_wait_limit(&bar_full[n % kStages], (n / kStages) & 1, &none, 1ll << 28);
             }
         }
-    } else if (warp == 21 || warp == 22) {
-        // =============================================================== MMA issuers
-        // the chunks left of the item at hand, then of the next one that has any
-        auto more = [&](int left) {
-            while (left == 0) {
-                if (!next_item()) return 0;
-                left = it.chunks;
-            }
-            return left;
-        };
-        int left = more(0);
-        if (warp == 21) {
-            constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, false);
-            const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
+    } else if (warp == 21) {
+        // =============================================================== products of the output
+        constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, false);
+        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
+        while (next_item()) {
 #pragma unroll 1
-            while (left > 0) {
+            for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages, b = gc & 1;
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
@@ -675,45 +684,44 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 else mma_ts_k64_w<true, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
                 mma_commit_w(&bar_o[b]);
                 mma_commit_w(&bar_empty[s]);
-                ++gc;
-                left = more(left - 1);
             }
-        } else {
-            constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
-            constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true);
-            const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
-            const uint64_t dKm = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024);  // read MN-major
-            bool first = true;
-            uint32_t n = 0;  // chunk of the next Q K^T, which goes out ahead of the increment of the chunk before
+        }
+    } else if (warp == 22) {
+        // =============================================================== increments
+        constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true);
+        const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024);  // read MN-major
+        while (next_item()) {
 #pragma unroll 1
-            while (left > 0) {
-                const uint32_t s = n % kStages, bn = n & 1;
-                mbar_wait_short(&bar_full[s], (n / kStages) & 1, abort_flag);
-                if (n > 1) mbar_wait_short(&bar_p[bn], ((n >> 1) + 1) & 1, abort_flag);  // the scores of two chunks before have been read
+            for (int c = 0; c < it.chunks; ++c, ++gc) {
+                const uint32_t s = gc % kStages, b = gc & 1;
+                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
+                const uint32_t tV = tmem + (__shfl_sync(0xffffffffu, gate_buf(gc)[259], 0) != 0.f ? kTmV : kTmVd) + 32 * b;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
+                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-                const uint32_t tP = tmem + kTmP + (bn ? (16u << 16) : 0u);
+                mma_ts_k64_w<true, 128>(tmem + kTmF, tV, desc_advance(dK, s * L::kStage), id_d);
+                mma_commit_w(&bar_d[b]);
+                mma_commit_w(&bar_empty[s]);
+            }
+        }
+    } else if (warp == 24) {
+        // =============================================================== scores
+        constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
+        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
+        while (next_item()) {
+#pragma unroll 1
+            for (int c = 0; c < it.chunks; ++c, ++gc) {
+                const uint32_t s = gc % kStages, b = gc & 1;
+                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                if (gc > 1) mbar_wait_short(&bar_p[b], ((gc >> 1) + 1) & 1, abort_flag);  // the scores of two chunks before have been read
+                tc_fence_after_sync();
+                const uint32_t tP = tmem + kTmP + (b << 20);  // (16 lanes on for odd chunks)
                 const uint64_t q = desc_advance(dQ, s * L::kStage), k = desc_advance(dK, s * L::kStage);
                 mma_ss_k64_w<false, 2, 2>(tP, q, k, id_qk);
                 if (DK == 128) mma_ss_k64_w<true, 2, 2>(tP, desc_advance(q, 8192), desc_advance(k, 8192), id_qk);
-                mma_commit_w(&bar_score[bn]);
-                ++n;
-                left = more(left - 1);
-                if (first && left > 0) {
-                    first = false;
-                    continue;
-                }
-                do {  // (twice behind the last Q K^T)
-                    const uint32_t sd = gc % kStages, b = gc & 1;
-                    mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
-                    tc_fence_after_sync();
-                    const bool plain = gate_buf(gc)[259] != 0.f;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
-                    mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + (plain ? kTmV : kTmVd) + 32 * b, desc_advance(dKm, sd * L::kStage), id_d);
-                    mma_commit_w(&bar_d[b]);
-                    mma_commit_w(&bar_empty[sd]);
-                    ++gc;
-                } while (left == 0 && gc < n);
+                mma_commit_w(&bar_score[b]);
             }
         }
     } else if (warp == 23) {
@@ -729,10 +737,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             __syncwarp();
             ++n;
         };
+        const int size_log2 = p.gate.is_f32 ? 2 : 1;
+        const char* from = nullptr;  // the next chunk's gate of this lane
+        auto load1 = [&](const char* at, bool there) {  // as bits, converted where it is used
+            uint32_t bits = 0u;
+            if (there) bits = size_log2 == 2 ? __ldg(reinterpret_cast<const uint32_t*>(at)) : static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(at))) << 16;
+            return bits;
+        };
         auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
-            const int t = c * kChunk + lane;
-            a0 = p.gate.ptr && t < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t, it.head) : 0u;
-            a1 = p.gate.ptr && t + 32 < it.tokens ? p.gate.load_bits(it.batch, it.tok0 + t + 32, it.head) : 0u;
+            const int t = c * kChunk + lane, end = p.gate.ptr ? it.tokens : 0;
+            a0 = load1(from, t < end);
+            a1 = load1(from + (p.gate.st << (5 + size_log2)), t + 32 < end);
+            from += p.gate.st << (6 + size_log2);
         };
 #pragma unroll 1
         for (int i = blockIdx.x; i < p.num_items; i += gridDim.x) {
@@ -740,10 +756,11 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             hand_out();
             uint32_t a0, a1;
             float expo = 0.f;  // c
+            from = static_cast<const char*>(p.gate.ptr) + ((it.batch * p.gate.sb + (it.tok0 + lane) * p.gate.st + it.head * p.gate.sh) << size_log2);
             load(0, a0, a1);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                float g0 = lin_gate_log2(p.gate.value(a0)), g1 = lin_gate_log2(p.gate.value(a1));
+                float g0 = lin_gate_log2(__uint_as_float(a0)), g1 = lin_gate_log2(__uint_as_float(a1));
                 load(c + 1, a0, a1);
                 scan64(g0, g1, lane);  // (tokens past the end have no decay: they carry the last one's sum)
                 const float last = __shfl_sync(0xffffffffu, g1, 31);
@@ -751,14 +768,14 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 auto within = [&](float c) { return __all_sync(0xffffffffu, fabsf(g0 + c) <= kPlainLog2 && fabsf(g1 + c) <= kPlainLog2); };
                 float before = 1.f, behind = 1.f;
                 bool plain = within(expo);
-                if (!plain) {  // the state takes its exponent
+                if (__builtin_expect(!plain, 0)) {  // the state takes its exponent
                     before = ex2(expo);
                     expo = 0.f;
                     plain = within(0.f);
                 }
                 mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
-                if (plain) {
+                if (__builtin_expect(plain, 1)) {
                     g0 += expo;
                     g1 += expo;
                     gb[lane] = ex2(-g0);

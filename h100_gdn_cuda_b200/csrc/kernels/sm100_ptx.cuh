@@ -98,30 +98,25 @@ GDN_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_fl
     return mbar_wait_limit(bar, parity, abort_flag, kWaitLimitCycles);
 }
 
-// The same in a few instructions, for kernels of many roles whose waits would not all fit the instruction cache.  The hardware is asked to
-// keep the warp suspended for up to 4 us a poll: two dozen warps that poll in a loop take half of an SM's issue slots from the ones that work.  The
-// limit is a number of polls, four seconds where they last that long.
-GDN_DEVICE bool mbar_try_wait_long(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
+// The same in as few instructions as there can be, for kernels of many roles, whose code does not fit the instruction cache otherwise.  The hardware
+// is asked to keep the warp suspended for up to 4 us a poll; the limit is a number of polls, four seconds where they last that long.
+GDN_DEVICE void mbar_wait_short(uint64_t* bar, uint32_t parity, const int* abort_flag) {
     asm volatile(
-        "{\n\t.reg .pred P;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, 4000;\n\t"
-        "selp.u32 %0, 1, 0, P;\n\t}\n"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity)
+        "{\n\t.reg .pred P;\n\t.reg .u32 left, given_up;\n\t"
+        "mov.u32 left, 1048576;\n"
+        "WAIT:\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1, 4000;\n\t"
+        "@P bra DONE;\n\t"
+        "ld.volatile.shared.u32 given_up, [%2];\n\t"
+        "setp.ne.u32 P, given_up, 0;\n\t"
+        "@P bra DONE;\n\t"
+        "sub.u32 left, left, 1;\n\t"
+        "setp.ne.u32 P, left, 0;\n\t"
+        "@P bra WAIT;\n\t"
+        "st.volatile.shared.u32 [%2], 1;\n"
+        "DONE:\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(parity), "r"(smem_u32(abort_flag))
         : "memory");
-    return ok != 0;
-}
-GDN_DEVICE bool mbar_wait_short(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    int left = 1 << 20;
-#pragma unroll 1
-    while (!mbar_try_wait_long(bar, parity)) {
-        if (*abort_flag != 0 || --left == 0) {
-            *abort_flag = 1;
-            return false;
-        }
-    }
-    return true;
 }
 
 // The same wait for warps that are not on a critical path: sleeps `kSleepNs` between polls so
@@ -184,6 +179,19 @@ GDN_DEVICE void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int c0, 
         ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0),
         "r"(c1), "r"(c2), "r"(c3)
         : "memory");
+}
+GDN_DEVICE void tma_load_5d(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2, int c3, int c4) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+        : "memory");
+}
+GDN_DEVICE void tma_prefetch_5d(const void* tmap, int c0, int c1, int c2, int c3, int c4) {
+    asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global.tile [%0, {%1, %2, %3, %4, %5}];" ::"l"(
+                     reinterpret_cast<uint64_t>(tmap)),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
+                 : "memory");
 }
 // Warp-collective TMA loads: the converged warp calls them with warp-uniform arguments and one
 // elected lane issues (keeps the tensor-map address and coordinates in uniform registers).
