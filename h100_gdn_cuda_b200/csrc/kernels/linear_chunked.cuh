@@ -3,13 +3,13 @@
 //     O = scale * ( e^{G_i} Q S^T  +  (Q K^T .* e^{G_i - G_j}, j <= i) V )
 //     S <- e^{G_L} S + (e^{G_L - G_j} V)^T K .
 // The state's increment does not depend on the state, so all products of a chunk can be issued ahead of it.  Where no decay of the chunk is
-// below 2^-64 it is a factor of the values alone,
+// below 2^-120 it is a factor of the values alone,
 //     V' = e^{-G_j} V ,   O = scale e^{G_i} * ( Q S^T + (Q K^T, j <= i) V' ) ,   S <- e^{G_L} (S + V'^T K) ,
 // so that the scores only have to be cut off above the diagonal and both parts of O are one accumulation ("plain" chunks).  The factor
 // e^{G_L} is not applied either but kept as an exponent c of the whole state, which joins the factors of the chunks that follow,
 //     S = 2^c S' ,   V' = e^{-G_j} 2^{-c} V ,   O = scale e^{G_i} 2^c * ( ... ) ,
-// until it leaves 2^-64 too: S' is an accumulator in tensor memory that the increments are added to by the products themselves.  (2^64 leaves
-// 2^60 for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: it goes into the
+// until it leaves 2^-60 .. 2^60: S' is an accumulator in tensor memory that the increments are added to by the products themselves.  (That leaves
+// 2^60 and more for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: it goes into the
 // scores, the rows of Q are scaled where they lie, the values come twice and the state is scaled between its read and its increment.
 //
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
@@ -19,10 +19,9 @@
 //   warps 12-15 score warps: the scores as bf16 tile
 //   warps 16-19 value warps: V^T times its factors into tensor memory
 //   warp 20     producer: tensor copies of Q, K, V into a ring of stages
-//   warp 21     issues the products of the output, V'^T P^T and S Q^T
-//   warp 22     issues the state's increment V'^T K
+//   warp 21     issues the state's increment V'^T K, which the next chunk waits for, then the products of the output, V'^T P^T and S Q^T
+//   warp 22     issues the scores Q K^T
 //   warp 23     finds the items; the gates' running sums and the factors made of them
-//   warp 24     issues the scores Q K^T
 // All products that feed output and state are transposed (128 dv rows = M): S and V' are A operands in tensor memory; Q, K and the scores
 // are B operands.
 // What bounds a chunk is shared memory (176 KB of copies, operands and tiles at 128 bytes a cycle: 1400 cycles) and what a warp of each role
@@ -143,14 +142,14 @@ struct LinSmem {
 };
 
 namespace lin {
-constexpr int kThreads = 800;  // 25 warps
+constexpr int kThreads = 768;  // 24 warps
 constexpr uint32_t kTmS = 0;     // its bf16 copy, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
 constexpr uint32_t kTmF = 128;   // fp32 state, 128 columns
 constexpr uint32_t kTmO = 256;   // 2 x fp32 V'^T P^T + S Q^T, 64 columns
 constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: V^T), 32 columns
 constexpr uint32_t kTmVd = 448;  // 2 x bf16 (e^{G_L - G_j} V)^T of chunks that are not plain, 32 columns
-constexpr float kPlainLog2 = 64.f;
+constexpr float kPlainLog2 = 60.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
@@ -221,28 +220,27 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     // No barrier may run two phases ahead of somebody who waits on it: each one's next phase but one needs what its waiters do after
     // theirs.  Barriers of two are those of even and of odd chunks.
     uint64_t* bar_full = bars;                  // [stages] Q, K, V of a stage have arrived
-    uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done (both issuers)
+    uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done
     uint64_t* bar_gate = bar_empty + kStages;   // [4] gate factors of a chunk
-    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps and the increments' issuer
+    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps and the products' issuer
     uint64_t* bar_score = bar_gfree + 4;        // [2] Q K^T done
     uint64_t* bar_p = bar_score + 2;            // [2] scores and values written, and the output's accumulator read two chunks before
-    uint64_t* bar_dgo = bar_p + 2;              // [2] values written, and the state copied
+    uint64_t* bar_dgo = bar_p + 2;              // [2] values written and the state copied
     uint64_t* bar_o = bar_dgo + 2;              // [2] O done: scores, state and values read
-    uint64_t* bar_d = bar_o + 2;                // [2] increment added: values read
-    uint64_t* bar_sgo = bar_d + 2;              // the state's copy is there
-    uint64_t* bar_item = bar_sgo + 1;           // [2] an item is there
+    uint64_t* bar_d = bar_o + 2;                // [2] increment added
+    uint64_t* bar_item = bar_d + 2;             // [2] an item is there
     uint64_t* bar_itemfree = bar_item + 2;      // [2] and every warp has it
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_itemfree + 2);
     int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
     LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
-    static_assert((2 * kStages + 23) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
+    static_assert((2 * kStages + 22) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         *abort_flag = 0;
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&bar_full[i], 1);
-            mbar_init(&bar_empty[i], 2);
+            mbar_init(&bar_empty[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar_gate[i], 1);
@@ -255,9 +253,8 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             mbar_init(&bar_o[i], 1);
             mbar_init(&bar_d[i], 1);
             mbar_init(&bar_item[i], 1);
-            mbar_init(&bar_itemfree[i], 24);
+            mbar_init(&bar_itemfree[i], 23);
         }
-        mbar_init(bar_sgo, 8);
         mbar_fence_init();
     }
     // the scores' blocks above the diagonal stay zero: nobody writes them
@@ -330,14 +327,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 pow_c = gate_buf(gc)[258];
                 const bool scaled = before != 1.f || behind != 1.f;  // (a NaN is)
                 const f2 before2 = pk(before, before), behind2 = pk(behind, behind);
-                if (gc > 0) {  // the copy of the chunk before has been read, its increment added
-                    mbar_wait_short(&bar_o[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
-                    mbar_wait_short(&bar_d[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
-                }
+                if (gc > 0) mbar_wait_short(&bar_d[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-#pragma unroll 1
+                uint32_t w[kCols / 2];  // (rounded to bf16 as an operand: the state itself stays in fp32)
+#pragma unroll
                 for (int q = 0; q < kCols; q += 32) {
-                    uint32_t r[32], w[16];
+                    uint32_t r[32];
                     tmem_ld32(tF + q, r);
                     tmem_wait_ld();
                     if (__builtin_expect(scaled, 0)) {
@@ -345,7 +340,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         for (int e = 0; e < 16; ++e) {
                             float x, y;
                             const f2 v = mul2(pk(r[2 * e], r[2 * e + 1]), before2);
-                            w[e] = pack2(v);
+                            w[q / 2 + e] = pack2(v);
                             unpk(mul2(v, behind2), x, y);
                             r[2 * e] = __float_as_uint(x);
                             r[2 * e + 1] = __float_as_uint(y);
@@ -354,15 +349,17 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         tmem_st16(tF + q + 16, r + 16);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) w[e] = pack2(pk(r[2 * e], r[2 * e + 1]));
+                        for (int e = 0; e < 16; ++e) w[q / 2 + e] = pack2(pk(r[2 * e], r[2 * e + 1]));
                     }
-                    tmem_st16(tS + q / 2, w);  // (rounded to bf16 as an operand: the state itself stays in fp32)
                 }
+                if (gc > 0) mbar_wait_short(&bar_o[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);  // the copy before has been read
+                tc_fence_after_sync();
+#pragma unroll
+                for (int q = 0; q < kCols / 2; q += 16) tmem_st16(tS + q, w + q);
                 tmem_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(bar_sgo);
                     mbar_arrive(&bar_dgo[gc & 1]);
                     mbar_arrive(&bar_gfree[gc & 3]);
                 }
@@ -552,10 +549,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 uint8_t* stage = smem + s * L::kStage;
                 const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                if (gc > 1) {
-                    mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
-                    mbar_wait_short(&bar_d[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);
-                }
+                if (gc > 1) mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the values of two chunks before have been read
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 tc_fence_after_sync();
                 const bool plain = gb[259] != 0.f;
@@ -667,46 +661,31 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             }
         }
     } else if (warp == 21) {
-        // =============================================================== products of the output
-        constexpr uint32_t id_o = make_idesc_bf16(128, 64, false, false);
-        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
-        while (next_item()) {
-#pragma unroll 1
-            for (int c = 0; c < it.chunks; ++c, ++gc) {
-                const uint32_t s = gc % kStages, b = gc & 1;
-                mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
-                mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
-                tc_fence_after_sync();
-                mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmV + 32 * b, desc_advance(dP, b * 8192), id_o);
-                mbar_wait_short(bar_sgo, gc & 1, abort_flag);
-                tc_fence_after_sync();
-                if (DK == 128) mma_ts_k128_w<true>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
-                else mma_ts_k64_w<true, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
-                mma_commit_w(&bar_o[b]);
-                mma_commit_w(&bar_empty[s]);
-            }
-        }
-    } else if (warp == 22) {
-        // =============================================================== increments
-        constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true);
+        // =============================================================== products of state and output
+        constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true), id_o = make_idesc_bf16(128, 64, false, false);
         const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024);  // read MN-major
+        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages, b = gc & 1;
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 const uint32_t tV = tmem + (__shfl_sync(0xffffffffu, gate_buf(gc)[259], 0) != 0.f ? kTmV : kTmVd) + 32 * b;
-                __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
+                mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
                 mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 mma_ts_k64_w<true, 128>(tmem + kTmF, tV, desc_advance(dK, s * L::kStage), id_d);
                 mma_commit_w(&bar_d[b]);
+                if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
+                else mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
+                mma_ts_k64_w<true, 2>(tmem + kTmO + 64 * b, tmem + kTmV + 32 * b, desc_advance(dP, b * 8192), id_o);
+                mma_commit_w(&bar_o[b]);
                 mma_commit_w(&bar_empty[s]);
             }
         }
-    } else if (warp == 24) {
+    } else if (warp == 22) {
         // =============================================================== scores
         constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
         const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
@@ -768,10 +747,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 auto within = [&](float c) { return __all_sync(0xffffffffu, fabsf(g0 + c) <= kPlainLog2 && fabsf(g1 + c) <= kPlainLog2); };
                 float before = 1.f, behind = 1.f;
                 bool plain = within(expo);
-                if (__builtin_expect(!plain, 0)) {  // the state takes its exponent
-                    before = ex2(expo);
-                    expo = 0.f;
-                    plain = within(0.f);
+                if (__builtin_expect(!plain, 0)) {  // the state takes another exponent, the largest one if that does
+                    plain = within(kPlainLog2);
+                    const float other = plain ? kPlainLog2 : 0.f;
+                    if (!plain) plain = within(0.f);
+                    before = ex2(expo - other);
+                    expo = other;
                 }
                 mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
