@@ -1,6 +1,8 @@
 // C-ABI entry points of linear attention with decay (see include/gdn_b200.h): argument checks and launches.
+#include "heuristics.hpp"
 #include "kernels/linear_chunked.cuh"
 #include "kernels/linear_recurrent.cuh"
+#include "kernels/linear_segments.cuh"
 #include "token_host.hpp"
 
 using namespace gdn;
@@ -54,9 +56,33 @@ int linear_map(CUtensorMap* out, GdnTokenTensor t, const GdnShape& s, int heads,
 
 bool wide_linear(const GdnShape& s) { return s.head_dim_k > 128; }
 
+// Segments of a problem on `sms` SMs and where they lie in the workspace: [states of (slot, v-head, dv tile)][decays of (slot, v-head)].
+struct LinearPlan {
+    int seg_chunks, num_segments;  // num_segments: padded mode
+    long long slots;
+    size_t states, bytes;
+};
+LinearPlan linear_plan(const GdnShape& s) {
+    const bool packed = s.cu_seqlens != nullptr;
+    const long long tokens = packed ? s.total_tokens : s.seq_len, chunks = std::max<long long>(1, (tokens + kChunk - 1) / kChunk);
+    const int tiles = (s.head_dim_v + 127) / 128;
+    LinearPlan plan{};
+    plan.seg_chunks = linear_segment_chunks(s.batch, static_cast<long long>(s.num_v_heads) * tiles, chunks, packed);
+    plan.num_segments = static_cast<int>((chunks + plan.seg_chunks - 1) / plan.seg_chunks);
+    plan.slots = packed ? s.batch + tokens / (static_cast<long long>(kChunk) * plan.seg_chunks) : static_cast<long long>(s.batch) * plan.num_segments;
+    if (plan.seg_chunks >= chunks) {  // (no sequence has more chunks than that)
+        plan.slots = s.batch;
+        return plan;
+    }
+    plan.states = static_cast<size_t>(plan.slots) * s.num_v_heads * tiles * 128 * (s.head_dim_k <= 64 ? 64 : 128) * sizeof(float);
+    plan.bytes = plan.states + (static_cast<size_t>(plan.slots) * s.num_v_heads * sizeof(float) + 255) / 256 * 256;
+    return plan;
+}
+
 template <int DK, int DV, bool kWhole>
 int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, int sms, cudaStream_t st) {
     using L = LinSmem<DK, DV>;
+    using LS = LinSegSmem<DK, DV>;
     const GdnShape& s = a.shape;
     CUtensorMap tmQ, tmK, tmV, tmO;
     if (int rc = linear_map(&tmQ, a.q, s, s.num_k_heads, s.head_dim_k, "q", kWhole ? DK : 0)) return rc;
@@ -65,15 +91,26 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     if (int rc = linear_map(&tmO, a.out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
     if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV, kWhole>>(L::kBytes)) return rc;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.num_items, sms)));
-    cfg.blockDim = dim3(lin::kThreads);
-    cfg.dynamicSmemBytes = L::kBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
+    if (p.seg_state) {
+        if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole>>(LS::kBytes)) return rc;
+        cfg.gridDim = dim3(static_cast<unsigned>(p.num_items));
+        cfg.blockDim = dim3(lin::kSegThreads);
+        cfg.dynamicSmemBytes = LS::kBytes;
+        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole>, tmK, tmV, p));
+        cfg.gridDim = dim3(static_cast<unsigned>(p.num_seqs * p.vh * p.dv_tiles), 128 * DK / 4 / kLinCombineThreads);
+        cfg.blockDim = dim3(kLinCombineThreads);
+        cfg.dynamicSmemBytes = 0;
+        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_combine_kernel, p, DK));
+    }
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.num_items, sms)));
+    cfg.blockDim = dim3(lin::kThreads);
+    cfg.dynamicSmemBytes = L::kBytes;
     GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV, kWhole>, tmQ, tmK, tmV, tmO, p));
     return GDN_OK;
 }
@@ -120,7 +157,10 @@ int gdn_linear_recurrent(const GdnLinearRecurrentArgs* a, gdn_stream_t stream) {
     return a->state_dtype == GDN_F32 ? launch_linear_recurrent<true>(p, st) : launch_linear_recurrent<false>(p, st);
 }
 
-size_t gdn_linear_chunked_workspace_bytes(const GdnShape*) { return 0; }
+size_t gdn_linear_chunked_workspace_bytes(const GdnShape* s) {
+    if (!s || wide_linear(*s) || check_linear_shape(*s, "gdn_linear_chunked_workspace_bytes") != GDN_OK) return 0;
+    return linear_plan(*s).bytes;
+}
 
 int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     GDN_REQUIRE(a != nullptr, "gdn_linear_chunked: args is NULL");
@@ -161,11 +201,18 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     p.state_f32 = a->state_dtype == GDN_F32;
     p.scale = a->scale;
     p.status = d->status;
-    p.seg_chunks = static_cast<int>((tokens + kChunk - 1) / kChunk);  // (no sequence has more)
-    p.num_segments = 1;
-    const long long items = static_cast<long long>(s.batch) * p.vh * p.dv_tiles;
-    GDN_REQUIRE(items < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
+    const LinearPlan plan = linear_plan(s);
+    p.seg_chunks = plan.seg_chunks;
+    p.num_segments = plan.num_segments;
+    const long long items = plan.slots * p.vh * p.dv_tiles;
+    GDN_REQUIRE(items < (1ll << 31) && static_cast<long long>(s.batch) * p.vh * p.dv_tiles < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
     p.num_items = static_cast<int>(items);
+    if (plan.bytes) {
+        if (!a->workspace || a->workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a->workspace) & 255u))
+            return fail(GDN_ERR_WORKSPACE, "gdn_linear_chunked: workspace of %zu bytes (256-byte aligned) required, got %zu", plan.bytes, a->workspace_bytes);
+        p.seg_state = static_cast<float*>(a->workspace);
+        p.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + plan.states);
+    }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // (a single column block needs no rank 5: its map clips what is missing)
     const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);

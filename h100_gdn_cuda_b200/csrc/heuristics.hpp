@@ -228,4 +228,12 @@ inline int conv_tok_block(long long tokens, long long blocks_per_token_block, in
     return best;
 }
 
+// Linear attention, prompts: chunks of a segment, for `seqs` sequences of `heads` (v-head, dv tile) pairs and `chunks` chunks each (packed:
+// in all).  A CTA an SM runs through a segment.
+inline int linear_segment_chunks(long long seqs, long long heads, long long chunks, bool packed) {
+    static const int forced = std::getenv("LIN_SEG") ? atoi(std::getenv("LIN_SEG")) : 0;
+    if (forced > 0) return static_cast<int>(std::min<long long>(forced, chunks));
+    return static_cast<int>(chunks);
+}
+
 }  // namespace gdn
