@@ -56,31 +56,43 @@ int linear_map(CUtensorMap* out, GdnTokenTensor t, const GdnShape& s, int heads,
 
 bool wide_linear(const GdnShape& s) { return s.head_dim_k > 128; }
 
-// Segments of a problem on `sms` SMs and where they lie in the workspace: [states of (slot, v-head, dv tile)][decays of (slot, v-head)].
+// Items of a problem (see LinChunkedParams), and where the segments' states lie in the workspace: [states][decays], one each per item behind `whole`.
 struct LinearPlan {
-    int seg_chunks, num_segments;  // num_segments: padded mode
-    long long slots;
-    size_t states, bytes;
+    long long whole, items, cut_chains;  // cut_chains: chains in segments (packed: all, if any)
+    int seg_chunks, num_segments, by_length;
+    size_t states, bytes;  // 0: no segments
 };
 LinearPlan linear_plan(const GdnShape& s) {
     const bool packed = s.cu_seqlens != nullptr;
     const long long tokens = packed ? s.total_tokens : s.seq_len, chunks = std::max<long long>(1, (tokens + kChunk - 1) / kChunk);
-    const int tiles = (s.head_dim_v + 127) / 128;
+    const long long per = static_cast<long long>(s.num_v_heads) * ((s.head_dim_v + 127) / 128), chains = s.batch * per;
     LinearPlan plan{};
-    plan.seg_chunks = linear_segment_chunks(s.batch, static_cast<long long>(s.num_v_heads) * tiles, chunks, packed);
-    plan.num_segments = static_cast<int>((chunks + plan.seg_chunks - 1) / plan.seg_chunks);
-    plan.slots = packed ? s.batch + tokens / (static_cast<long long>(kChunk) * plan.seg_chunks) : static_cast<long long>(s.batch) * plan.num_segments;
-    if (plan.seg_chunks >= chunks) {  // (no sequence has more chunks than that)
-        plan.slots = s.batch;
-        return plan;
+    plan.whole = plan.items = chains;
+    plan.num_segments = 1;
+    plan.seg_chunks = static_cast<int>(chunks);
+    plan.by_length = packed && s.batch > 1 && s.batch <= kLinRankedSeqs;
+    const LinearCut cut = linear_cut(chains, packed ? (chunks + s.batch - 1) / s.batch : chunks, packed);
+    if (cut.segments <= 1) return plan;
+    plan.seg_chunks = static_cast<int>(cut.seg_chunks);
+    if (packed) {
+        plan.by_length = 0;
+        plan.whole = 0;
+        plan.cut_chains = chains;
+        plan.items = (s.batch + tokens / (static_cast<long long>(kChunk) * plan.seg_chunks)) * per;
+    } else {
+        plan.num_segments = static_cast<int>(cut.segments);
+        plan.whole = cut.whole;
+        plan.cut_chains = chains - cut.whole;
+        plan.items = cut.whole + plan.cut_chains * cut.segments;
     }
-    plan.states = static_cast<size_t>(plan.slots) * s.num_v_heads * tiles * 128 * (s.head_dim_k <= 64 ? 64 : 128) * sizeof(float);
-    plan.bytes = plan.states + (static_cast<size_t>(plan.slots) * s.num_v_heads * sizeof(float) + 255) / 256 * 256;
+    const size_t places = static_cast<size_t>(plan.items - plan.whole);
+    plan.states = places * 128 * (s.head_dim_k <= 64 ? 64 : 128) * sizeof(float);
+    plan.bytes = plan.states + (places * sizeof(float) + 255) / 256 * 256;
     return plan;
 }
 
 template <int DK, int DV, bool kWhole>
-int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, int sms, cudaStream_t st) {
+int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, long long cut_chains, cudaStream_t st) {
     using L = LinSmem<DK, DV>;
     using LS = LinSegSmem<DK, DV>;
     const GdnShape& s = a.shape;
@@ -99,16 +111,16 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     cfg.numAttrs = 1;
     if (p.seg_state) {
         if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole>>(LS::kBytes)) return rc;
-        cfg.gridDim = dim3(static_cast<unsigned>(p.num_items));
+        cfg.gridDim = dim3(static_cast<unsigned>(p.num_items - p.whole));
         cfg.blockDim = dim3(lin::kSegThreads);
         cfg.dynamicSmemBytes = LS::kBytes;
         GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole>, tmK, tmV, p));
-        cfg.gridDim = dim3(static_cast<unsigned>(p.num_seqs * p.vh * p.dv_tiles), 128 * DK / 4 / kLinCombineThreads);
+        cfg.gridDim = dim3(static_cast<unsigned>(cut_chains), 128 * DK / 4 / kLinCombineThreads);
         cfg.blockDim = dim3(kLinCombineThreads);
         cfg.dynamicSmemBytes = 0;
         GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_combine_kernel, p, DK));
     }
-    cfg.gridDim = dim3(static_cast<unsigned>(std::min(p.num_items, sms)));
+    cfg.gridDim = dim3(static_cast<unsigned>(p.num_items));
     cfg.blockDim = dim3(lin::kThreads);
     cfg.dynamicSmemBytes = L::kBytes;
     GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV, kWhole>, tmQ, tmK, tmV, tmO, p));
@@ -202,11 +214,12 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     p.scale = a->scale;
     p.status = d->status;
     const LinearPlan plan = linear_plan(s);
+    GDN_REQUIRE(plan.items < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
+    p.whole = static_cast<int>(plan.whole);
     p.seg_chunks = plan.seg_chunks;
     p.num_segments = plan.num_segments;
-    const long long items = plan.slots * p.vh * p.dv_tiles;
-    GDN_REQUIRE(items < (1ll << 31) && static_cast<long long>(s.batch) * p.vh * p.dv_tiles < (1ll << 31), "gdn_linear_chunked: too many sequences and heads");
-    p.num_items = static_cast<int>(items);
+    p.by_length = plan.by_length;
+    p.num_items = static_cast<int>(plan.items);
     if (plan.bytes) {
         if (!a->workspace || a->workspace_bytes < plan.bytes || (reinterpret_cast<uintptr_t>(a->workspace) & 255u))
             return fail(GDN_ERR_WORKSPACE, "gdn_linear_chunked: workspace of %zu bytes (256-byte aligned) required, got %zu", plan.bytes, a->workspace_bytes);
@@ -216,10 +229,10 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // (a single column block needs no rank 5: its map clips what is missing)
     const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);
-    if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false>(*a, p, d->sms, st);
-    if (p.dk <= 64) return launch_linear_chunked<64, 128, false>(*a, p, d->sms, st);
-    if (p.dv <= 64) return launch_linear_chunked<128, 64, false>(*a, p, d->sms, st);
-    return whole ? launch_linear_chunked<128, 128, true>(*a, p, d->sms, st) : launch_linear_chunked<128, 128, false>(*a, p, d->sms, st);
+    if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false>(*a, p, plan.cut_chains, st);
+    if (p.dk <= 64) return launch_linear_chunked<64, 128, false>(*a, p, plan.cut_chains, st);
+    if (p.dv <= 64) return launch_linear_chunked<128, 64, false>(*a, p, plan.cut_chains, st);
+    return whole ? launch_linear_chunked<128, 128, true>(*a, p, plan.cut_chains, st) : launch_linear_chunked<128, 128, false>(*a, p, plan.cut_chains, st);
 }
 
 }  // extern "C"

@@ -228,12 +228,19 @@ inline int conv_tok_block(long long tokens, long long blocks_per_token_block, in
     return best;
 }
 
-// Linear attention, prompts: chunks of a segment, for `seqs` sequences of `heads` (v-head, dv tile) pairs and `chunks` chunks each (packed:
-// in all).  A CTA an SM runs through a segment.
-inline int linear_segment_chunks(long long seqs, long long heads, long long chunks, bool packed) {
+// Linear attention, prompts: which of `chains` (sequence, v-head, dv tile) chains of `chunks` chunks each (packed: on average) are cut into how many
+// segments.
+struct LinearCut {
+    long long whole;       // the first chains, which stay whole (padded)
+    long long segments;    // 1: nothing is cut
+    long long seg_chunks;  // of a segment
+};
+inline LinearCut linear_cut(long long chains, long long chunks, bool packed) {
+    constexpr long long kSms = 148;
     static const int forced = std::getenv("LIN_SEG") ? atoi(std::getenv("LIN_SEG")) : 0;
-    if (forced > 0) return static_cast<int>(std::min<long long>(forced, chunks));
-    return static_cast<int>(chunks);
+    LinearCut cut{chains, 1, chunks};
+    if (forced > 0 && forced < chunks) return LinearCut{packed ? 0 : chains / kSms * kSms, (chunks + forced - 1) / forced, forced};
+    return cut;
 }
 
 }  // namespace gdn

@@ -46,11 +46,13 @@ struct LinChunkedParams {
     int state_f32;
     float scale;
     int* status;
-    // segments of `seg_chunks` chunks: a sequence of c chunks has max(1, ceil(c / seg_chunks)) of them; slots are numbered through the
-    // sequences.  num_items: slots (an upper bound in packed mode) x vh x dv_tiles.
-    int seg_chunks, num_segments, num_items;
-    float* seg_state;  // per item: what the segment adds to the state (gdn_linear_segment_kernel), then the state behind it
-    float* seg_decay;  // per slot and head: the segment's sum of log2-decays
+    // Work items.  Chains are (sequence, v-head, dv tile); a segment is `seg_chunks` chunks of one.
+    //   padded: the first `whole` chains are an item each, every other one `num_segments` of them, one behind the other;
+    //   packed: slots x vh x dv_tiles, where a sequence of c chunks has max(1, ceil(c / seg_chunks)) slots, numbered through the sequences
+    //           (`by_length`: one each, in falling order of length).  num_items is an upper bound there.
+    int whole, seg_chunks, num_segments, num_items, by_length;
+    float* seg_state;  // per item behind `whole`: what the segment adds to the state (gdn_linear_segment_kernel), then the state behind it
+    float* seg_decay;  // and its sum of log2-decays
 };
 
 // Decays are handled as powers of two; anything below 2^-160 is zero in fp32, and sums of 64 such stay exact enough to tell G_i - G_j
@@ -62,66 +64,98 @@ __device__ __forceinline__ float lin_gate_log2(float g) {
 
 struct alignas(16) LinItem {
     int seq, head, khead, dvt;
-    int batch, segment, segments, index;  // index: of the item
-    int slot, tok0, tokens, chunks;       // of the segment; chunks < 0: no more items
+    int batch, segment, segments, mine;  // mine: the item's place among the segments' states (packed, padded behind `whole`)
+    int before, tok0, tokens, chunks;    // before: that of the segment in front; tokens of the segment; chunks < 0: no more items
 };
 
-// Walks the items of a CTA in rising order; warp-collective.
+constexpr int kLinRankedSeqs = 32;  // packed sequences that are ordered by length, a lane each
+
+// Finds items; warp-collective.
 struct LinWalker {
     int base = 0;   // packed mode: first sequence of the 32 that were looked at last
     int first = 0;  // its first slot
     // false: a surplus item
     __device__ __forceinline__ bool locate(const LinChunkedParams& p, int it, LinItem& o) {
+        int bos = 0, len = p.seq_len, chain = it;
         const int per = p.vh * p.dv_tiles;
-        o.slot = it / per;
-        const int r = it - o.slot * per;
+        o.segment = 0;
+        o.segments = 1;
+        if (!p.cu_seqlens) {
+            o.mine = it - p.whole;
+            o.before = o.mine - 1;
+            if (o.mine >= 0) {
+                const int r = o.mine / p.num_segments;
+                chain = p.whole + r;
+                o.segment = o.mine - r * p.num_segments;
+                o.segments = p.num_segments;
+            }
+            o.seq = chain / per;
+            o.batch = o.seq;
+        } else {
+            const int lane = threadIdx.x & 31, slot = it / per;
+            o.batch = 0;
+            o.mine = it;
+            o.before = it - per;
+            auto offset = [&](int s) { return min(max(p.cu_seqlens[s], 0), p.total_tokens); };
+            if (p.by_length) {
+                if (slot >= p.num_seqs) return false;
+                // order: more tokens first, of equally many the one in front first
+                const int b = lane < p.num_seqs ? offset(lane) : 0, mine = lane < p.num_seqs ? max(offset(lane + 1) - b, 0) : -1;
+                int rank = 0;
+#pragma unroll 1
+                for (int j = 0; j < p.num_seqs; ++j) {
+                    const int other = __shfl_sync(0xffffffffu, mine, j);
+                    rank += other > mine || (other == mine && j < lane);
+                }
+                o.seq = __ffs(__ballot_sync(0xffffffffu, lane < p.num_seqs && rank == slot)) - 1;
+                bos = __shfl_sync(0xffffffffu, b, o.seq);
+                len = __shfl_sync(0xffffffffu, mine, o.seq);
+            } else {
+                if (slot < first) base = first = 0;
+#pragma unroll 1
+                while (true) {
+                    if (base >= p.num_seqs) return false;
+                    const int s = base + lane;
+                    int b = 0, e = 0, n = 0;
+                    if (s < p.num_seqs) {
+                        b = offset(s);
+                        e = max(offset(s + 1), b);
+                        n = max(1, ((e - b + kChunk - 1) / kChunk + p.seg_chunks - 1) / p.seg_chunks);
+                    }
+                    int incl = n;
+#pragma unroll
+                    for (int m = 1; m < 32; m <<= 1) {
+                        const int y = __shfl_up_sync(0xffffffffu, incl, m);
+                        if (lane >= m) incl += y;
+                    }
+                    const int total = __shfl_sync(0xffffffffu, incl, 31);
+                    if (slot >= first + total) {
+                        base += 32;
+                        first += total;
+                        continue;
+                    }
+                    const int mine = __ffs(__ballot_sync(0xffffffffu, slot < first + incl)) - 1;
+                    o.seq = base + mine;
+                    o.segments = __shfl_sync(0xffffffffu, n, mine);
+                    o.segment = slot - first - (__shfl_sync(0xffffffffu, incl, mine) - o.segments);
+                    bos = __shfl_sync(0xffffffffu, b, mine);
+                    len = __shfl_sync(0xffffffffu, e, mine) - bos;
+                    break;
+                }
+            }
+        }
+        const int r = chain % per;
         o.head = r / p.dv_tiles;
         o.dvt = r - o.head * p.dv_tiles;
         o.khead = o.head / (p.vh / p.kh);
-        o.index = it;
-        int bos = 0, len = p.seq_len;
-        if (!p.cu_seqlens) {
-            o.seq = o.slot / p.num_segments;
-            o.segment = o.slot - o.seq * p.num_segments;
-            o.segments = p.num_segments;
-            o.batch = o.seq;
-        } else {
-            const int lane = threadIdx.x & 31;
-            o.batch = 0;
-            while (true) {
-                if (base >= p.num_seqs) return false;
-                const int s = base + lane;
-                int b = 0, e = 0, n = 0;
-                if (s < p.num_seqs) {
-                    b = min(max(p.cu_seqlens[s], 0), p.total_tokens);
-                    e = min(max(p.cu_seqlens[s + 1], b), p.total_tokens);
-                    n = max(1, ((e - b + kChunk - 1) / kChunk + p.seg_chunks - 1) / p.seg_chunks);
-                }
-                int incl = n;
-#pragma unroll
-                for (int m = 1; m < 32; m <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, incl, m);
-                    if (lane >= m) incl += y;
-                }
-                const int total = __shfl_sync(0xffffffffu, incl, 31);
-                if (o.slot >= first + total) {
-                    base += 32;
-                    first += total;
-                    continue;
-                }
-                const int mine = __ffs(__ballot_sync(0xffffffffu, o.slot < first + incl)) - 1;
-                o.seq = base + mine;
-                o.segments = __shfl_sync(0xffffffffu, n, mine);
-                o.segment = o.slot - first - (__shfl_sync(0xffffffffu, incl, mine) - o.segments);
-                bos = __shfl_sync(0xffffffffu, b, mine);
-                len = __shfl_sync(0xffffffffu, e, mine) - bos;
-                break;
-            }
+        if (o.segments > 1) {
+            const int t0 = o.segment * p.seg_chunks * kChunk;
+            bos += t0;
+            len = min(len - t0, p.seg_chunks * kChunk);
         }
-        const int t0 = o.segment * p.seg_chunks * kChunk;
-        o.tok0 = bos + t0;
-        o.tokens = min(len - t0, p.seg_chunks * kChunk);
-        o.chunks = (o.tokens + kChunk - 1) / kChunk;
+        o.tok0 = bos;
+        o.tokens = len;
+        o.chunks = (len + kChunk - 1) / kChunk;
         return true;
     }
 };
@@ -230,10 +264,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     uint64_t* bar_d = bar_o + 2;                // [2] increment added
     uint64_t* bar_item = bar_d + 2;             // [2] an item is there
     uint64_t* bar_itemfree = bar_item + 2;      // [2] and every warp has it
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_itemfree + 2);
+    uint64_t* bar_next = bar_itemfree + 2;      // the answer to a request for another item is there
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_next + 1);
     int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
     LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
-    static_assert((2 * kStages + 22) * 8 + 8 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
+    uint8_t* next = smem + L::kOffBar + 512 - 2 * sizeof(LinItem) - 16;  // the answer
+    static_assert((2 * kStages + 23) * 8 + 8 + 16 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -255,6 +291,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             mbar_init(&bar_item[i], 1);
             mbar_init(&bar_itemfree[i], 23);
         }
+        mbar_init(bar_next, 1);
         mbar_fence_init();
     }
     // the scores' blocks above the diagonal stay zero: nobody writes them
@@ -298,7 +335,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 uint32_t r[16];
                 const int cols = row_in ? p.dk - c0 - q : 0;  // columns that are there from this one on
                 if (it.segment > 0) {
-                    const uint4* src = reinterpret_cast<const uint4*>(p.seg_state + static_cast<long long>(it.index - p.vh * p.dv_tiles) * (128 * DK) + (32 * lq + lane) * DK + c0 + q);
+                    const uint4* src = reinterpret_cast<const uint4*>(p.seg_state + static_cast<long long>(it.before) * (128 * DK) + (32 * lq + lane) * DK + c0 + q);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = __ldcg(src + e);
                 } else if (p.state_in && p.state_f32) {
@@ -729,8 +766,11 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             a1 = load1(from + (p.gate.st << (5 + size_log2)), t + 32 < end);
             from += p.gate.st << (6 + size_log2);
         };
+        // The launch has a block for every item.  A block that runs asks for the next one that has not started and takes it over.
+        uint32_t asked = 0;
+        int i = blockIdx.x;
 #pragma unroll 1
-        for (int i = blockIdx.x; i < p.num_items; i += gridDim.x) {
+        while (i >= 0) {
             if (!walker.locate(p, i, it)) break;  // (surplus items are the last ones)
             hand_out();
             uint32_t a0, a1;
@@ -778,6 +818,15 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gate[gc & 3]);
             }
+            if (lane == 0) {
+                fence_proxy_async_smem();
+                mbar_arrive_expect_tx(bar_next, 16);
+                next_block_request(next, bar_next);
+            }
+            __syncwarp();
+            mbar_wait_short(bar_next, asked & 1, abort_flag);
+            ++asked;
+            i = *static_cast<volatile int*>(abort_flag) == 0 ? next_block_answer(next) : -1;
         }
         it.chunks = -1;
         hand_out();

@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
     grid_dep_launch();
     LinWalker walker;
     LinItem it;
-    if (!walker.locate(p, blockIdx.x, it) || it.segment == it.segments - 1) return;  // (the same for all threads)
+    if (!walker.locate(p, p.whole + blockIdx.x, it) || it.segment == it.segments - 1) return;  // (the same for all threads)
     const int chunks = __shfl_sync(0xffffffffu, it.chunks, 0);
     if (tid == 0) {
         *abort_flag = 0;
@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
         mbar_wait_short(&bar_done[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1, abort_flag);
         tc_fence_after_sync();
         if (*static_cast<volatile int*>(abort_flag) == 0 && (DV == 128 || lq < 2)) {
-            uint4* dst = reinterpret_cast<uint4*>(p.seg_state + static_cast<long long>(blockIdx.x) * (128 * DK) + (32 * lq + lane) * DK);
+            uint4* dst = reinterpret_cast<uint4*>(p.seg_state + static_cast<long long>(it.mine) * (128 * DK) + (32 * lq + lane) * DK);
 #pragma unroll 1
             for (int q = 0; q < DK; q += 16) {
                 uint32_t r[16];
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_gate[n & 3]);
         }
-        if (lane == 0 && it.dvt == 0) p.seg_decay[static_cast<long long>(it.slot) * p.vh + it.head] = suffix;
+        if (lane == 0) p.seg_decay[it.mine] = suffix;
     }
     tc_fence_before_sync();
     __syncthreads();
@@ -229,26 +229,26 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
     __shared__ int first_slot, segments;
     ptx::grid_dep_wait();
     ptx::grid_dep_launch();
-    const int per = p.vh * p.dv_tiles, seq = blockIdx.x / per, rest = blockIdx.x % per, head = rest / p.dv_tiles, dvt = rest % p.dv_tiles;
-    if (!p.cu_seqlens) {
-        if (threadIdx.x == 0) {
-            first_slot = seq * p.num_segments;
-            segments = p.num_segments;
-        }
-    } else if (threadIdx.x < 32) {  // the segments of the sequences in front
-        int mine = 0;
-        for (int s = threadIdx.x; s <= seq; s += 32) {
-            const int b = min(max(p.cu_seqlens[s], 0), p.total_tokens), e = min(max(p.cu_seqlens[s + 1], b), p.total_tokens);
-            const int n = max(1, ((e - b + kChunk - 1) / kChunk + p.seg_chunks - 1) / p.seg_chunks);
-            if (s < seq) mine += n;
-            else segments = n;
-        }
+    const int per = p.vh * p.dv_tiles, chain = p.whole + blockIdx.x, seq = chain / per, rest = chain % per, head = rest / p.dv_tiles, dvt = rest % p.dv_tiles;
+    int place = blockIdx.x * p.num_segments, stride = 1, n = p.num_segments - 1;  // of the chain's first segment; from one to the next
+    if (p.cu_seqlens) {
+        if (threadIdx.x < 32) {  // the segments of the sequences in front
+            int mine = 0;
+            for (int s = threadIdx.x; s <= seq; s += 32) {
+                const int b = min(max(p.cu_seqlens[s], 0), p.total_tokens), e = min(max(p.cu_seqlens[s + 1], b), p.total_tokens);
+                const int k = max(1, ((e - b + kChunk - 1) / kChunk + p.seg_chunks - 1) / p.seg_chunks);
+                if (s < seq) mine += k;
+                else segments = k;
+            }
 #pragma unroll
-        for (int m = 16; m > 0; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
-        if (threadIdx.x == 0) first_slot = mine;
+            for (int m = 16; m > 0; m >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, m);
+            if (threadIdx.x == 0) first_slot = mine;
+        }
+        __syncthreads();
+        place = first_slot * per + rest;
+        stride = per;
+        n = min(segments - 1, p.num_items / per - first_slot);  // (offsets that are not in order may ask for more slots than there are)
     }
-    __syncthreads();
-    const int n = min(segments - 1, p.num_items / per - first_slot);  // (offsets that are not in order may ask for more slots than there are)
     if (n <= 0) return;
     const int at = (blockIdx.y * kLinCombineThreads + threadIdx.x) * 4, row = at / dk_tile, col = at % dk_tile;
     const long long drow = dvt * 128 + row;
@@ -262,9 +262,9 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
             s = make_float4(ptx::bf16_lo(v.x), ptx::bf16_hi(v.x), ptx::bf16_lo(v.y), ptx::bf16_hi(v.y));
         }
     }
-    const long long step = static_cast<long long>(per) * 128 * dk_tile;
-    float* from = p.seg_state + (static_cast<long long>(first_slot) * per + rest) * 128 * dk_tile + at;
-    const float* decay = p.seg_decay + static_cast<long long>(first_slot) * p.vh + head;
+    const long long step = static_cast<long long>(stride) * 128 * dk_tile;
+    float* from = p.seg_state + static_cast<long long>(place) * 128 * dk_tile + at;
+    const float* decay = p.seg_decay + place;
     constexpr int kAhead = 4;
     float4 d[kAhead];
     float g[kAhead];
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
     for (int i = 0; i < kAhead; ++i)
         if (i < n) {
             d[i] = __ldcg(reinterpret_cast<const float4*>(from + i * step));
-            g[i] = __ldcg(decay + static_cast<long long>(i) * p.vh);
+            g[i] = __ldcg(decay + static_cast<long long>(i) * stride);
         }
     for (int i0 = 0; i0 < n; i0 += kAhead) {
 #pragma unroll
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
                 *reinterpret_cast<float4*>(from + (i0 + i) * step) = s;
                 if (i0 + i + kAhead < n) {
                     d[i] = __ldcg(reinterpret_cast<const float4*>(from + (i0 + i + kAhead) * step));
-                    g[i] = __ldcg(decay + static_cast<long long>(i0 + i + kAhead) * p.vh);
+                    g[i] = __ldcg(decay + static_cast<long long>(i0 + i + kAhead) * stride);
                 }
             }
         }

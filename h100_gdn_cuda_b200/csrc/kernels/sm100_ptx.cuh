@@ -252,6 +252,27 @@ GDN_DEVICE void grid_dep_takeover() {
     asm volatile("fence.acq_rel.gpu;" ::: "memory");
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
+// Work taken over from blocks of the same launch that have not started: a request (16 bytes are written to `answer`, 16-byte aligned, and
+// complete on `bar`), and its answer: the x index of the block that will not start any more, or -1 when there is none left (then no
+// further request may be made).
+GDN_DEVICE void next_block_request(void* answer, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)),
+                 "r"(smem_u32(bar))
+                 : "memory");
+}
+GDN_DEVICE int next_block_answer(const void* answer) {
+    int x;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+        "ld.shared.b128 a, [%1];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "mov.b32 %0, -1;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %0, a;\n\t}\n"
+        : "=r"(x)
+        : "r"(smem_u32(answer))
+        : "memory");
+    return x;
+}
 // Untiled bulk copy global -> shared; both addresses 16-byte aligned, bytes % 16 == 0.
 GDN_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile(
