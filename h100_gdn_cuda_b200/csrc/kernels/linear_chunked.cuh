@@ -302,6 +302,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    if (warp == 20 && lane < 4) prefetch_tmap(lane == 0 ? &tmQ : lane == 1 ? &tmK : lane == 2 ? &tmV : &tmO);
     grid_dep_wait();
     grid_dep_launch();
 
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             const int row = it.dvt * 128 + 32 * lq + lane;
             const bool row_in = 32 * lq + lane < DV && row < p.dv;
             // ---- the state that enters the segment (the increments of the item before have been read at its end)
-#pragma unroll 1
+#pragma unroll 2
             for (int q = 0; q < kCols; q += 16) {
                 uint32_t r[16];
                 const int cols = row_in ? p.dk - c0 - q : 0;  // columns that are there from this one on
@@ -773,14 +774,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         while (i >= 0) {
             if (!walker.locate(p, i, it)) break;  // (surplus items are the last ones)
             hand_out();
-            uint32_t a0, a1;
+            uint32_t a0, a1, b0, b1, c0, c1;  // the gates of this chunk and the two behind it: DRAM answers later than a chunk takes
             float expo = 0.f;  // c
             from = static_cast<const char*>(p.gate.ptr) + ((it.batch * p.gate.sb + (it.tok0 + lane) * p.gate.st + it.head * p.gate.sh) << size_log2);
             load(0, a0, a1);
+            load(1, b0, b1);
+            load(2, c0, c1);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 float g0 = lin_gate_log2(__uint_as_float(a0)), g1 = lin_gate_log2(__uint_as_float(a1));
-                load(c + 1, a0, a1);
+                a0 = b0; a1 = b1;
+                b0 = c0; b1 = c1;
+                load(c + 3, c0, c1);
                 scan64(g0, g1, lane);  // (tokens past the end have no decay: they carry the last one's sum)
                 const float last = __shfl_sync(0xffffffffu, g1, 31);
                 // (a NaN is not plain, neither are gates that grow)

@@ -190,19 +190,23 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
     } else {
         // =============================================================== gates
         float suffix = 0.f;  // of the chunks behind, log2
-        auto load = [&](int c, float& a0, float& a1) {
-            a0 = a1 = 0.f;
+        auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
+            a0 = a1 = 0u;
             if (c >= 0 && p.gate.ptr) {  // (segments in front of the last one are whole chunks)
-                a0 = p.gate.load(it.batch, it.tok0 + c * kChunk + lane, it.head);
-                a1 = p.gate.load(it.batch, it.tok0 + c * kChunk + 32 + lane, it.head);
+                a0 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + lane, it.head);
+                a1 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + 32 + lane, it.head);
             }
         };
-        float a0, a1;
+        uint32_t a0, a1, b0, b1, c0, c1;  // the gates of this chunk and the two in front of it: DRAM answers later than a chunk takes
         load(chunks - 1, a0, a1);
+        load(chunks - 2, b0, b1);
+        load(chunks - 3, c0, c1);
 #pragma unroll 1
         for (int n = 0; n < chunks; ++n) {
-            float g0 = lin_gate_log2(a0), g1 = lin_gate_log2(a1);
-            load(chunks - 2 - n, a0, a1);
+            float g0 = lin_gate_log2(p.gate.value(a0)), g1 = lin_gate_log2(p.gate.value(a1));
+            a0 = b0; a1 = b1;
+            b0 = c0; b1 = c1;
+            load(chunks - 4 - n, c0, c1);
             scan64(g0, g1, lane);
             const float last = __shfl_sync(0xffffffffu, g1, 31);
             mbar_wait_short(&bar_gfree[n & 3], ((n >> 2) + 1) & 1, abort_flag);
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
     const long long step = static_cast<long long>(stride) * 128 * dk_tile;
     float* from = p.seg_state + static_cast<long long>(place) * 128 * dk_tile + at;
     const float* decay = p.seg_decay + place;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     float4 d[kAhead];
     float g[kAhead];
 #pragma unroll
