@@ -1,27 +1,36 @@
 // C-ABI entry point of the channels-last group norm (see include/gdn_b200.h).
+#include <type_traits>
+
 #include "host_common.hpp"
 #include "kernels/group_norm.cuh"
+#include "token_host.hpp"
 
 using namespace gdn;
 
 namespace {
 
-// How a long sample is cut: channels of a block (whole groups), rows of a part.
+// How a long sample is cut: channels of a block (whole groups, up to 256 vectors), rows of a part.
 struct NormPlan {
-    int block_channels, blocks, part_rows, parts;
+    int block_channels, blocks, part_rows, parts;  // block_channels == 0: the groups are too wide for it
 };
 
-NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int vec) {
+NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int vec, int size) {
     const int width = channels / groups;
-    NormPlan plan;
+    NormPlan plan{};
     int unit = 1;  // groups of a block come in multiples that are whole vectors
     while (unit * width % vec != 0) ++unit;
-    int per = std::max(unit, 256 * vec / width / unit * unit);
-    per = std::min(per, kNormMaxGroups / unit * unit);
-    plan.block_channels = std::min(per * width, channels);
+    if (unit * width > kNormThreads * vec) return plan;
+    const int per = std::min(kNormThreads * vec / (unit * width), kNormMaxGroups / unit) * unit;
+    // blocks of about the same number of groups
+    const int units = (groups + unit - 1) / unit, blocks = (groups + per - 1) / per;
+    plan.block_channels = std::min((units + blocks - 1) / blocks * unit * width, channels);
     plan.blocks = (channels + plan.block_channels - 1) / plan.block_channels;
-    const int64_t want = std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(1, samples * plan.blocks));
-    plan.part_rows = static_cast<int>(std::max<int64_t>(16, (rows + want - 1) / want));
+    const int vecs = plan.block_channels / vec, rstep = kNormThreads / vecs;
+    // three CTAs an SM, as far as rows go round; no more than the part's shared memory holds, no fewer than a few rows a thread
+    const int64_t most = static_cast<int64_t>(kNormPartBytes / (kNormThreads * vec * size)) * rstep;
+    const int64_t want = std::max<int64_t>(1, 3 * 148 / std::max<int64_t>(1, samples * plan.blocks));
+    int64_t part = std::max<int64_t>((rows + want - 1) / want, 4 * rstep);
+    plan.part_rows = static_cast<int>(std::min(part, most));
     plan.parts = static_cast<int>((rows + plan.part_rows - 1) / plan.part_rows);
     return plan;
 }
@@ -30,8 +39,37 @@ constexpr int kShortValues = 1024;  // values of a (sample, group) that stay in 
 bool short_groups(int64_t rows, int width) { return rows * width <= kShortValues; }
 
 template <typename T, int V>
+int launch_rows(const GroupNormParams& p, cudaStream_t st) {
+    int lpr = 1;
+    while (lpr < 32 && lpr * V < p.width) lpr *= 2;
+    const int passes = (p.width + lpr * V - 1) / (lpr * V);
+    auto launch = [&](auto kernel, int unroll) -> int {
+        // (a CTA goes on to further rows while weight and bias stay where they are: as many CTAs as fit the SMs at once)
+        const long long bx = (p.groups + 256 / lpr - 1) / (256 / lpr), slots = std::max<long long>(1, (passes > 1 ? 2 : 4) * 148 / bx);
+        const long long by = std::min<long long>(std::min<long long>((p.n + unroll - 1) / unroll, slots), 65535);
+        GDN_CUDA(launch_dependent(kernel, dim3(static_cast<unsigned>(bx), static_cast<unsigned>(by)), 256, 0, st, p));
+        return GDN_OK;
+    };
+    auto pick = [&](auto gated) -> int {
+        constexpr bool kG = decltype(gated)::value;
+        switch (passes > 1 ? 32 * passes : lpr) {
+            case 1: return launch(gdn_group_norm_rows_kernel<T, V, 1, 1, kG>, 2);
+            case 2: return launch(gdn_group_norm_rows_kernel<T, V, 2, 1, kG>, 2);
+            case 4: return launch(gdn_group_norm_rows_kernel<T, V, 4, 1, kG>, 2);
+            case 8: return launch(gdn_group_norm_rows_kernel<T, V, 8, 1, kG>, 2);
+            case 16: return launch(gdn_group_norm_rows_kernel<T, V, 16, 1, kG>, 2);
+            case 32: return launch(gdn_group_norm_rows_kernel<T, V, 32, 1, kG>, 2);
+            case 64: return launch(gdn_group_norm_rows_kernel<T, V, 32, 2, kG>, 1);
+            default: return launch(gdn_group_norm_rows_kernel<T, V, 32, 4, kG>, 1);
+        }
+    };
+    return p.z ? pick(std::true_type{}) : pick(std::false_type{});
+}
+
+template <typename T, int V>
 int launch_short(const GroupNormParams& p, cudaStream_t st) {
     const long long size = p.l * p.width;
+    if (p.l == 1 && size <= 4 * 32 * V) return launch_rows<T, V>(p, st);
     int lpr = 4;
     while (lpr < 32 && lpr * V < size) lpr *= 2;
     const int passes = static_cast<int>((size + lpr * V - 1) / (lpr * V));
@@ -42,42 +80,63 @@ int launch_short(const GroupNormParams& p, cudaStream_t st) {
     else if (lpr == 8) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 8, 1>));
     else if (lpr == 16) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 16, 1>));
     else if (passes <= 1) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 1>));
-    else if (passes <= 2) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 2>));
     else if (passes <= 4) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 4>));
-    else if (passes <= 8) GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 8>));
     else GDN_CUDA(launch(gdn_group_norm_short_kernel<T, V, 32, 32>));
     return GDN_OK;
 }
 
 template <typename T, int V>
 int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
+    if (plan.block_channels == 0) {
+        GDN_REQUIRE(p.n * p.groups < (1ll << 31), "gdn_group_norm: too many samples");
+        GDN_CUDA(launch_dependent(gdn_group_norm_wide_kernel<T, V>, dim3(static_cast<unsigned>(p.n * p.groups)), kNormThreads, 0, st, p));
+        return GDN_OK;
+    }
     p.part_rows = plan.part_rows;
     p.parts = plan.parts;
     p.block_channels = plan.block_channels;
     GDN_REQUIRE(p.n <= 65535 && plan.blocks <= 65535, "gdn_group_norm: too many samples or channels for one launch");
     const dim3 grid(static_cast<unsigned>(plan.parts), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
-    GDN_CUDA(launch_dependent(gdn_group_norm_stats_kernel<T, V>, grid, kNormThreads, 0, st, p));
-    GDN_CUDA(launch_dependent(gdn_group_norm_apply_kernel<T, V>, grid, kNormThreads, 0, st, p));
+    const int rstep = kNormThreads / (plan.block_channels / V), smem = (plan.part_rows + rstep - 1) / rstep * kNormThreads * V * static_cast<int>(sizeof(T));
+    if (int rc = set_smem<gdn_group_norm_stats_kernel<T, V>>(kNormPartBytes)) return rc;
+    GDN_CUDA(launch_dependent(gdn_group_norm_stats_kernel<T, V>, grid, kNormThreads, smem, st, p));
+    p.join = p.partial;
+    p.join_rows = p.part_rows;
+    p.join_parts = p.parts;
+    if (p.parts > kNormJoinParts) {
+        p.join = p.partial + static_cast<size_t>(p.n) * p.parts * p.groups;
+        p.join_rows = p.l;
+        p.join_parts = 1;
+        const long long blocks = (p.n * p.groups + 7) / 8;
+        GDN_REQUIRE(blocks < (1ll << 31), "gdn_group_norm: too many samples");
+        GDN_CUDA(launch_dependent(gdn_group_norm_join_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, p));
+    }
+    // CTAs of the second launch: four fit an SM; no fewer than eight rows a thread
+    const long long want = std::max<long long>(1, 4 * 148 / std::max<long long>(1, p.n * plan.blocks));
+    p.apply_rows = static_cast<int>(std::min<long long>(std::max<long long>((p.l + want - 1) / want, 8 * rstep), 1 << 20));
+    const dim3 apply(static_cast<unsigned>((p.l + p.apply_rows - 1) / p.apply_rows), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
+    GDN_CUDA(launch_dependent(p.z ? gdn_group_norm_apply_kernel<T, V, true> : gdn_group_norm_apply_kernel<T, V, false>, apply, kNormThreads, 0, st, p));
     return GDN_OK;
 }
 
 template <typename T, int V>
 int launch_norm(const GroupNormParams& p, bool is_short, const GdnGroupNormArgs& a, cudaStream_t st) {
     if (is_short) return launch_short<T, V>(p, st);
-    return launch_long<T, V>(p, norm_plan(a.samples, a.rows, a.channels, a.groups, V), st);
+    return launch_long<T, V>(p, norm_plan(a.samples, a.rows, a.channels, a.groups, V, sizeof(T)), st);
 }
 
 }  // namespace
 
 extern "C" {
 
-// An upper bound over the vector widths, which go by pointers and strides.
+// An upper bound over the vector widths, which go by the type, pointers and strides.
 size_t gdn_group_norm_workspace_bytes(int64_t samples, int64_t rows, int32_t channels, int32_t groups) {
     if (samples <= 0 || rows <= 0 || groups <= 0 || channels <= 0 || channels % groups != 0 || short_groups(rows, channels / groups)) return 0;
     size_t parts = 0;
-    for (int v = 1; v <= 8; v *= 2)
-        if (channels % v == 0) parts = std::max<size_t>(parts, norm_plan(samples, rows, channels, groups, v).parts);
-    return parts * static_cast<size_t>(samples) * groups * sizeof(float2);
+    for (int size = 2; size <= 4; size *= 2)
+        for (int v = 1; v * size <= 16; v *= 2)
+            if (channels % v == 0) parts = std::max<size_t>(parts, norm_plan(samples, rows, channels, groups, v, size).parts);
+    return parts == 0 ? 0 : (parts + 1) * static_cast<size_t>(samples) * groups * sizeof(float2);  // (one more: the parts joined)
 }
 
 int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
@@ -102,7 +161,7 @@ int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
     const bool is_short = short_groups(a->rows, p.width);
     if (!is_short) {
         const size_t need = gdn_group_norm_workspace_bytes(a->samples, a->rows, a->channels, a->groups);
-        if (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace))
+        if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
             return fail(GDN_ERR_WORKSPACE, "gdn_group_norm: workspace of %zu bytes (16-byte aligned) required, got %zu", need, a->workspace_bytes);
         p.partial = static_cast<float2*>(a->workspace);
     }
@@ -112,7 +171,8 @@ int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
         auto whole = [&](const void* ptr, int64_t sn, int64_t sl) {
             return reinterpret_cast<uintptr_t>(ptr) % (static_cast<unsigned>(v * size)) == 0 && (a->samples == 1 || sn % v == 0) && (a->rows == 1 || sl % v == 0);
         };
-        return (is_short ? p.width : p.channels) % v == 0 && whole(p.x, p.x_sn, p.x_sl) && whole(p.y, p.y_sn, p.y_sl) &&
+        const bool lanes_share = is_short || p.width > kNormThreads;  // lanes of one group: its width is whole vectors
+        return (lanes_share ? p.width : p.channels) % v == 0 && whole(p.x, p.x_sn, p.x_sl) && whole(p.y, p.y_sn, p.y_sl) &&
                (!p.z || whole(p.z, p.z_sn, p.z_sl));
     };
     int v = 16 / size;

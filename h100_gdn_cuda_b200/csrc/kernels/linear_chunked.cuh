@@ -31,6 +31,7 @@
 #pragma once
 #include <cuda.h>
 
+#include "pairs.cuh"
 #include "prefill_common.cuh"
 
 namespace gdn {
@@ -185,35 +186,7 @@ constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: V^T), 32 columns
 constexpr uint32_t kTmVd = 448;  // 2 x bf16 (e^{G_L - G_j} V)^T of chunks that are not plain, 32 columns
 constexpr float kPlainLog2 = 60.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// two fp32 values in a 64-bit register pair
-using f2 = unsigned long long;
-__device__ __forceinline__ f2 pk(float lo, float hi) {
-    f2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ f2 pk(uint32_t lo, uint32_t hi) { return pk(__uint_as_float(lo), __uint_as_float(hi)); }
-__device__ __forceinline__ void unpk(f2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
-    f2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
-    f2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ uint32_t pack2(f2 v) {
-    float lo, hi;
-    unpk(v, lo, hi);
-    return ptx::pack_bf16(lo, hi);
-}
+using namespace pairs;
 // the running sums of 64 log2-decays, lane l: tokens l and l + 32
 __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
 #pragma unroll
