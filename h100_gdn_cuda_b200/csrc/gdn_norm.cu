@@ -111,8 +111,8 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
         GDN_REQUIRE(blocks < (1ll << 31), "gdn_group_norm: too many samples");
         GDN_CUDA(launch_dependent(gdn_group_norm_join_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, p));
     }
-    // CTAs of the second launch: four fit an SM; no fewer than eight rows a thread
-    const long long want = std::max<long long>(1, 4 * 148 / std::max<long long>(1, p.n * plan.blocks));
+    // CTAs of the second launch: three fit an SM; no fewer than eight rows a thread
+    const long long want = std::max<long long>(1, 3 * 148 / std::max<long long>(1, p.n * plan.blocks));
     p.apply_rows = static_cast<int>(std::min<long long>(std::max<long long>((p.l + want - 1) / want, 8 * rstep), 1 << 20));
     const dim3 apply(static_cast<unsigned>((p.l + p.apply_rows - 1) / p.apply_rows), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
     GDN_CUDA(launch_dependent(p.z ? gdn_group_norm_apply_kernel<T, V, true> : gdn_group_norm_apply_kernel<T, V, false>, apply, kNormThreads, 0, st, p));

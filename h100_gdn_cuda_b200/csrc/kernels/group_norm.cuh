@@ -263,14 +263,15 @@ __global__ void __launch_bounds__(256) gdn_group_norm_short_kernel(const GroupNo
     }
 }
 
-// Long groups, in two launches: a CTA takes `part_rows` rows of `block_channels` channels (whole groups) of a sample.  The first keeps its part in shared
-// memory, so that the mean is there before the distances are summed, and leaves both per group; the second joins the parts of its sample and
-// writes y.  x is read twice, from L2 the second time where it fits.  (640 channels, 4 x 4095 rows: XX us; with loops over memory and a
-// division per value 62.)
+// Long groups, in two launches: a CTA takes `part_rows` rows of `block_channels` channels (whole groups) of a sample, all of them asked for at once, and
+// keeps them in shared memory, so that the mean is there before the distances are summed; it leaves both per group.  The second launch
+// joins the parts of its sample and writes y; where they are more than a few, a small one between joins them.  x is read twice, from L2
+// the second time where it fits.  (640 channels, 4 x 4095 rows: XX us; with loops over memory and a division per value 62.  A cluster of CTAs
+// that holds a sample in its shared memory reads x once, but took 48: the clusters of eight whole SMs do not all fit at once.)
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxGroups = 64;           // groups of a block
 constexpr int kNormPartBytes = 72 * 1024;    // of a part: three CTAs share an SM
-constexpr int kNormJoinParts = 128;          // more parts than that are joined by a launch of their own (every CTA of the second one reads all of its sample's)
+constexpr int kNormJoinParts = 32;           // more parts than that are joined by a launch of their own (every CTA of the second one reads all of its sample's)
 
 // From the sums of a thread's V channels (rows r0, r0 + rstep, ... of the part) to sums of groups, in `out`.  Everybody calls it.
 template <int V>
@@ -288,7 +289,7 @@ __device__ __forceinline__ void gn_group_sums(const pairs::f2* s, int vecs, int 
     }
     __syncthreads();
     const int l = t & 7;
-    for (int g = t >> 3; g < (groups + 31) / 32 * 32; g += kNormThreads / 8) {
+    for (int g = t >> 3; g < (groups + kNormThreads / 8 - 1) / (kNormThreads / 8) * (kNormThreads / 8); g += kNormThreads / 8) {
         float sum = 0.f;
         if (g < groups)
             for (int r = 0; r < rstep; ++r)
@@ -322,24 +323,23 @@ __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_stats_kernel(cons
     f2 s[P];
 #pragma unroll
     for (int e = 0; e < P; ++e) s[e] = 0ull;
-    constexpr int kUnroll = 16;  // rows in flight
-#pragma unroll 1
-    for (int i = 0; i < mine; i += kUnroll) {
-        gn::Raw<T, V> raw[kUnroll];
+    constexpr int kBytes = V * static_cast<int>(sizeof(T));
+#pragma unroll 4
+    for (int i = 0; i < mine; ++i, x += x_step) {
+        if (kBytes == 16)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(tile + t + i * kNormThreads)), "l"(x) : "memory");
+        else if (kBytes >= 4)
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ptx::smem_u32(tile + t + i * kNormThreads)), "l"(x), "n"(kBytes >= 4 ? kBytes : 4) : "memory");
+        else
+            tile[t + i * kNormThreads] = gn::load<T, V>(x);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (a thread reads what it has copied itself)
+#pragma unroll 4
+    for (int i = 0; i < mine; ++i) {
+        f2 v[P];
+        gn::widen2<T, V>(tile[t + i * kNormThreads], v);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            raw[u] = gn::Raw<T, V>{};
-            if (i + u < mine) raw[u] = gn::load<T, V>(x);
-            x += x_step;
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            f2 v[P];
-            gn::widen2<T, V>(raw[u], v);
-#pragma unroll
-            for (int e = 0; e < P; ++e) s[e] = add2(s[e], v[e]);  // (zero where there is nothing)
-            if (i + u < mine) tile[t + (i + u) * kNormThreads] = raw[u];
-        }
+        for (int e = 0; e < P; ++e) s[e] = add2(s[e], v[e]);
     }
     const float count = static_cast<float>(rows) * static_cast<float>(p.width);
     gn_group_sums<V>(s, vecs, rstep, p.width, groups, scratch, mean);
@@ -373,15 +373,35 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
     if (unit >= p.n * p.groups) return;
     const float2* in = p.partial + unit / p.groups * p.parts * p.groups + unit % p.groups;
     auto count = [&](int i) { return static_cast<float>(min(static_cast<long long>(p.part_rows), p.l - static_cast<long long>(i) * p.part_rows)); };
+    constexpr int kMine = 8;  // entries a lane has in flight, and keeps from the means to the distances where there are no more
+    const int l = threadIdx.x & 31;
+    float2 mine[kMine];
     float sum = 0.f, q = 0.f;
-    for (int i = threadIdx.x & 31; i < p.parts; i += 32) sum += count(i) * __ldcg(in + static_cast<long long>(i) * p.groups).x;
+    auto fetch = [&](int i0) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int i = i0 + l + 32 * j;
+            mine[j] = i < p.parts ? __ldcg(in + static_cast<long long>(i) * p.groups) : make_float2(0.f, 0.f);
+        }
+    };
+    for (int i0 = 0; i0 < p.parts; i0 += 32 * kMine) {
+        fetch(i0);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j)
+            if (i0 + l + 32 * j < p.parts) sum += count(i0 + l + 32 * j) * mine[j].x;
+    }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
     const float mu = sum / static_cast<float>(p.l);
-    for (int i = threadIdx.x & 31; i < p.parts; i += 32) {
-        const float2 part = __ldcg(in + static_cast<long long>(i) * p.groups);
-        const float d = part.x - mu;
-        q += part.y + count(i) * static_cast<float>(p.width) * d * d;
+    for (int i0 = 0; i0 < p.parts; i0 += 32 * kMine) {
+        if (p.parts > 32 * kMine) fetch(i0);
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            if (i0 + l + 32 * j < p.parts) {
+                const float d = mine[j].x - mu;
+                q += mine[j].y + count(i0 + l + 32 * j) * static_cast<float>(p.width) * d * d;
+            }
+        }
     }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
@@ -389,7 +409,7 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
 }
 
 template <typename T, int V, bool kGated>
-__global__ void __launch_bounds__(kNormThreads, 4) gdn_group_norm_apply_kernel(const GroupNormParams p) {
+__global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(const GroupNormParams p) {
     __shared__ float mean[kNormMaxGroups], rstd[kNormMaxGroups];
     const long long n = blockIdx.z, r_first = static_cast<long long>(blockIdx.x) * p.apply_rows;
     const int c_first = blockIdx.y * p.block_channels, channels = min(p.block_channels, p.channels - c_first), groups = channels / p.width;
@@ -410,9 +430,9 @@ __global__ void __launch_bounds__(kNormThreads, 4) gdn_group_norm_apply_kernel(c
     for (int g = t >> 3; g < (groups + 31) / 32 * 32; g += kNormThreads / 8) {
         const float2* in = p.join + n * p.join_parts * p.groups + c_first / p.width + g;
         constexpr int kMine = kNormJoinParts / 8;
-        float sum = 0.f, q = 0.f, mu = 0.f;
+        float sum = 0.f, q = 0.f;
         auto count = [&](int i) { return static_cast<float>(min(p.join_rows, p.l - i * p.join_rows)); };
-        float2 mine[kMine];  // all in flight at once
+        float2 mine[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int i = l + 8 * j;
@@ -422,14 +442,12 @@ __global__ void __launch_bounds__(kNormThreads, 4) gdn_group_norm_apply_kernel(c
         for (int j = 0; j < kMine; ++j) sum += l + 8 * j < p.join_parts ? count(l + 8 * j) * mine[j].x : 0.f;
 #pragma unroll
         for (int m = 4; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-        mu = sum / static_cast<float>(p.l);
-        auto join = [&](int i, float2 part) {
-            const float d = part.x - mu;
-            q += part.y + count(i) * static_cast<float>(p.width) * d * d;
-        };
+        const float mu = sum / static_cast<float>(p.l);
 #pragma unroll
-        for (int j = 0; j < kMine; ++j)
-            if (l + 8 * j < p.join_parts) join(l + 8 * j, mine[j]);
+        for (int j = 0; j < kMine; ++j) {
+            const float d = mine[j].x - mu;
+            if (l + 8 * j < p.join_parts) q += mine[j].y + count(l + 8 * j) * static_cast<float>(p.width) * d * d;
+        }
 #pragma unroll
         for (int m = 4; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
         if (l == 0 && g < groups) {

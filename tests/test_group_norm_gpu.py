@@ -45,7 +45,8 @@ def make(shape, dtype, offset=0.0, seed=0):
 
 
 SHAPES = [((1, 8), 1), ((3, 4096), 32), ((5, 128), 128), ((7, 96), 3), ((2, 1040), 1), ((33, 2 * 1500), 2), ((300, 3 * 80), 3), ((2, 5, 12), 4),
-          ((2, 7, 9), 3), ((1, 1000, 64), 8), ((4, 4095, 40), 2), ((2, 33, 17, 30), 3), ((1, 300, 4100), 1), ((3, 50, 5000), 1000), ((2, 2000, 6), 6), ((1, 1, 4, 1, 16), 2)]
+          ((2, 7, 9), 3), ((1, 1000, 64), 8), ((4, 4095, 40), 2), ((2, 33, 17, 30), 3), ((1, 300, 4100), 1), ((3, 50, 5000), 1000), ((2, 2000, 6), 6), ((1, 1, 4, 1, 16), 2),
+          ((1, 60000, 48), 2), ((2, 9001, 40), 1), ((1, 40000, 320), 5), ((2, 300, 700), 7), ((70, 40, 64), 2), ((1, 50001, 3), 1)]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
