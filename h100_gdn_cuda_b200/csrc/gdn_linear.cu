@@ -30,6 +30,12 @@ int launch_linear_recurrent(const LinRecurrentParams& p, cudaStream_t st) {
     const long long grid = static_cast<long long>(p.batch) * p.vh * ((p.dv + kLinRows - 1) / kLinRows);
     GDN_REQUIRE(grid < (1ll << 31), "gdn_linear_recurrent: too many state tiles");
     const dim3 g(static_cast<unsigned>(grid));
+    if (!p.cu_seqlens && p.seq_len == 1 && !p.num_accepted) {  // (a state per token is then a state per sequence)
+        if (p.dk <= 64) GDN_CUDA(launch_dependent(gdn_linear_decode_kernel<8, kF32>, g, kLinThreads, 0, st, p));
+        else if (p.dk <= 128) GDN_CUDA(launch_dependent(gdn_linear_decode_kernel<16, kF32>, g, kLinThreads, 0, st, p));
+        else GDN_CUDA(launch_dependent(gdn_linear_decode_kernel<32, kF32>, g, kLinThreads, 0, st, p));
+        return GDN_OK;
+    }
     if (p.dk <= 64) GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<8, kF32>, g, kLinThreads, 0, st, p));
     else if (p.dk <= 128) GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<16, kF32>, g, kLinThreads, 0, st, p));
     else GDN_CUDA(launch_dependent(gdn_linear_recurrent_kernel<32, kF32>, g, kLinThreads, 0, st, p));

@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda_bf16.h>
 
+#include "pairs.cuh"
 #include "prefill_common.cuh"
 
 namespace gdn {
@@ -25,10 +26,113 @@ struct LinRecurrentParams {
     float scale;
 };
 
+// One token per sequence.  HBM-bound (the state in and out): nothing is kept beyond a row's own arithmetic, so that many CTAs, all of their loads
+// out at once, fit an SM.  Columns as below.
+template <int LPR, bool kF32>
+__global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 5 : kF32 ? 8 : 10) gdn_linear_decode_kernel(const LinRecurrentParams p) {
+    using namespace ptx;
+    using namespace pairs;
+    constexpr int kRowsAtOnce = 32 / LPR;
+    constexpr int kIter = 8 / kRowsAtOnce;
+    grid_dep_wait();
+    grid_dep_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int l = lane % LPR, sub = lane / LPR;
+    const int row_tiles = (p.dv + kLinRows - 1) / kLinRows;
+    const int unit = blockIdx.x / row_tiles, tile = blockIdx.x - unit * row_tiles;
+    const int seq = unit / p.vh, head = unit - seq * p.vh, khead = head / (p.vh / p.kh);
+    const int slot = p.state_idx ? p.state_idx[seq] : seq;
+    const int c0 = kF32 ? 4 * l : 8 * l, c1 = kF32 ? 4 * (LPR + l) : 8 * l + 4;
+    const bool in0 = c0 < p.dk, in1 = c1 < p.dk;
+    const int row0 = tile * kLinRows + warp * 8 + sub;  // + kRowsAtOnce * i
+    // the token's inputs do not depend on the slot
+    const uint2 zero = make_uint2(0u, 0u);
+    const __nv_bfloat16* const qt = p.q.ptr + seq * p.q.sb + khead * p.q.sh;
+    const __nv_bfloat16* const kt = p.k.ptr + seq * p.k.sb + khead * p.k.sh;
+    const unsigned short* const vt = reinterpret_cast<const unsigned short*>(p.v.ptr + seq * p.v.sb + head * p.v.sh);
+    const uint2 q0 = in0 ? __ldg(reinterpret_cast<const uint2*>(qt + c0)) : zero, q1 = in1 ? __ldg(reinterpret_cast<const uint2*>(qt + c1)) : zero;
+    const uint2 k0 = in0 ? __ldg(reinterpret_cast<const uint2*>(kt + c0)) : zero, k1 = in1 ? __ldg(reinterpret_cast<const uint2*>(kt + c1)) : zero;
+    const uint32_t gate = p.gate.ptr ? p.gate.load_bits(seq, 0, head) : 0u;
+    unsigned short v[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+        const int row = row0 + kRowsAtOnce * i;
+        v[i] = row < p.dv ? __ldg(vt + row) : static_cast<unsigned short>(0);
+    }
+    if (p.state_idx && (slot < 0 || slot >= p.num_slots)) return;  // padding sequence
+    uint4 a[kIter], b[kF32 ? kIter : 1];  // the state as it lies
+    const long long base = slot * p.si_ss + head * p.si_sh + static_cast<long long>(row0) * p.dk;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+        const bool in = p.state_in && row0 + kRowsAtOnce * i < p.dv;
+        const long long at = base + kRowsAtOnce * i * p.dk;
+        a[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (kF32) {
+            const float* src = static_cast<const float*>(p.state_in) + at;
+            b[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (in && in0) a[i] = *reinterpret_cast<const uint4*>(src + c0);
+            if (in && in1) b[i] = *reinterpret_cast<const uint4*>(src + c1);
+        } else if (in && in0) {
+            a[i] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.state_in) + at + c0);
+        }
+    }
+    const float decay = __expf(p.gate.value(gate));
+    const f2 d2 = pk(decay, decay);
+    f2 k[4] = {pk(bf16_lo(k0.x), bf16_hi(k0.x)), pk(bf16_lo(k0.y), bf16_hi(k0.y)), pk(bf16_lo(k1.x), bf16_hi(k1.x)), pk(bf16_lo(k1.y), bf16_hi(k1.y))};
+    f2 q[4] = {pk(bf16_lo(q0.x), bf16_hi(q0.x)), pk(bf16_lo(q0.y), bf16_hi(q0.y)), pk(bf16_lo(q1.x), bf16_hi(q1.x)), pk(bf16_lo(q1.y), bf16_hi(q1.y))};
+    const long long to = slot * p.so_ss + head * p.so_sh + static_cast<long long>(row0) * p.dk;
+    float o[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+        const float vf = __uint_as_float(static_cast<uint32_t>(v[i]) << 16);
+        const f2 v2 = pk(vf, vf);
+        f2 s[4];
+        if (kF32) {
+            s[0] = pk(a[i].x, a[i].y); s[1] = pk(a[i].z, a[i].w);
+            s[2] = pk(b[i].x, b[i].y); s[3] = pk(b[i].z, b[i].w);
+        } else {
+            s[0] = pk(bf16_lo(a[i].x), bf16_hi(a[i].x)); s[1] = pk(bf16_lo(a[i].y), bf16_hi(a[i].y));
+            s[2] = pk(bf16_lo(a[i].z), bf16_hi(a[i].z)); s[3] = pk(bf16_lo(a[i].w), bf16_hi(a[i].w));
+        }
+        f2 sum = 0ull;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s[e] = fma2(s[e], d2, mul2(v2, k[e]));
+            sum = fma2(s[e], q[e], sum);
+        }
+        float lo, hi;
+        unpk(sum, lo, hi);
+        o[i] = lo + hi;
+        if (p.state_out && row0 + kRowsAtOnce * i < p.dv) {
+            const long long at = to + kRowsAtOnce * i * p.dk;
+            if (kF32) {
+                float* dst = static_cast<float*>(p.state_out) + at;
+                float4 x, y;
+                unpk(s[0], x.x, x.y); unpk(s[1], x.z, x.w);
+                unpk(s[2], y.x, y.y); unpk(s[3], y.z, y.w);
+                if (in0) *reinterpret_cast<float4*>(dst + c0) = x;
+                if (in1) *reinterpret_cast<float4*>(dst + c1) = y;
+            } else if (in0) {
+                *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.state_out) + at + c0) = make_uint4(pack2(s[0]), pack2(s[1]), pack2(s[2]), pack2(s[3]));
+            }
+        }
+    }
+#pragma unroll
+    for (int m = LPR / 2; m > 0; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) o[i] += __shfl_xor_sync(0xffffffffu, o[i], m);
+    __nv_bfloat16* const op = p.out.ptr + seq * p.out.sb + head * p.out.sh;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+        const int row = row0 + kRowsAtOnce * i;
+        if (l == 0 && row < p.dv) op[row] = __float2bfloat16(p.scale * o[i]);
+    }
+}
+
 // LPR lanes share a row, 8 columns each: dk <= 8 LPR.  bf16 states: lane l holds columns 8 l .. 8 l + 7.  fp32 states: columns
 // 4 l .. and 4 (LPR + l) .., so that a warp's 16-byte accesses are contiguous.
 template <int LPR, bool kF32>
-__global__ void __launch_bounds__(kLinThreads) gdn_linear_recurrent_kernel(const LinRecurrentParams p) {
+__global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_recurrent_kernel(const LinRecurrentParams p) {
     using namespace ptx;
     constexpr int kRowsAtOnce = 32 / LPR;
     constexpr int kIter = 8 / kRowsAtOnce;  // rows per thread

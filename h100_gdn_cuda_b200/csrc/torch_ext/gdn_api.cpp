@@ -585,20 +585,27 @@ at::Tensor group_norm(const at::Tensor& x, int64_t num_groups, const std::option
     on_device(weight, x, "weight");
     on_device(bias, x, "bias");
     on_device(z, x, "z");
-    // (samples, rows, channels) with contiguous channels: a view where the axes between can be one
-    auto rows_of = [&](const at::Tensor& t) {
-        if (t.stride(-1) != 1 && C > 1) return t.contiguous().view({N, -1, C});
-        if (t.dim() == 2) return t.unsqueeze(1);
-        if (t.dim() == 3) return t;
-        return t.is_contiguous() ? t.view({N, -1, C}) : t.reshape({N, x.numel() / std::max<int64_t>(N * C, 1), C});
+    // (samples, rows, channels) with contiguous channels: as it lies where the axes between are one
+    struct Rows {
+        at::Tensor t;
+        int64_t rows, stride_sample, stride_row;
+    };
+    auto rows_of = [&](const at::Tensor& given) {
+        at::Tensor t = given.stride(-1) != 1 && C > 1 ? given.contiguous() : given;
+        if (t.dim() == 2) return Rows{t, 1, t.stride(0), 0};
+        if (t.dim() > 3) t = t.reshape({N, t.numel() / (N * C), C});
+        return Rows{t, t.size(1), t.stride(0), t.stride(1)};
     };
     at::Tensor y = empty(x.sizes(), x, x.scalar_type()), w, b;
     if (x.numel() == 0) return y;
-    const at::Tensor xr = rows_of(x), yr = rows_of(y);
-    at::Tensor zr;
+    const Rows xr = rows_of(x);
+    Rows zr{};
     if (z.has_value()) {
         require(z->sizes() == x.sizes() && z->scalar_type() == x.scalar_type(), "z must have the shape and dtype of x");
         zr = rows_of(*z);
+        a.z = zr.t.data_ptr();
+        a.z_stride_sample = zr.stride_sample;
+        a.z_stride_row = zr.stride_row;
     }
     for (const auto* t : {&weight, &bias})
         if (t->has_value()) {
@@ -608,23 +615,18 @@ at::Tensor group_norm(const at::Tensor& x, int64_t num_groups, const std::option
     if (weight.has_value()) w = weight->contiguous();
     if (bias.has_value()) b = bias->contiguous();
     require(!w.defined() || !b.defined() || w.scalar_type() == b.scalar_type(), "weight and bias must share a dtype");
-    a.x = xr.data_ptr();
-    a.y = yr.data_ptr();
-    a.z = zr.defined() ? zr.data_ptr() : nullptr;
+    a.x = xr.t.data_ptr();
+    a.y = y.data_ptr();
     a.weight = w.defined() ? w.data_ptr() : nullptr;
     a.bias = b.defined() ? b.data_ptr() : nullptr;
     a.samples = N;
-    a.rows = xr.size(1);
+    a.rows = xr.rows;
     a.channels = static_cast<int32_t>(C);
     a.groups = static_cast<int32_t>(num_groups);
-    a.x_stride_sample = xr.stride(0);
-    a.x_stride_row = xr.stride(1);
-    a.y_stride_sample = yr.stride(0);
-    a.y_stride_row = yr.stride(1);
-    if (zr.defined()) {
-        a.z_stride_sample = zr.stride(0);
-        a.z_stride_row = zr.stride(1);
-    }
+    a.x_stride_sample = xr.stride_sample;
+    a.x_stride_row = xr.stride_row;
+    a.y_stride_sample = xr.rows * C;
+    a.y_stride_row = C;
     a.eps = eps;
     a.silu = activation ? 1 : 0;
     at::Tensor ws;
