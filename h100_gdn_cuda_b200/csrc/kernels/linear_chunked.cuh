@@ -622,9 +622,8 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
     } else if (warp == 20) {
         // =============================================================== producer
-        // A stage's loads are issued two chunks before their use, sooner than DRAM under load answers: they are asked for kLead chunks ahead, so
-        // that L2 has them by then.
-        constexpr int kLead = 4;
+        // (A stage's loads are issued two chunks before their use.  Asking L2 for chunks further ahead costs more than it brings: 4 x 4096 tokens 89
+        // -> 99 us, 148 heads of 4096 111 -> 164, from DRAM.)
         while (next_item()) {
             const int khead = __shfl_sync(0xffffffffu, it.khead, 0), head = __shfl_sync(0xffffffffu, it.head, 0), batch = __shfl_sync(0xffffffffu, it.batch, 0);
             const int tok0 = __shfl_sync(0xffffffffu, it.tok0, 0), dvt = __shfl_sync(0xffffffffu, it.dvt, 0);
@@ -633,33 +632,21 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 const uint32_t s = gc % kStages;
                 mbar_wait_short(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
                 uint8_t* st = smem + s * L::kStage;
-                const int tok = tok0 + c * kChunk, ahead = tok + kLead * kChunk;
+                const int tok = tok0 + c * kChunk;
                 if (elect_one()) {
                     mbar_arrive_expect_tx(&bar_full[s], L::kStage);
                     if (kWhole) {
                         tma_load_5d(st + L::kOffK, &tmK, &bar_full[s], 0, tok, 0, khead, batch);
                         tma_load_5d(st + L::kOffQ, &tmQ, &bar_full[s], 0, tok, 0, khead, batch);
                         tma_load_5d(st + L::kOffV, &tmV, &bar_full[s], 0, tok, 2 * dvt, head, batch);
-                        if (c + kLead < it.chunks) {
-                            tma_prefetch_5d(&tmK, 0, ahead, 0, khead, batch);
-                            tma_prefetch_5d(&tmQ, 0, ahead, 0, khead, batch);
-                            tma_prefetch_5d(&tmV, 0, ahead, 2 * dvt, head, batch);
-                        }
                     } else {
 #pragma unroll 1
                         for (int a = 0; a < DK / 64; ++a) {
                             tma_load_4d(st + L::kOffK + a * 8192, &tmK, &bar_full[s], a * 64, khead, tok, batch);
                             tma_load_4d(st + L::kOffQ + a * 8192, &tmQ, &bar_full[s], a * 64, khead, tok, batch);
-                            if (c + kLead < it.chunks) {
-                                tma_prefetch_4d(&tmK, a * 64, khead, ahead, batch);
-                                tma_prefetch_4d(&tmQ, a * 64, khead, ahead, batch);
-                            }
                         }
 #pragma unroll 1
-                        for (int a = 0; a < DV / 64; ++a) {
-                            tma_load_4d(st + L::kOffV + a * 8192, &tmV, &bar_full[s], dvt * 128 + a * 64, head, tok, batch);
-                            if (c + kLead < it.chunks) tma_prefetch_4d(&tmV, dvt * 128 + a * 64, head, ahead, batch);
-                        }
+                        for (int a = 0; a < DV / 64; ++a) tma_load_4d(st + L::kOffV + a * 8192, &tmV, &bar_full[s], dvt * 128 + a * 64, head, tok, batch);
                     }
                 }
                 __syncwarp();

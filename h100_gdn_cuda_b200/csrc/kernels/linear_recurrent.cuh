@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 5 : kF32 ? 8 : 10) gd
 template <int LPR, bool kF32>
 __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_recurrent_kernel(const LinRecurrentParams p) {
     using namespace ptx;
+    using namespace pairs;
     constexpr int kRowsAtOnce = 32 / LPR;
     constexpr int kIter = 8 / kRowsAtOnce;  // rows per thread
     grid_dep_wait();
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_rec
     const bool in0 = c0 < p.dk, in1 = c1 < p.dk;
     const int row0 = tile * kLinRows + warp * 8 + sub;  // + kRowsAtOnce * i
     auto state_offset = [&](int i) { return static_cast<long long>(row0 + kRowsAtOnce * i) * p.dk; };
-    float S[kIter][8];
+    f2 S[kIter][4];
     if (p.state_in) {
         const long long base = static_cast<long long>(slot) * p.si_ss + static_cast<long long>(head) * p.si_sh;
 #pragma unroll
@@ -176,20 +177,20 @@ __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_rec
                 const float* src = static_cast<const float*>(p.state_in) + base + state_offset(i);
                 const float4 a = row_in && in0 ? *reinterpret_cast<const float4*>(src + c0) : make_float4(0.f, 0.f, 0.f, 0.f);
                 const float4 b = row_in && in1 ? *reinterpret_cast<const float4*>(src + c1) : make_float4(0.f, 0.f, 0.f, 0.f);
-                S[i][0] = a.x; S[i][1] = a.y; S[i][2] = a.z; S[i][3] = a.w;
-                S[i][4] = b.x; S[i][5] = b.y; S[i][6] = b.z; S[i][7] = b.w;
+                S[i][0] = pk(a.x, a.y); S[i][1] = pk(a.z, a.w);
+                S[i][2] = pk(b.x, b.y); S[i][3] = pk(b.z, b.w);
             } else {
                 const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.state_in) + base + state_offset(i);
                 const uint4 a = row_in && in0 ? *reinterpret_cast<const uint4*>(src + c0) : make_uint4(0u, 0u, 0u, 0u);
-                S[i][0] = bf16_lo(a.x); S[i][1] = bf16_hi(a.x); S[i][2] = bf16_lo(a.y); S[i][3] = bf16_hi(a.y);
-                S[i][4] = bf16_lo(a.z); S[i][5] = bf16_hi(a.z); S[i][6] = bf16_lo(a.w); S[i][7] = bf16_hi(a.w);
+                S[i][0] = pk(bf16_lo(a.x), bf16_hi(a.x)); S[i][1] = pk(bf16_lo(a.y), bf16_hi(a.y));
+                S[i][2] = pk(bf16_lo(a.z), bf16_hi(a.z)); S[i][3] = pk(bf16_lo(a.w), bf16_hi(a.w));
             }
         }
     } else {
 #pragma unroll
         for (int i = 0; i < kIter; ++i)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) S[i][e] = 0.f;
+            for (int e = 0; e < 4; ++e) S[i][e] = 0ull;
     }
     auto store_state = [&](long long where) {
         const long long base = where * p.so_ss + static_cast<long long>(head) * p.so_sh;
@@ -198,13 +199,15 @@ __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_rec
             if (row0 + kRowsAtOnce * i >= p.dv) continue;
             if (kF32) {
                 float* dst = static_cast<float*>(p.state_out) + base + state_offset(i);
-                if (in0) *reinterpret_cast<float4*>(dst + c0) = make_float4(S[i][0], S[i][1], S[i][2], S[i][3]);
-                if (in1) *reinterpret_cast<float4*>(dst + c1) = make_float4(S[i][4], S[i][5], S[i][6], S[i][7]);
+                float4 a, b;
+                unpk(S[i][0], a.x, a.y); unpk(S[i][1], a.z, a.w);
+                unpk(S[i][2], b.x, b.y); unpk(S[i][3], b.z, b.w);
+                if (in0) *reinterpret_cast<float4*>(dst + c0) = a;
+                if (in1) *reinterpret_cast<float4*>(dst + c1) = b;
             } else {
                 __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.state_out) + base + state_offset(i);
                 if (in0)
-                    *reinterpret_cast<uint4*>(dst + c0) = make_uint4(pack_bf16(S[i][0], S[i][1]), pack_bf16(S[i][2], S[i][3]),
-                                                                     pack_bf16(S[i][4], S[i][5]), pack_bf16(S[i][6], S[i][7]));
+                    *reinterpret_cast<uint4*>(dst + c0) = make_uint4(pack2(S[i][0]), pack2(S[i][1]), pack2(S[i][2]), pack2(S[i][3]));
             }
         }
     };
@@ -237,23 +240,29 @@ __global__ void __launch_bounds__(kLinThreads, LPR == 32 ? 4 : 7) gdn_linear_rec
     for (long long t = 0; t < tokens; ++t) {
         if (t + 1 < tokens) load_token(tok0 + t + 1, next);
         const float decay = __expf(p.gate.value(cur.g));
-        float q[8], k[8], o[kIter];
+        const f2 d2 = pk(decay, decay);
+        f2 q[4], k[4];
+        float o[kIter];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            q[4 * h] = bf16_lo(cur.q[h].x); q[4 * h + 1] = bf16_hi(cur.q[h].x);
-            q[4 * h + 2] = bf16_lo(cur.q[h].y); q[4 * h + 3] = bf16_hi(cur.q[h].y);
-            k[4 * h] = bf16_lo(cur.k[h].x); k[4 * h + 1] = bf16_hi(cur.k[h].x);
-            k[4 * h + 2] = bf16_lo(cur.k[h].y); k[4 * h + 3] = bf16_hi(cur.k[h].y);
+            q[2 * h] = pk(bf16_lo(cur.q[h].x), bf16_hi(cur.q[h].x));
+            q[2 * h + 1] = pk(bf16_lo(cur.q[h].y), bf16_hi(cur.q[h].y));
+            k[2 * h] = pk(bf16_lo(cur.k[h].x), bf16_hi(cur.k[h].x));
+            k[2 * h + 1] = pk(bf16_lo(cur.k[h].y), bf16_hi(cur.k[h].y));
         }
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {
-            const float v = __uint_as_float(static_cast<uint32_t>(cur.v[i]) << 16);
-            o[i] = 0.f;
+            const float vf = __uint_as_float(static_cast<uint32_t>(cur.v[i]) << 16);
+            const f2 v2 = pk(vf, vf);
+            f2 sum = 0ull;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                S[i][e] = fmaf(S[i][e], decay, v * k[e]);
-                o[i] = fmaf(S[i][e], q[e], o[i]);
+            for (int e = 0; e < 4; ++e) {
+                S[i][e] = fma2(S[i][e], d2, mul2(v2, k[e]));
+                sum = fma2(S[i][e], q[e], sum);
             }
+            float lo, hi;
+            unpk(sum, lo, hi);
+            o[i] = lo + hi;
         }
 #pragma unroll
         for (int i = 0; i < kIter; ++i) {

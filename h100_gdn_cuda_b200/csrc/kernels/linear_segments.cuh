@@ -145,17 +145,12 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             const int s = n % kStages;
             mbar_wait_short(&bar_empty[s], ((n / kStages) + 1) & 1, abort_flag);
             uint8_t* st = smem + s * L::kStage;
-            constexpr int kLead = 4;
-            const int tok = tok0 + (chunks - 1 - n) * kChunk, ahead = tok - kLead * kChunk;
+            const int tok = tok0 + (chunks - 1 - n) * kChunk;
             if (elect_one()) {
                 mbar_arrive_expect_tx(&bar_full[s], L::kStage);
                 if (kWhole) {
                     tma_load_5d(st, &tmK, &bar_full[s], 0, tok, 0, khead, batch);
                     tma_load_5d(st + L::kOffV, &tmV, &bar_full[s], 0, tok, 2 * dvt, head, batch);
-                    if (n + kLead < chunks) {
-                        tma_prefetch_5d(&tmK, 0, ahead, 0, khead, batch);
-                        tma_prefetch_5d(&tmV, 0, ahead, 2 * dvt, head, batch);
-                    }
                 } else {
 #pragma unroll 1
                     for (int a = 0; a < DK / 64; ++a) tma_load_4d(st + a * 8192, &tmK, &bar_full[s], a * 64, khead, tok, batch);

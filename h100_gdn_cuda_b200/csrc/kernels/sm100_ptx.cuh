@@ -187,12 +187,6 @@ GDN_DEVICE void tma_load_5d(void* dst, const void* tmap, uint64_t* bar, int c0, 
         ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
         : "memory");
 }
-GDN_DEVICE void tma_prefetch_5d(const void* tmap, int c0, int c1, int c2, int c3, int c4) {
-    asm volatile("cp.async.bulk.prefetch.tensor.5d.L2.global.tile [%0, {%1, %2, %3, %4, %5}];" ::"l"(
-                     reinterpret_cast<uint64_t>(tmap)),
-                 "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4)
-                 : "memory");
-}
 // Warp-collective TMA loads: the converged warp calls them with warp-uniform arguments and one
 // elected lane issues (keeps the tensor-map address and coordinates in uniform registers).
 GDN_DEVICE void tma_load_4d_w(void* dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2, int c3) {
