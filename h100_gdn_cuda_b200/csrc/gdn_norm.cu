@@ -35,7 +35,7 @@ NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int 
     return plan;
 }
 
-constexpr int kShortValues = 1024;  // values of a (sample, group) that stay in the registers of a warp
+constexpr int kShortValues = 512;  // values of a (sample, group) that stay in the registers of a warp (1024: 65536 groups 100 -> 150 us and more)
 bool short_groups(int64_t rows, int width) { return rows * width <= kShortValues; }
 
 template <typename T, int V>
@@ -119,9 +119,51 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     return GDN_OK;
 }
 
+// Shared memory of a CTA of `threads` that keeps a (sample, group); 0: it does not fit.
+int whole_bytes(int64_t rows, int width, int vec, int size, int threads) {
+    if (vec * size < 4 || width % vec != 0 || width / vec > threads) return 0;
+    const int rstep = threads / (width / vec);
+    const int64_t bytes = (rows + rstep - 1) / rstep * threads * vec * size;
+    return bytes <= kNormWholeBytes ? static_cast<int>(bytes) : 0;
+}
+// One launch that reads x once is faster than two or three that read it twice (4 x 32 groups of 16 KB 8.5 -> 2.8 us, of 64 KB 18 -> 7,
+// of 150 KB 24 -> 14), except where
+//  - very many groups are so small that the CTAs' turn-over shows (65536 groups of 2 KB 99 -> 280 us), or
+//  - a group's piece of a row is not whole sectors of 32 bytes: copies of less than 16 bytes go through L1, of which the tile leaves little (20
+//    channels, bf16, 32 groups of 200 KB 21 -> 30 us, of 150 KB 20 -> 16), and where CTAs come in several waves, or read a gate as well, the
+//    sectors that groups share move twice (512 groups of 64 KB 33 -> 42 us, 256 of 40 KB 20 -> 14; gated, 512 of 48 KB 30 -> 42, of 16 KB 19 -> 11).
+bool whole_groups(int64_t count, int64_t rows, int width, int vec, int size, bool gated) {
+    const int bytes = whole_bytes(rows, width, vec, size, 1024);
+    if (bytes == 0 || (rows * width * size < 16 * 1024 && count > 2048)) return false;
+    return width * size % 32 == 0 || bytes <= (gated ? 24 : count > 148 ? 48 : 176) * 1024;
+}
+
 template <typename T, int V>
-int launch_norm(const GroupNormParams& p, bool is_short, const GdnGroupNormArgs& a, cudaStream_t st) {
+int launch_whole(const GroupNormParams& p, cudaStream_t st) {
+    GDN_REQUIRE(p.n * p.groups < (1ll << 31), "gdn_group_norm: too many samples");
+    auto launch = [&](auto gated) -> int {
+        constexpr bool kG = decltype(gated)::value;
+        const int small = whole_bytes(p.l, p.width, V, sizeof(T), 256);
+        const unsigned grid = static_cast<unsigned>(p.n * p.groups);
+        // (512 groups of 64 KB: 29 us with CTAs of 1024 threads, 20 with three of 256 on an SM; of 150 KB: 51 and 54.  Copies that go through L1
+        // are better few at a time: 128 groups of 160 KB, 20 channels, 21 and 19)
+        if (small > 0 && (small <= kNormPartBytes || V * sizeof(T) < 16)) {
+            if (int rc = set_smem<gdn_group_norm_whole_kernel<T, V, 256, kG>>(kNormWholeBytes)) return rc;
+            GDN_CUDA(launch_dependent(gdn_group_norm_whole_kernel<T, V, 256, kG>, grid, 256, small, st, p));
+        } else {
+            if (int rc = set_smem<gdn_group_norm_whole_kernel<T, V, 1024, kG>>(kNormWholeBytes)) return rc;
+            GDN_CUDA(launch_dependent(gdn_group_norm_whole_kernel<T, V, 1024, kG>, grid, 1024, whole_bytes(p.l, p.width, V, sizeof(T), 1024), st, p));
+        }
+        return GDN_OK;
+    };
+    return p.z ? launch(std::true_type{}) : launch(std::false_type{});
+}
+
+template <typename T, int V>
+int launch_norm(const GroupNormParams& p, bool is_short, bool is_whole, const GdnGroupNormArgs& a, cudaStream_t st) {
     if (is_short) return launch_short<T, V>(p, st);
+    if constexpr (V * sizeof(T) >= 4)
+        if (is_whole) return launch_whole<T, V>(p, st);
     return launch_long<T, V>(p, norm_plan(a.samples, a.rows, a.channels, a.groups, V, sizeof(T)), st);
 }
 
@@ -167,26 +209,31 @@ int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
     }
     // the widest access, up to 16 bytes, that pointers, strides and (where lanes share a group) the group's width allow
     const int size = a->dtype == GDN_F32 ? 4 : 2;
-    auto fits = [&](int v) {
+    auto fits = [&](int v, bool lanes_share) {  // lanes of one group: its width is whole vectors
         auto whole = [&](const void* ptr, int64_t sn, int64_t sl) {
             return reinterpret_cast<uintptr_t>(ptr) % (static_cast<unsigned>(v * size)) == 0 && (a->samples == 1 || sn % v == 0) && (a->rows == 1 || sl % v == 0);
         };
-        const bool lanes_share = is_short || p.width > kNormThreads;  // lanes of one group: its width is whole vectors
         return (lanes_share ? p.width : p.channels) % v == 0 && whole(p.x, p.x_sn, p.x_sl) && whole(p.y, p.y_sn, p.y_sl) &&
                (!p.z || whole(p.z, p.z_sn, p.z_sl));
     };
-    int v = 16 / size;
-    while (!fits(v)) v /= 2;
+    auto widest = [&](bool lanes_share) {
+        int v = 16 / size;
+        while (!fits(v, lanes_share)) v /= 2;
+        return v;
+    };
+    const int shared = widest(true);
+    const bool is_whole = !is_short && whole_groups(a->samples * a->groups, a->rows, p.width, shared, size, p.z != nullptr);
+    const int v = is_short || is_whole || p.width > kNormThreads ? shared : widest(false);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a->dtype == GDN_F32) {
-        if (v == 4) return launch_norm<float, 4>(p, is_short, *a, st);
-        if (v == 2) return launch_norm<float, 2>(p, is_short, *a, st);
-        return launch_norm<float, 1>(p, is_short, *a, st);
+        if (v == 4) return launch_norm<float, 4>(p, is_short, is_whole, *a, st);
+        if (v == 2) return launch_norm<float, 2>(p, is_short, is_whole, *a, st);
+        return launch_norm<float, 1>(p, is_short, is_whole, *a, st);
     }
-    if (v == 8) return launch_norm<__nv_bfloat16, 8>(p, is_short, *a, st);
-    if (v == 4) return launch_norm<__nv_bfloat16, 4>(p, is_short, *a, st);
-    if (v == 2) return launch_norm<__nv_bfloat16, 2>(p, is_short, *a, st);
-    return launch_norm<__nv_bfloat16, 1>(p, is_short, *a, st);
+    if (v == 8) return launch_norm<__nv_bfloat16, 8>(p, is_short, is_whole, *a, st);
+    if (v == 4) return launch_norm<__nv_bfloat16, 4>(p, is_short, is_whole, *a, st);
+    if (v == 2) return launch_norm<__nv_bfloat16, 2>(p, is_short, is_whole, *a, st);
+    return launch_norm<__nv_bfloat16, 1>(p, is_short, is_whole, *a, st);
 }
 
 }  // extern "C"

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256, kPass == 1 ? 4 : 2) gdn_group_norm_rows_k
     }
 }
 
-// Short groups of several rows (L W up to 1024 values): LPR lanes per (sample, group), the values in registers.
+// Short groups of several rows (L W up to 512 values): LPR lanes per (sample, group), the values in registers.
 template <typename T, int V, int LPR, int kPass>
 __global__ void __launch_bounds__(256) gdn_group_norm_short_kernel(const GroupNormParams p) {
     ptx::grid_dep_wait();
@@ -263,14 +263,132 @@ __global__ void __launch_bounds__(256) gdn_group_norm_short_kernel(const GroupNo
     }
 }
 
+// Groups that a CTA's shared memory holds: a CTA per (sample, group), x read once and y written in one launch.  Neighbouring groups' pieces of a row may
+// share a sector: L2 joins them.  Large groups are bound by one SM's rate of copies and of SiLU's
+// exponentials, one after the other (640 channels, 4 x 4095 rows, 128 CTAs: 18 us, of which 6 are DRAM's).
+constexpr int kNormWholeBytes = 224 * 1024;
+constexpr int kNormPartBytes = 72 * 1024;  // three CTAs share an SM
+
+// the sum over a CTA of `kWarps` warps; everybody gets it
+template <int kWarps>
+__device__ __forceinline__ float gn_block_sum(float v, float* part) {
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float sum = static_cast<int>(threadIdx.x & 31) < kWarps ? part[threadIdx.x & 31] : 0.f;
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    __syncthreads();
+    return sum;
+}
+
+template <typename T, int V, int kThreads, bool kGated>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) gdn_group_norm_whole_kernel(const GroupNormParams p) {
+    extern __shared__ __align__(16) uint8_t tile_raw[];
+    __shared__ float part[kThreads / 32];
+    ptx::grid_dep_wait();
+    ptx::grid_dep_launch();
+    using namespace pairs;
+    constexpr int P = gn::kPairs<V>;
+    const long long n = blockIdx.x / p.groups;
+    const int c_first = static_cast<int>(blockIdx.x % p.groups) * p.width, rows = static_cast<int>(p.l);
+    const int vecs = p.width / V, rstep = kThreads / vecs, t = threadIdx.x, vec = t % vecs, r0 = t / vecs;  // (r0 == rstep: an idle thread)
+    const int mine = r0 < rstep && r0 < rows ? (rows - r0 + rstep - 1) / rstep : 0, c = c_first + vec * V;
+    gn::Raw<T, V>* const tile = reinterpret_cast<gn::Raw<T, V>*>(tile_raw) + t;  // this thread's rows, kThreads apart
+    {
+        const T* x = static_cast<const T*>(p.x) + n * p.x_sn + r0 * p.x_sl + c;
+        const long long step = rstep * p.x_sl;
+        constexpr int kBytes = V * static_cast<int>(sizeof(T));
+#pragma unroll 4
+        for (int i = 0; i < mine; ++i, x += step) {
+            if (kBytes == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ptx::smem_u32(tile + i * kThreads)), "l"(x) : "memory");
+            else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(ptx::smem_u32(tile + i * kThreads)), "l"(x), "n"(kBytes) : "memory");
+        }
+    }
+    f2 w[P], b[P], s[P];
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+        const int ca = c + 2 * e, cb = V > 1 ? ca + 1 : ca;
+        w[e] = pk(gn::param(p.weight, p.param_f32, ca, 1.f), gn::param(p.weight, p.param_f32, cb, 1.f));
+        b[e] = pk(gn::param(p.bias, p.param_f32, ca, 0.f), gn::param(p.bias, p.param_f32, cb, 0.f));
+        s[e] = 0ull;
+    }
+    auto total = [&]() {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            float lo, hi;
+            unpk(s[e], lo, hi);
+            sum += V > 1 ? lo + hi : lo;
+            s[e] = 0ull;
+        }
+        return gn_block_sum<kThreads / 32>(sum, part);
+    };
+    asm volatile("cp.async.wait_all;" ::: "memory");  // (a thread reads what it has copied itself)
+#pragma unroll 4
+    for (int i = 0; i < mine; ++i) {
+        f2 v[P];
+        gn::widen2<T, V>(tile[i * kThreads], v);
+#pragma unroll
+        for (int e = 0; e < P; ++e) s[e] = add2(s[e], v[e]);
+    }
+    const float count = static_cast<float>(rows) * static_cast<float>(p.width), mean = total() / count;
+    const f2 m = pk(-mean, -mean);
+#pragma unroll 4
+    for (int i = 0; i < mine; ++i) {
+        f2 v[P];
+        gn::widen2<T, V>(tile[i * kThreads], v);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+            const f2 d = add2(v[e], m);
+            s[e] = fma2(d, d, s[e]);
+        }
+    }
+    const float rstd = rsqrtf(total() / count + p.eps);
+    const f2 rstd2 = pk(rstd, rstd);
+#pragma unroll
+    for (int e = 0; e < P; ++e) w[e] = mul2(w[e], rstd2);
+    const T* z = static_cast<const T*>(p.z) + n * p.z_sn + r0 * p.z_sl + c;
+    T* y = static_cast<T*>(p.y) + n * p.y_sn + r0 * p.y_sl + c;
+    const long long z_step = rstep * p.z_sl, y_step = rstep * p.y_sl;
+    constexpr int kUnroll = 4;  // rows in flight
+    const bool silu = p.silu != 0;
+#pragma unroll 1
+    for (int i = 0; i < mine; i += kUnroll) {
+        gn::Raw<T, V> zr[kUnroll];
+        if (kGated) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (i + u < mine) zr[u] = gn::load<T, V>(z);
+                z += z_step;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            if (i + u >= mine) break;
+            f2 v[P], g[P];
+            gn::widen2<T, V>(tile[(i + u) * kThreads], v);
+            if (kGated) gn::widen2<T, V>(zr[u], g);
+#pragma unroll
+            for (int e = 0; e < P; ++e) {
+                const f2 t2 = fma2(add2(v[e], m), w[e], b[e]);
+                if (kGated) v[e] = mul2(t2, silu ? silu2(g[e]) : g[e]);
+                else v[e] = silu ? silu2(t2) : t2;
+            }
+            gn::store2<T, V>(y, v);
+            y += y_step;
+        }
+    }
+}
+
 // Long groups, in two launches: a CTA takes `part_rows` rows of `block_channels` channels (whole groups) of a sample, all of them asked for at once, and
 // keeps them in shared memory, so that the mean is there before the distances are summed; it leaves both per group.  The second launch
 // joins the parts of its sample and writes y; where they are more than a few, a small one between joins them.  x is read twice, from L2
-// the second time where it fits.  (640 channels, 4 x 4095 rows: XX us; with loops over memory and a division per value 62.  A cluster of CTAs
+// the second time where it fits.  (640 channels, 4 x 4095 rows: 25 us; with loops over memory and a division per value 62.  A cluster of CTAs
 // that holds a sample in its shared memory reads x once, but took 48: the clusters of eight whole SMs do not all fit at once.)
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxGroups = 64;           // groups of a block
-constexpr int kNormPartBytes = 72 * 1024;    // of a part: three CTAs share an SM
 constexpr int kNormJoinParts = 32;           // more parts than that are joined by a launch of their own (every CTA of the second one reads all of its sample's)
 
 // From the sums of a thread's V channels (rows r0, r0 + rstep, ... of the part) to sums of groups, in `out`.  Everybody calls it.

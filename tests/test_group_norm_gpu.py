@@ -118,3 +118,18 @@ def test_refusals():
                 lambda: gdn.group_norm(x, 3, z=z.bfloat16()), lambda: gdn.group_norm(x, 3, w.cpu())):
         with pytest.raises(RuntimeError):
             bad()
+
+
+# around the limits of the kernel that keeps a group in shared memory: 16 KB, 72 KB, 176 and 224 KB of a group, rows of whole sectors and not, more
+# groups than SMs, very many small groups, a width that only pairs or single values divide
+WHOLE = [((2, 1023, 64), 4), ((1, 2304, 32), 2), ((1, 2305, 32), 2), ((1, 7167, 32), 2), ((1, 7169, 32), 2), ((1, 4481, 60), 3), ((1, 3001, 60), 3),
+         ((40, 500, 80), 4), ((40, 700, 80), 4), ((1100, 40, 32), 2), ((3, 900, 22), 2), ((3, 2000, 21), 3), ((1, 9, 9000), 1), ((2, 3, 4100), 2), ((1, 13, 8200), 1)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,G", WHOLE, ids=str)
+def test_groups_in_shared_memory(shape, G, dtype):
+    x, z, w, b = make(shape, dtype, 3.0)
+    check(gdn.group_norm(x, G, w, b, z), x, G, w, b, z)
+    check(gdn.group_norm(x, G, w, b), x, G, w, b)
+    check(gdn.group_norm(x, G, None, None, None, 1e-5, False), x, G, None, None, None, 1e-5, False)
