@@ -719,8 +719,8 @@ def linear_attention_recurrent(query, key, value, initial_state=None, gate=None,
         S <- exp(gate) S + v k^T ,   o = scale S q .
 
     query/key (B,T,kh,dk) or packed (N,kh,dk) with cu_seqlens, value (B,T,vh,dv) / (N,vh,dv), bf16, head dims up to 256; `gate` holds log-decays
-    (<= 0; -inf forgets all before the token), bf16 or fp32: (vh), one per head, or (B,T,vh) / (N,vh), one per token and head; None: no decay.  The state is (sequences,vh,dv,dk), bf16
-    or fp32 as `initial_state` is (bf16 without one), and is computed with in fp32.  Returns (output, new_state), with a state per token when
+    (<= 0; -inf forgets all before the token), bf16 or fp32: (vh), one per head, or (B,T,vh) / (N,vh), one per token and head; None: no
+    decay.  The state is (sequences,vh,dv,dk), bf16 or fp32 as `initial_state` is (bf16 without one), and is computed with in fp32.  Returns (output, new_state), with a state per token when
     inference_mode == SpecVerify.  num_accepted_tokens, inplace_state and state_indices are those of recurrent_forward: outputs past a
     sequence's cap, of a padding sequence or behind the last packed one are not written.  A slot outside the pool is a padding sequence; the
     slots of a call must differ.  No gradients."""
@@ -762,9 +762,10 @@ def linear_attention_chunked(query, key, value, gate=None, scale: Optional[float
     """Linear attention with decay over whole prompts: what linear_attention_recurrent computes, 64 tokens at a time.
 
     The arguments are those of linear_attention_recurrent (packed inputs need cu_seqlens alone).  Returns (output, final_state), the
-    final state in initial_state's dtype (bf16 without one).  Matrix products take bf16 operands: scores with their decay and the
-    state a chunk reads are rounded to bf16 there, the state itself is kept in fp32 throughout.  A NaN or an infinity in `value` reaches
-    all tokens of its 64-token chunk.  No gradients."""
+    final state in initial_state's dtype (bf16 without one).  Matrix products take bf16 operands: values with their decay, scores and the
+    state that a chunk reads are rounded to bf16 there (and the queries that read it, in a chunk that forgets by more than 2^60), the state
+    itself is kept in fp32 throughout.  A NaN or an infinity in `value` reaches all tokens of its 64-token chunk.  Key dims above 128 go
+    token by token.  No gradients."""
     ext = _ext if _ext is not None else _load_ext()
     if ext:
         return ext._fast_linear_attention_chunked(query, key, value, gate, scale, initial_state, cu_seqlens)

@@ -85,6 +85,8 @@ int launch_short(const GroupNormParams& p, cudaStream_t st) {
     return GDN_OK;
 }
 
+constexpr long long kMostSamples = 65535;  // of a launch in parts
+
 template <typename T, int V>
 int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     if (plan.block_channels == 0) {
@@ -95,7 +97,18 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     p.part_rows = plan.part_rows;
     p.parts = plan.parts;
     p.block_channels = plan.block_channels;
-    GDN_REQUIRE(p.n <= 65535 && plan.blocks <= 65535, "gdn_group_norm: too many samples or channels for one launch");
+    GDN_REQUIRE(plan.blocks <= kMostSamples, "gdn_group_norm: too many channels");
+    if (p.n > kMostSamples) {  // a grid's limit: in turn, with the same workspace
+        for (long long first = 0; first < p.n; first += kMostSamples) {
+            GroupNormParams q = p;
+            q.n = std::min<long long>(p.n - first, kMostSamples);
+            q.x = static_cast<const T*>(p.x) + first * p.x_sn;
+            q.y = static_cast<T*>(p.y) + first * p.y_sn;
+            if (p.z) q.z = static_cast<const T*>(p.z) + first * p.z_sn;
+            if (int rc = launch_long<T, V>(q, plan, st)) return rc;
+        }
+        return GDN_OK;
+    }
     const dim3 grid(static_cast<unsigned>(plan.parts), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
     const int rstep = kNormThreads / (plan.block_channels / V), smem = (plan.part_rows + rstep - 1) / rstep * kNormThreads * V * static_cast<int>(sizeof(T));
     if (int rc = set_smem<gdn_group_norm_stats_kernel<T, V>>(kNormPartBytes)) return rc;

@@ -364,8 +364,8 @@ int gdn_gated_rmsnorm(const void* x, const void* z, void* y, const void* weight,
  * The output norm of linear attention is one sample per token (rows = 1, channels = heads * dv, groups = heads) with a gate.
  * x, z, y share `dtype` (GDN_BF16 or GDN_F32) and are addressed sample*stride_sample + row*stride_row + c (elements; any strides and
  * alignment: 16-byte aligned pointers, channels and strides that are multiples of 16 bytes are the fast case).  weight, bias: (channels) of `param_dtype`,
- * either may be NULL (1 and 0).  y may be x or z itself (same strides).  Samples of more than 1024 values per group need a workspace of gdn_group_norm_workspace_bytes() bytes,
- * 16-byte aligned. */
+ * either may be NULL (1 and 0).  y may be x or z itself (same strides).  A workspace of gdn_group_norm_workspace_bytes() bytes,
+ * 16-byte aligned, is needed where that is not 0 (more than 512 values of a sample per group). */
 typedef struct {
     const void* x;
     const void* z;

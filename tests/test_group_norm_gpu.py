@@ -133,3 +133,65 @@ def test_groups_in_shared_memory(shape, G, dtype):
     check(gdn.group_norm(x, G, w, b, z), x, G, w, b, z)
     check(gdn.group_norm(x, G, w, b), x, G, w, b)
     check(gdn.group_norm(x, G, None, None, None, 1e-5, False), x, G, None, None, None, 1e-5, False)
+
+
+@pytest.mark.parametrize("shape,G", [((70000, 200, 3), 1), ((70000, 40, 32), 2)], ids=str)
+def test_more_samples_than_a_grid_has_rows(shape, G):
+    x, z, w, b = make(shape, torch.bfloat16)
+    y, gated = gdn.group_norm(x, G, w, b), gdn.group_norm(x, G, w, b, z)
+    for at in (slice(0, 40), slice(65500, 65570), slice(69960, 70000)):
+        check(y[at], x[at], G, w, b)
+        check(gated[at], x[at], G, w, b, z[at])
+
+
+@pytest.mark.parametrize("shape,G", [((3, 4, 64), 2), ((2, 300, 64), 4), ((2, 9000, 40), 2), ((1, 30, 4100), 1)], ids=str)
+def test_in_place_through_the_library(shape, G):
+    """y may be x or z itself."""
+    import ctypes as C
+    from h100_gdn_cuda_b200 import _cabi as cabi
+    x, z, w, b = make(shape, torch.bfloat16)
+    N, L, ch = shape
+    lib = cabi.load()
+    ws = torch.empty(lib.gdn_group_norm_workspace_bytes(N, L, ch, G) + 16, dtype=torch.uint8, device="cuda")
+    for onto_z in (False, True):
+        want = gdn.group_norm(x, G, w, b, z if onto_z else None)
+        xc, zc = x.clone(), z.clone()
+        a = cabi.GroupNormArgs()
+        y = zc if onto_z else xc
+        a.x, a.z, a.y, a.weight, a.bias = xc.data_ptr(), zc.data_ptr() if onto_z else None, y.data_ptr(), w.data_ptr(), b.data_ptr()
+        a.samples, a.rows, a.channels, a.groups = N, L, ch, G
+        for n in ("x", "z", "y"):
+            setattr(a, n + "_stride_sample", L * ch)
+            setattr(a, n + "_stride_row", ch)
+        a.dtype, a.param_dtype, a.eps, a.silu = cabi.GDN_BF16, cabi.GDN_F32, 1e-5, 1
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        cabi.check(lib.gdn_group_norm(C.byref(a), torch.cuda.current_stream().cuda_stream), "group_norm")
+        assert torch.equal(y, want)
+
+
+def test_two_captured_graphs_and_another_stream():
+    """Graphs that were captured from the same call, replayed on two streams at once and on new inputs."""
+    shapes = [((2, 9000, 40), 2), ((4, 600, 64), 4)]
+    data = [make(shape, torch.bfloat16) + (G,) for shape, G in shapes]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for x, z, w, b, G in data:
+            gdn.group_norm(x, G, w, b, z)
+    side.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([gdn.group_norm(x, G, w, b, z) for x, z, w, b, G in data])
+        graphs.append(g)
+    for x, *_ in data:
+        x.mul_(-1.5).add_(0.25)
+    want = [gdn.group_norm(x, G, w, b, z) for x, z, w, b, G in data]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        graphs[0].replay()
+        with torch.cuda.stream(side):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))

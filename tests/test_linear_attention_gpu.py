@@ -4,7 +4,8 @@ Bounds.  A half step of a type t is u(t) = eps / 2 relative (bf16 2^-8, fp32 2^-
 absolute values, and R the same for the state:
   token by token: sums of fp32 products; a value passes at most T decays (each off by a few u(fp32), exp included) and a sum of dk terms:
       |o - ref| <= u(bf16) |ref| + F A ,   |S - ref| <= u(state) |ref| + F R ,   F = (dk + 16 T + 32) u(fp32)
-  in chunks the operands of the products are bf16: the scores (intra part) or the keys and the state they are read from (inter part):
+  in chunks the operands of the products are bf16: values with their decay and scores (intra part), the state and, where a chunk forgets
+  much, the queries with their decay (inter part); of the state's increment the values:
       |o - ref| <= u(bf16) |ref| + (2 u(bf16) + u(bf16)^2 + F) A ,   |S - ref| <= u(state) |ref| + (u(bf16) + F) R
 Every rounding there is independent of the others and v has random signs: the error's norm stays below 2 u(bf16) of the result's."""
 import math
@@ -340,3 +341,47 @@ def test_refusals():
                 lambda: Cc(*(torch.zeros(1, 2, 1, 264, dtype=torch.bfloat16, device="cuda"),) * 3)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+# cut into segments or not: one long chain, chains of a last round that is not full (160 on 148 SMs), chains of very different decay side by side,
+# each tile shape
+CUT = [((1, 4000, 1, 2, 128, 128), torch.bfloat16), ((5, 3330, 4, 32, 64, 64), torch.float32), ((1, 2500, 2, 4, 64, 128), None), ((2, 2049, 1, 3, 128, 40), torch.float32),
+       ((1, 3000, 1, 1, 72, 256), torch.bfloat16)]
+
+
+@pytest.mark.parametrize("shape,state", CUT, ids=str)
+def test_cut_chains(shape, state):
+    p = make(*shape, gate="token", state=state)
+    p["g"] *= torch.exp2(4 - 12 * torch.rand(shape[3], generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))  # forgets in a token, or in hundreds
+    check(*gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"]), p, True)
+
+
+@pytest.mark.parametrize("lens", [[3000, 1, 0, 2000], [0, 1200, 64, 1], [300] * 33 + [0, 1], [1] * 100], ids=lambda x: "%d of %d" % (len(x), sum(x)))
+def test_packed_cut_chains(lens):
+    total = sum(lens)
+    p = make(len(lens), total, 1, 2, 64, 64, gate="token", state=torch.bfloat16, packed=True)
+    p["g"] *= 0.02
+    cu = torch.tensor([0] + torch.tensor(lens).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+    o, s = gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"], cu)
+    for i, n in enumerate(lens):
+        a = int(cu[i])
+        if n == 0:
+            assert torch.equal(s[i], p["s"][i])
+        elif i in (0, 1, 2, 3, 34, len(lens) - 1):
+            check(o[None, a:a + n], s[i:i + 1], dict({x: p[x][None, a:a + n] for x in "qkvg"}, s=p["s"][i:i + 1]), True)
+
+
+def test_two_calls_at_once():
+    """Two cut prompts on two streams at the same time, at the bits of one after the other."""
+    ps = [make(1, 3000, 2, 4, 128, 128, gate="token", seed=i) for i in range(2)]
+    want = [gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"]) for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        got = []
+        for p, st in zip(ps, streams):
+            with torch.cuda.stream(st):
+                got.append(gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"]))
+        torch.cuda.synchronize()
+        for (o, s), (o2, s2) in zip(got, want):
+            assert torch.equal(o, o2) and torch.equal(s, s2)
