@@ -24,10 +24,14 @@
 //   warp 23     finds the items; the gates' running sums and the factors made of them
 // All products that feed output and state are transposed (128 dv rows = M): S and V' are A operands in tensor memory; Q, K and the scores
 // are B operands.
-// What bounds a chunk is shared memory (176 KB of copies, operands and tiles at 128 bytes a cycle: 1400 cycles) and what a warp of each role
-// needs for its part, a few hundred instructions one behind the other, not the tensor pipe (900 cycles of products); HBM allows 2750 at d = 128.  The instruction cache
-// counts: the waits are the short form and the item search is one warp's (104 KB of code took 5200 cycles a chunk with both SMs of a pair at work, 2900 with one).
-// The form with decays in keys and scores throughout (240 KB a chunk, two accumulators) took 118 us where this takes XX (4 x 4096 tokens, 32 v-heads).
+// What bounds it: HBM allows 2750 cycles a chunk at d = 128 on all SMs (2080 where two v-heads share Q and K), shared memory 1400 (176 KB of
+// copies, operands and tiles), the tensor pipe 900; a warp of each role needs 1000 to 1700 for its part, a few hundred instructions one behind the
+// other.  4 x 4096 tokens from DRAM: 88 us on 32 v-heads with 16 k-heads, 98 with 32, 148 heads of 4096 110; the same copies in and out and nothing
+// else take 69, 89 and 100.  From a chunk's copies to its end are 5300 cycles, so that three stages last 1780; with four of K, five of Q (the output
+// staged there) and V's given back early the copies took as much longer, and the whole as long.
+// The instruction cache counts: the waits are the short form and the item search is one warp's (104 KB of code took 5200 cycles a chunk with
+// both SMs of a pair at work, 2900 with one).  The form with decays in keys and scores throughout (240 KB of shared memory a chunk, two
+// accumulators) took 118 us where this takes 92 (4 x 4096 tokens, 32 v-heads, back to back).
 #pragma once
 #include <cuda.h>
 
