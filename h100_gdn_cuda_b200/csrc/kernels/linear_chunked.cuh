@@ -186,8 +186,8 @@ constexpr uint32_t kTmS = 0;     // its bf16 copy, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
 constexpr uint32_t kTmF = 128;   // fp32 state, 128 columns
 constexpr uint32_t kTmO = 256;   // 2 x fp32 V'^T P^T + S Q^T, 64 columns
-constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: V^T), 32 columns
-constexpr uint32_t kTmVd = 448;  // 2 x bf16 (e^{G_L - G_j} V)^T of chunks that are not plain, 32 columns
+constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: (e^{G_L - G_j} V)^T), 32 columns
+constexpr uint32_t kTmVlo = 448; // 2 x bf16: what is left of it
 constexpr float kPlainLog2 = 60.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 using namespace pairs;
@@ -213,6 +213,13 @@ __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
     v.w = pack2(mul2(pk(bf16_lo(v.w), bf16_hi(v.w)), w));
     return v;
 }
+// a pair of bf16 values times fp32 factors, as bf16 and what that leaves, to 2^-16 of it
+__device__ __forceinline__ void split_bf16(uint32_t& v, uint32_t& rest, f2 factors) {
+    using namespace ptx;
+    const f2 x = mul2(pk(bf16_lo(v), bf16_hi(v)), factors);
+    v = pack2(x);
+    rest = pack2(fma2(pk(bf16_lo(v), bf16_hi(v)), pk(-1.f, -1.f), x));
+}
 }  // namespace lin
 
 // kWhole: head dims are multiples of 64, so that one copy fetches all columns of a tile (maps of rank 5: 64 columns, tokens, column blocks, heads,
@@ -233,7 +240,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     uint64_t* bar_full = bars;                  // [stages] Q, K, V of a stage have arrived
     uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done
     uint64_t* bar_gate = bar_empty + kStages;   // [4] gate factors of a chunk
-    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps and the products' issuer
+    uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps
     uint64_t* bar_score = bar_gfree + 4;        // [2] Q K^T done
     uint64_t* bar_p = bar_score + 2;            // [2] scores and values written, and the output's accumulator read two chunks before
     uint64_t* bar_dgo = bar_p + 2;              // [2] values written and the state copied
@@ -257,7 +264,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar_gate[i], 1);
-            mbar_init(&bar_gfree[i], 13);
+            mbar_init(&bar_gfree[i], 12);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_score[i], 1);
@@ -501,21 +508,21 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     uint32_t r[16], w[8];
                     tmem_ld_frag32(tP + 32 * h, r);
                     tmem_wait_ld();
-                    if (__builtin_expect(!plain, 0)) {
+                    if (__builtin_expect(plain, 1)) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {  // (rounded to bf16 as an operand)
+                            const f2 f = *reinterpret_cast<const f2*>(gb + 32 * h + 8 * j + 2 * (lane & 3));
+                            w[j] = pack2(mul2(pk(r[4 * j], r[4 * j + 1]), f));
+                            w[4 + j] = pack2(mul2(pk(r[4 * j + 2], r[4 * j + 3]), f));
+                        }
+                    } else {
                         const float g0 = gb[128 + i0], g1 = gb[128 + i0 + 8];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             const float2 gj = *reinterpret_cast<const float2*>(gb + 128 + 32 * h + 8 * j + 2 * (lane & 3));
-                            r[4 * j] = __float_as_uint(__uint_as_float(r[4 * j]) * ex2(g0 - gj.x));
-                            r[4 * j + 1] = __float_as_uint(__uint_as_float(r[4 * j + 1]) * ex2(g0 - gj.y));
-                            r[4 * j + 2] = __float_as_uint(__uint_as_float(r[4 * j + 2]) * ex2(g1 - gj.x));
-                            r[4 * j + 3] = __float_as_uint(__uint_as_float(r[4 * j + 3]) * ex2(g1 - gj.y));
+                            w[j] = pack2(pk(__uint_as_float(r[4 * j]) * ex2(g0 - gj.x), __uint_as_float(r[4 * j + 1]) * ex2(g0 - gj.y)));
+                            w[4 + j] = pack2(pk(__uint_as_float(r[4 * j + 2]) * ex2(g1 - gj.x), __uint_as_float(r[4 * j + 3]) * ex2(g1 - gj.y)));
                         }
-                    }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {  // (rounded to bf16 as an operand)
-                        w[j] = pack2(pk(r[4 * j], r[4 * j + 1]));
-                        w[4 + j] = pack2(pk(r[4 * j + 2], r[4 * j + 3]));
                     }
                     if (h == lq >> 1) {  // the diagonal blocks and what is above them
                         if (lq & 1) {
@@ -564,10 +571,9 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 uint8_t* stage = smem + s * L::kStage;
                 const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                if (gc > 1) mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the values of two chunks before have been read
+                if (gc > 1) mbar_wait_short(&bar_d[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the values of two chunks before have been read
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 tc_fence_after_sync();
-                const bool plain = gb[259] != 0.f;
                 const uint32_t sV = smem_u32(stage + L::kOffV);
                 if (DV == 128 || lq < 2) {
 #pragma unroll 1
@@ -591,28 +597,35 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             }
                         }
                         const uint32_t to = tmem + tm_lane + 32 * (gc & 1) + 16 * hf;
-                        if (__builtin_expect(!plain, 0)) {
-                            tmem_st_frag16(to + kTmV, v[0][0]);
-                            tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
-                        }
+                        uint32_t u[2][2][4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const f2 f = *reinterpret_cast<const f2*>(gb + t0 + 8 * i);
 #pragma unroll
                             for (int a = 0; a < 2; ++a) {
-                                uint32_t &x = v[0][i >> 1][2 * (i & 1) + a], &y = v[1][i >> 1][2 * (i & 1) + a];
-                                x = pack2(mul2(pk(bf16_lo(x), bf16_hi(x)), f));  // (rounded to bf16 as an operand)
-                                y = pack2(mul2(pk(bf16_lo(y), bf16_hi(y)), f));
+                                split_bf16(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                                split_bf16(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
                             }
                         }
-                        tmem_st_frag16(to + (plain ? kTmV : kTmVd), v[0][0]);
-                        tmem_st_frag16(to + (plain ? kTmV : kTmVd) + (16u << 16), v[1][0]);
+                        tmem_st_frag16(to + kTmV, v[0][0]);
+                        tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
+                        if (p.state_f32) {
+                            tmem_st_frag16(to + kTmVlo, u[0][0]);
+                            tmem_st_frag16(to + kTmVlo + (16u << 16), u[1][0]);
+                        }
                     }
                 }
-                if (__builtin_expect(packed && n < kChunk, 0)) {  // keys of the next sequence meet zero values, but zero times their NaN is one
+                if (__builtin_expect(packed && n < kChunk, 0)) {  // zero scores and values meet what the next sequence has there, but zero times its NaN is one
 #pragma unroll 1
                     for (int at = n * (DK / 8) + vtid; at < kChunk * (DK / 8); at += 128)
                         *reinterpret_cast<uint4*>(stage + L::kOffK + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
+                    if (DV == 128 || lq < 2) {  // the columns of V that this warp has read itself
+#pragma unroll 1
+                        for (int at = n * 4 + lane; at < kChunk * 4; at += 32)
+                            *reinterpret_cast<uint4*>(stage + L::kOffV + (lq >> 1) * 8192 + (at >> 2) * 128 + (((4 * (lq & 1) + (at & 3)) ^ ((at >> 2) & 7)) << 4)) =
+                                make_uint4(0u, 0u, 0u, 0u);
+                    }
                     fence_proxy_async_smem();
                 }
                 tmem_wait_st();
@@ -664,25 +677,24 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         }
     } else if (warp == 21) {
         // =============================================================== products of state and output
-        constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true), id_o = make_idesc_bf16(128, 64, false, false);
-        const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024);  // read MN-major
+        constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true), id_o = make_idesc_bf16(128, 64, false, false), id_v = make_idesc_bf16(128, 64, true, false);
+        // read MN-major (DV == 64: rows 64 on are what follows V's tile, and reach rows of O that nobody looks at)
+        const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024), dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), 8192, 1024);
         const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages, b = gc & 1;
-                mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
-                const uint32_t tV = tmem + (__shfl_sync(0xffffffffu, gate_buf(gc)[259], 0) != 0.f ? kTmV : kTmVd) + 32 * b;
-                if (lane == 0) mbar_arrive(&bar_gfree[gc & 3]);
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
                 mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-                mma_ts_k64_w<true, 128>(tmem + kTmF, tV, desc_advance(dK, s * L::kStage), id_d);
+                mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmV + 32 * b, desc_advance(dK, s * L::kStage), id_d);
+                if (p.state_f32) mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmVlo + 32 * b, desc_advance(dK, s * L::kStage), id_d);
                 mma_commit_w(&bar_d[b]);
                 if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
                 else mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
-                mma_ts_k64_w<true, 2>(tmem + kTmO + 64 * b, tmem + kTmV + 32 * b, desc_advance(dP, b * 8192), id_o);
+                mma_ss_k64_w<true, 128, 2>(tmem + kTmO + 64 * b, desc_advance(dV, s * L::kStage), desc_advance(dP, b * 8192), id_v);
                 mma_commit_w(&bar_o[b]);
                 mma_commit_w(&bar_empty[s]);
             }

@@ -21,7 +21,7 @@ struct LinSegSmem {
 namespace lin {
 constexpr int kSegThreads = 224;   // 4 value warps, producer, issuer, gates
 constexpr uint32_t kTmSegF = 0;    // fp32 increment, 128 columns
-constexpr uint32_t kTmSegV = 128;  // 2 x bf16 V'^T, 32 columns
+constexpr uint32_t kTmSegV = 128;  // 2 x bf16 V'^T, 32 columns; 2 x what is left of it
 }  // namespace lin
 
 template <int DK, int DV, bool kWhole>
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             if (DV == 128 || lq < 2) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {  // 32 tokens
-                    uint32_t v[2][2][4];
+                    uint32_t v[2][2][4], u[2][2][4];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         ldmatrix_x4_trans(sV + vsw0 + 4096 * hf + 2048 * j, v[0][j]);
@@ -105,14 +105,17 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
                         const f2 f = *reinterpret_cast<const f2*>(gb + 32 * hf + 2 * (lane & 3) + 8 * i);
 #pragma unroll
                         for (int a = 0; a < 2; ++a) {
-                            uint32_t &x = v[0][i >> 1][2 * (i & 1) + a], &y = v[1][i >> 1][2 * (i & 1) + a];
-                            x = pack2(mul2(pk(bf16_lo(x), bf16_hi(x)), f));  // (rounded to bf16 as an operand)
-                            y = pack2(mul2(pk(bf16_lo(y), bf16_hi(y)), f));
+                            split_bf16(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                            split_bf16(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
                         }
                     }
                     const uint32_t to = tmem + kTmSegV + tm_lane + 32 * (n & 1) + 16 * hf;
                     tmem_st_frag16(to, v[0][0]);
                     tmem_st_frag16(to + (16u << 16), v[1][0]);
+                    if (p.state_f32) {
+                        tmem_st_frag16(to + 64, u[0][0]);
+                        tmem_st_frag16(to + 64 + (16u << 16), u[1][0]);
+                    }
                 }
             }
             tmem_wait_st();
@@ -179,6 +182,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             const uint32_t tV = tmem + kTmSegV + 32 * b;
             if (n == 0) mma_ts_k64_w<false, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
             else mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
+            if (p.state_f32) mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV + 64, desc_advance(dK, s * L::kStage), id_d);
             mma_commit_w(&bar_done[b]);
             mma_commit_w(&bar_empty[s]);
         }

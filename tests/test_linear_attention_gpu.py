@@ -385,3 +385,16 @@ def test_two_calls_at_once():
         torch.cuda.synchronize()
         for (o, s), (o2, s2) in zip(got, want):
             assert torch.equal(o, o2) and torch.equal(s, s2)
+
+
+@pytest.mark.parametrize("gate", ["head", "token", "none"])
+@pytest.mark.parametrize("shape", [(2, 64, 1, 2, 128, 128), (2, 257, 2, 4, 64, 64), (1, 2000, 2, 4, 128, 128), (1, 900, 2, 2, 96, 200), (160, 200, 1, 1, 128, 64)], ids=str)
+def test_fp32_states_of_prompts(shape, gate):
+    """An fp32 state is more exact than bf16 values are: these go into it in two parts, 2^-16 off at most.  A decay is 2 to the difference of two sums
+    of log2-decays below 64 each, of six roundings of half a step, 2^-19, with ln 2 in front: 2^-16 as well.  Products and sums are fp32; the
+    errors of a sum's terms are independent, so the sum of both bounds, 2^-15, holds for the norm."""
+    p = make(*shape, gate=gate)
+    o, s = gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"])
+    ref, sref = O.linear_attention_ref(p["q"], p["k"], p["v"], p["g"], shape[4] ** -0.5, p["s"], False)
+    assert s.dtype == torch.float32 and (s.double() - sref).norm() <= 2.0 ** -15 * sref.norm()
+    check(o, s, p, True)
