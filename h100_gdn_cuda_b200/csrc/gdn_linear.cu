@@ -97,7 +97,7 @@ LinearPlan linear_plan(const GdnShape& s) {
     return plan;
 }
 
-template <int DK, int DV, bool kWhole>
+template <int DK, int DV, bool kWhole, bool kF32>
 int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, long long cut_chains, cudaStream_t st) {
     using L = LinSmem<DK, DV>;
     using LS = LinSegSmem<DK, DV>;
@@ -107,7 +107,7 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     if (int rc = linear_map(&tmK, a.k, s, s.num_k_heads, s.head_dim_k, "k", kWhole ? DK : 0)) return rc;
     if (int rc = linear_map(&tmV, a.v, s, s.num_v_heads, s.head_dim_v, "v", kWhole ? DV : 0)) return rc;
     if (int rc = linear_map(&tmO, a.out, s, s.num_v_heads, s.head_dim_v, "out")) return rc;
-    if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV, kWhole>>(L::kBytes)) return rc;
+    if (int rc = set_smem<gdn_linear_chunked_kernel<DK, DV, kWhole, kF32>>(L::kBytes)) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -116,11 +116,11 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (p.seg_state) {
-        if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole>>(LS::kBytes)) return rc;
+        if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole, kF32>>(LS::kBytes)) return rc;
         cfg.gridDim = dim3(static_cast<unsigned>(p.num_items - p.whole));
         cfg.blockDim = dim3(lin::kSegThreads);
         cfg.dynamicSmemBytes = LS::kBytes;
-        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole>, tmK, tmV, p));
+        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole, kF32>, tmK, tmV, p));
         cfg.gridDim = dim3(static_cast<unsigned>(cut_chains), 128 * DK / 4 / kLinCombineThreads);
         cfg.blockDim = dim3(kLinCombineThreads);
         cfg.dynamicSmemBytes = 0;
@@ -129,8 +129,18 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     cfg.gridDim = dim3(static_cast<unsigned>(p.num_items));
     cfg.blockDim = dim3(lin::kThreads);
     cfg.dynamicSmemBytes = L::kBytes;
-    GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV, kWhole>, tmQ, tmK, tmV, tmO, p));
+    GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_chunked_kernel<DK, DV, kWhole, kF32>, tmQ, tmK, tmV, tmO, p));
     return GDN_OK;
+}
+
+template <bool kF32>
+int launch_linear_shape(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, long long cut_chains, cudaStream_t st) {
+    // (a single column block needs no rank 5: its map clips what is missing)
+    const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);
+    if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false, kF32>(a, p, cut_chains, st);
+    if (p.dk <= 64) return launch_linear_chunked<64, 128, false, kF32>(a, p, cut_chains, st);
+    if (p.dv <= 64) return launch_linear_chunked<128, 64, false, kF32>(a, p, cut_chains, st);
+    return whole ? launch_linear_chunked<128, 128, true, kF32>(a, p, cut_chains, st) : launch_linear_chunked<128, 128, false, kF32>(a, p, cut_chains, st);
 }
 
 }  // namespace
@@ -233,12 +243,7 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
         p.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + plan.states);
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // (a single column block needs no rank 5: its map clips what is missing)
-    const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);
-    if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false>(*a, p, plan.cut_chains, st);
-    if (p.dk <= 64) return launch_linear_chunked<64, 128, false>(*a, p, plan.cut_chains, st);
-    if (p.dv <= 64) return launch_linear_chunked<128, 64, false>(*a, p, plan.cut_chains, st);
-    return whole ? launch_linear_chunked<128, 128, true>(*a, p, plan.cut_chains, st) : launch_linear_chunked<128, 128, false>(*a, p, plan.cut_chains, st);
+    return a->state_dtype == GDN_F32 ? launch_linear_shape<true>(*a, p, plan.cut_chains, st) : launch_linear_shape<false>(*a, p, plan.cut_chains, st);
 }
 
 }  // extern "C"

@@ -3,35 +3,39 @@
 //     O = scale * ( e^{G_i} Q S^T  +  (Q K^T .* e^{G_i - G_j}, j <= i) V )
 //     S <- e^{G_L} S + (e^{G_L - G_j} V)^T K .
 // The state's increment does not depend on the state, so all products of a chunk can be issued ahead of it.  Where no decay of the chunk is
-// below 2^-120 it is a factor of the values alone,
-//     V' = e^{-G_j} V ,   O = scale e^{G_i} * ( Q S^T + (Q K^T, j <= i) V' ) ,   S <- e^{G_L} (S + V'^T K) ,
-// so that the scores only have to be cut off above the diagonal and both parts of O are one accumulation ("plain" chunks).  The factor
-// e^{G_L} is not applied either but kept as an exponent c of the whole state, which joins the factors of the chunks that follow,
-//     S = 2^c S' ,   V' = e^{-G_j} 2^{-c} V ,   O = scale e^{G_i} 2^c * ( ... ) ,
+// below 2^-120 it is a factor w_j = e^{-G_j} of the values alone,
+//     O = scale e^{G_i} * ( Q S^T + (Q K^T w_j, j <= i) V ) ,   S <- e^{G_L} (S + (w_j V)^T K) ,
+// so that the scores take one factor a column, have to be cut off above the diagonal, and both parts of O are one accumulation ("plain"
+// chunks).  The factor e^{G_L} is not applied either but kept as an exponent c of the whole state, which joins the factors of the chunks that follow,
+//     S = 2^c S' ,   w_j = e^{-G_j} 2^{-c} ,   O = scale e^{G_i} 2^c * ( ... ) ,
 // until it leaves 2^-60 .. 2^60: S' is an accumulator in tensor memory that the increments are added to by the products themselves.  (That leaves
-// 2^60 and more for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: it goes into the
-// scores, the rows of Q are scaled where they lie, the values come twice and the state is scaled between its read and its increment.
+// 2^60 and more for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: the scores take
+// e^{G_i - G_j}, the rows of Q are scaled where they lie, the values of the increment take e^{G_L - G_j} and the state is scaled between its read
+// and its increment.
+// Roundings: scores, the copy of the state that Q meets, and Q where it is scaled are bf16, once each.  Values of the increment are bf16 where the
+// state is; an fp32 state gets them in two parts, bf16 and what that leaves, by a second product (final states 2.3e-3 off without it, 5e-6 with;
+// 4 x 4096 tokens from DRAM 88 -> 91 us).
 //
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
 // items and chunks, handing tiles on through mbarriers:
 //   warps 0-7   state warps: a bf16 copy of the fp32 state for the products with Q (lane = dv row, half of the columns each); its scaling
-//   warps 8-11  output warps: O scaled, transposed through shared memory, stored
+//   warps 8-11  output warps: O scaled, transposed into Q's tile, stored
 //   warps 12-15 score warps: the scores as bf16 tile
-//   warps 16-19 value warps: V^T times its factors into tensor memory
+//   warps 16-19 value warps: V^T times its factors into tensor memory, for the increment
 //   warp 20     producer: tensor copies of Q, K, V into a ring of stages
-//   warp 21     issues the state's increment V'^T K, which the next chunk waits for, then the products of the output, V'^T P^T and S Q^T
+//   warp 21     issues the state's increment (w V)^T K, which the next chunk waits for, then the products of the output, S Q^T and V^T P^T
 //   warp 22     issues the scores Q K^T
 //   warp 23     finds the items; the gates' running sums and the factors made of them
-// All products that feed output and state are transposed (128 dv rows = M): S and V' are A operands in tensor memory; Q, K and the scores
-// are B operands.
-// What bounds it: HBM allows 2750 cycles a chunk at d = 128 on all SMs (2080 where two v-heads share Q and K), shared memory 1400 (176 KB of
-// copies, operands and tiles), the tensor pipe 900; a warp of each role needs 1000 to 1700 for its part, a few hundred instructions one behind the
-// other.  4 x 4096 tokens from DRAM: 88 us on 32 v-heads with 16 k-heads, 98 with 32, 148 heads of 4096 110; the same copies in and out and nothing
-// else take 69, 89 and 100.  From a chunk's copies to its end are 5300 cycles, so that three stages last 1780; with four of K, five of Q (the output
-// staged there) and V's given back early the copies took as much longer, and the whole as long.
-// The instruction cache counts: the waits are the short form and the item search is one warp's (104 KB of code took 5200 cycles a chunk with
-// both SMs of a pair at work, 2900 with one).  The form with decays in keys and scores throughout (240 KB of shared memory a chunk, two
-// accumulators) took 118 us where this takes 92 (4 x 4096 tokens, 32 v-heads, back to back).
+// All products that feed output and state are transposed (128 dv rows = M): S and w V are A operands in tensor memory, V one in shared memory as it
+// came; Q, K and the scores are B operands.
+// What bounds it: HBM allows 2750 cycles a chunk at d = 128 on all SMs (2080 where two v-heads share Q and K), shared memory 1600 (208 KB of
+// copies, operands and tiles), the tensor pipe 1150; a warp of each role needs 1000 to 1700 for its part, a few hundred instructions one behind the
+// other (4300 a chunk in all).  4 x 4096 tokens from DRAM: 91 us on 32 v-heads with 16 k-heads, 99 with 32, 148 heads of 4096 110; the same copies in
+// and out and nothing else take 69, 89 and 100.  From a chunk's copies to its end are 5300 cycles and more with all SMs at work, half of them the copies:
+// the ring has four stages, and a fifth tile for Q and the output (three stages: 95 us).
+// The instruction cache counts: the waits are the short form, the item search is one warp's, the state's type is the kernel's (104 KB of code took 5200
+// cycles a chunk with both SMs of a pair at work, 2900 with one).  The form with decays in keys and scores throughout (240 KB of shared memory
+// a chunk, two accumulators) took 118 us where this takes 100 (4 x 4096 tokens, 32 v-heads, back to back).
 #pragma once
 #include <cuda.h>
 
@@ -167,17 +171,17 @@ struct LinWalker {
 
 template <int DK, int DV>
 struct LinSmem {
-    static constexpr int kStages = 3;
-    static constexpr int kTileK = kChunk * DK * 2, kTileV = kChunk * DV * 2;
-    static constexpr int kOffQ = 0, kOffK = kTileK, kOffV = 2 * kTileK, kStage = 2 * kTileK + kTileV;
-    static constexpr int kOffP = kStages * kStage;  // 2 x scores, 64 x 64
-    static constexpr int kOffO = kOffP + 2 * 8192;  // 2 x output staging
-    // 4 x gate factors, fp32: of the values [64]; of the output [64]; not plain: G[64] (log2), e^{G_i}[64]; of the state in front of its copy
-    // and behind it; 2^c behind the chunk; plain or not
-    static constexpr int kOffGate = kOffO + 2 * kTileV;
-    static constexpr int kGateStride = (4 * 64 + 4) * 4;
+    static constexpr int kStages = DK == 64 && DV == 64 ? 6 : 4, kStagesQ = kStages + 1;  // (the output is staged in Q's tile, which so lasts longer)
+    static constexpr int kTileK = kChunk * DK * 2, kTileV = kChunk * DV * 2, kTileQ = kTileK > kTileV ? kTileK : kTileV;
+    static constexpr int kOffV = kStages * kTileK;
+    static constexpr int kOffQ = kOffV + kStages * kTileV;
+    static constexpr int kOffP = kOffQ + kStagesQ * kTileQ;  // scores, 64 x 64
+    // 4 x gate factors, fp32: of the scores [64]; of the output [64]; not plain: G[64] (log2), e^{G_i}[64]; of the state in front of its copy
+    // and behind it; 2^c behind the chunk; plain or not; of the values [64] (see put_factor)
+    static constexpr int kOffGate = kOffP + 8192;
+    static constexpr int kGateStride = (5 * 64 + 4) * 4;
     static constexpr int kOffBar = kOffGate + 4 * kGateStride;
-    static constexpr int kBytes = kOffBar + 512 + 1024;
+    static constexpr int kBytes = kOffBar + 640 + 1024;
 };
 
 namespace lin {
@@ -185,8 +189,8 @@ constexpr int kThreads = 768;  // 24 warps
 constexpr uint32_t kTmS = 0;     // its bf16 copy, 64 columns
 constexpr uint32_t kTmP = 64;    // fp32 Q K^T of even (lanes +0) and odd chunks (lanes +16), 64 columns
 constexpr uint32_t kTmF = 128;   // fp32 state, 128 columns
-constexpr uint32_t kTmO = 256;   // 2 x fp32 V'^T P^T + S Q^T, 64 columns
-constexpr uint32_t kTmV = 384;   // 2 x bf16 V'^T (not plain: (e^{G_L - G_j} V)^T), 32 columns
+constexpr uint32_t kTmO = 256;   // 2 x fp32 S Q^T + V^T P^T, 64 columns
+constexpr uint32_t kTmV = 384;   // 2 x bf16 (w V)^T (not plain: (e^{G_L - G_j} V)^T), 32 columns
 constexpr uint32_t kTmVlo = 448; // 2 x bf16: what is left of it
 constexpr float kPlainLog2 = 60.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -213,47 +217,66 @@ __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
     v.w = pack2(mul2(pk(bf16_lo(v.w), bf16_hi(v.w)), w));
     return v;
 }
-// a pair of bf16 values times fp32 factors, as bf16 and what that leaves, to 2^-16 of it
-__device__ __forceinline__ void split_bf16(uint32_t& v, uint32_t& rest, f2 factors) {
-    using namespace ptx;
-    const f2 x = mul2(pk(bf16_lo(v), bf16_hi(v)), factors);
-    v = pack2(x);
-    rest = pack2(fma2(pk(bf16_lo(v), bf16_hi(v)), pk(-1.f, -1.f), x));
+// Factors of values as two bf16 numbers each, which is 2^-16 of them: those of tokens 2t and 2t + 1 are pairs behind one another.
+__device__ __forceinline__ void put_factor(float* factors, int token, float f) {
+    __nv_bfloat16* const to = reinterpret_cast<__nv_bfloat16*>(factors) + 4 * (token >> 1) + (token & 1);
+    const __nv_bfloat16 head = __float2bfloat16(f);
+    to[0] = head;
+    to[2] = __float2bfloat16(f - __bfloat162float(head));
+}
+// A pair of values times its factors: v, rounded to bf16 as an operand, and with kTwo what that leaves, to 2^-16 of it (v times a factor's head is exact in
+// the difference).
+template <bool kTwo>
+__device__ __forceinline__ void times_factors(uint32_t& v, uint32_t& rest, uint2 f) {
+    const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v), head = *reinterpret_cast<const __nv_bfloat162*>(&f.x), tail = *reinterpret_cast<const __nv_bfloat162*>(&f.y);
+    __nv_bfloat162 y;
+    if (kTwo) {
+        y = __hmul2_rn(x, head);
+        const __nv_bfloat162 r = __hfma2(x, tail, __hfma2(x, head, __hneg2(y)));
+        rest = *reinterpret_cast<const uint32_t*>(&r);
+    } else {
+        y = __hfma2(x, head, __hmul2_rn(x, tail));
+    }
+    v = *reinterpret_cast<const uint32_t*>(&y);
 }
 }  // namespace lin
 
 // kWhole: head dims are multiples of 64, so that one copy fetches all columns of a tile (maps of rank 5: 64 columns, tokens, column blocks, heads,
 // batch); otherwise every 64 columns are a copy of their own, which leaves out the columns that the next head begins with.
-template <int DK, int DV, bool kWhole>
+template <int DK, int DV, bool kWhole, bool kF32>
 __global__ void __launch_bounds__(lin::kThreads, 1)
     gdn_linear_chunked_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                               const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO, const LinChunkedParams p) {
     using namespace ptx;
     using namespace lin;
     using L = LinSmem<DK, DV>;
-    constexpr int kStages = L::kStages;
+    constexpr int kStages = L::kStages, kStagesQ = L::kStagesQ;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
     // No barrier may run two phases ahead of somebody who waits on it: each one's next phase but one needs what its waiters do after
     // theirs.  Barriers of two are those of even and of odd chunks.
-    uint64_t* bar_full = bars;                  // [stages] Q, K, V of a stage have arrived
-    uint64_t* bar_empty = bar_full + kStages;   // [stages] the products of the stage's chunk are done
-    uint64_t* bar_gate = bar_empty + kStages;   // [4] gate factors of a chunk
+    uint64_t* bar_full = bars;                    // [stages] Q, K, V of a chunk have arrived
+    uint64_t* bar_empty = bar_full + kStages;     // [stages] the products of the stage's chunk are done
+    uint64_t* bar_qempty = bar_empty + kStages;   // [Q's stages] the output that was staged there has been read
+    uint64_t* bar_gate = bar_qempty + kStagesQ;  // [4] gate factors of a chunk
     uint64_t* bar_gfree = bar_gate + 4;         // [4] read by state and output warps
     uint64_t* bar_score = bar_gfree + 4;        // [2] Q K^T done
-    uint64_t* bar_p = bar_score + 2;            // [2] scores and values written, and the output's accumulator read two chunks before
+    uint64_t* bar_p = bar_score + 2;            // [2] scores written (and Q scaled)
     uint64_t* bar_dgo = bar_p + 2;              // [2] values written and the state copied
-    uint64_t* bar_o = bar_dgo + 2;              // [2] O done: scores, state and values read
+    uint64_t* bar_ofree = bar_dgo + 2;          // [2] O read
+    uint64_t* bar_s = bar_ofree + 2;            // [2] the copy of the state read
+    uint64_t* bar_o = bar_s + 2;                // [2] O done
     uint64_t* bar_d = bar_o + 2;                // [2] increment added
     uint64_t* bar_item = bar_d + 2;             // [2] an item is there
     uint64_t* bar_itemfree = bar_item + 2;      // [2] and every warp has it
     uint64_t* bar_next = bar_itemfree + 2;      // the answer to a request for another item is there
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar_next + 1);
     int* abort_flag = reinterpret_cast<int*>(tmem_slot + 1);
-    LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 512 - 2 * sizeof(LinItem));
-    uint8_t* next = smem + L::kOffBar + 512 - 2 * sizeof(LinItem) - 16;  // the answer
-    static_assert((2 * kStages + 23) * 8 + 8 + 16 + 2 * sizeof(LinItem) <= 512, "room for the barriers");
+    LinItem* items = reinterpret_cast<LinItem*>(smem + L::kOffBar + 640 - 2 * sizeof(LinItem));
+    uint8_t* next = smem + L::kOffBar + 640 - 2 * sizeof(LinItem) - 16;  // the answer
+    static_assert((2 * kStages + kStagesQ + 27) * 8 + 8 + 16 + 2 * sizeof(LinItem) <= 640, "room for the barriers");
+    static_assert(L::kBytes <= 232448, "room in shared memory");
 
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
@@ -262,13 +285,16 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             mbar_init(&bar_full[i], 1);
             mbar_init(&bar_empty[i], 1);
         }
+        for (int i = 0; i < kStagesQ; ++i) mbar_init(&bar_qempty[i], 1);
         for (int i = 0; i < 4; ++i) {
             mbar_init(&bar_gate[i], 1);
             mbar_init(&bar_gfree[i], 12);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar_score[i], 1);
-            mbar_init(&bar_p[i], 12);
+            mbar_init(&bar_p[i], 4);
+            mbar_init(&bar_ofree[i], 4);
+            mbar_init(&bar_s[i], 1);
             mbar_init(&bar_dgo[i], 12);
             mbar_init(&bar_o[i], 1);
             mbar_init(&bar_d[i], 1);
@@ -279,7 +305,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         mbar_fence_init();
     }
     // the scores' blocks above the diagonal stay zero: nobody writes them
-    for (int i = tid; i < 2 * 8192 / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + L::kOffP + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < 8192 / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + L::kOffP + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
     if (warp == 0) tmem_alloc(tmem_slot, 512);
     fence_proxy_async_smem();
     tc_fence_before_sync();
@@ -323,10 +349,10 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     const uint4* src = reinterpret_cast<const uint4*>(p.seg_state + static_cast<long long>(it.before) * (128 * DK) + (32 * lq + lane) * DK + c0 + q);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = __ldcg(src + e);
-                } else if (p.state_in && p.state_f32) {
+                } else if (kF32) {
                     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0 + q);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = 4 * e < cols ? src[e] : make_uint4(0u, 0u, 0u, 0u);
+                    for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = p.state_in && 4 * e < cols ? src[e] : make_uint4(0u, 0u, 0u, 0u);
                 } else {
                     const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.state_in) + it.seq * p.si_ss + it.head * p.si_sh + static_cast<long long>(row) * p.dk + c0 + q);
 #pragma unroll
@@ -374,7 +400,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         for (int e = 0; e < 16; ++e) w[q / 2 + e] = pack2(pk(r[2 * e], r[2 * e + 1]));
                     }
                 }
-                if (gc > 0) mbar_wait_short(&bar_o[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);  // the copy before has been read
+                if (gc > 0) mbar_wait_short(&bar_s[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);  // the copy before has been read
                 tc_fence_after_sync();
 #pragma unroll
                 for (int q = 0; q < kCols / 2; q += 16) tmem_st16(tS + q, w + q);
@@ -399,7 +425,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     const int cols = row_in ? p.dk - c0 - q : 0;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * pow_c);
-                    if (p.state_f32) {
+                    if (kF32) {
                         uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.state_out) + at + q);
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
@@ -424,13 +450,12 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         const uint32_t ochunk = static_cast<uint32_t>(4 * (lq & 1) + ((lane >> 3) & 1));
         const uint32_t osw0 = olane + ((ochunk ^ (lane & 7)) << 4), osw1 = olane + (((ochunk + 2) ^ (lane & 7)) << 4);
         const bool packed = p.cu_seqlens != nullptr;
-        if (lane < 2) mbar_arrive(&bar_p[lane]);  // (no accumulators before the first two)
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const int n = min(it.tokens - c * kChunk, kChunk);
                 const float* gb = gate_buf(gc) + 64;
-                uint8_t* const sO = smem + L::kOffO + (gc & 1) * L::kTileV;
+                uint8_t* const sO = smem + L::kOffQ + gc % kStagesQ * L::kTileQ;
                 const uint32_t sOa = smem_u32(sO), tO = tmem + kTmO + 64 * (gc & 1) + tm_lane;
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 mbar_wait_short(&bar_o[gc & 1], (gc >> 1) & 1, abort_flag);
@@ -455,12 +480,10 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 tc_fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&bar_p[gc & 1]);
+                    mbar_arrive(&bar_ofree[gc & 1]);
                     mbar_arrive(&bar_gfree[gc & 3]);
                 }
                 fence_proxy_async_smem();
-                // (a tile is written again two chunks on: the store between the two has been waited for here by then)
-                if (otid == 0) bulk_wait_read<0>();
                 named_bar_sync(1, 128);
                 const int tok0 = it.tok0 + c * kChunk;
                 const int left = p.dv - it.dvt * 128;  // columns from this tile on
@@ -471,7 +494,6 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
 #pragma unroll
                         for (int a = 0; a < DV / 64; ++a)  // columns past dv and tokens past the end are clipped
                             if (64 * a < left) tma_store_4d(&tmO, sO + 8192 * a, it.dvt * 128 + 64 * a, it.head, tok0, it.batch);
-                        bulk_commit();
                     }
                 } else {  // a whole box would reach into the next sequence
                     __nv_bfloat16* base = p.out.ptr + it.batch * p.out.sb + tok0 * p.out.st + static_cast<long long>(it.head) * p.out.sh + it.dvt * 128;
@@ -480,6 +502,13 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     for (int idx = otid; idx < n * 16; idx += 128) {
                         const int row = idx >> 4, c16 = idx & 15;
                         if (c16 < pieces) *reinterpret_cast<uint4*>(base + row * p.out.st + c16 * 8) = *reinterpret_cast<const uint4*>(sO + tile_off(row, c16));
+                    }
+                }
+                if (otid == 0) {
+                    bulk_commit();
+                    if (gc > 0) {
+                        bulk_wait_read<1>();  // the tile of the chunk before has been read
+                        mbar_arrive(&bar_qempty[(gc - 1) % kStagesQ]);
                     }
                 }
             }
@@ -498,11 +527,10 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 const bool plain = gb[259] != 0.f;
-                if (gc > 1) mbar_wait_short(&bar_o[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the tile of two chunks before has been read
                 mbar_wait_short(&bar_score[gc & 1], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t tP = tmem + kTmP + (static_cast<uint32_t>(32 * lq + ((gc & 1) ? 16 : 0)) << 16);
-                const uint32_t sP = smem_u32(smem + L::kOffP + (gc & 1) * 8192) + (16 * lq + (lane & 7)) * 128;
+                const uint32_t sP = smem_u32(smem + L::kOffP) + (16 * lq + (lane & 7)) * 128;
 #pragma unroll 1
                 for (int h = 0; h <= lq >> 1; ++h) {
                     uint32_t r[16], w[8];
@@ -535,14 +563,14 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             w[1] = w[2] = w[3] = w[6] = w[7] = 0u;
                         }
                     }
+                    if (h == 0 && gc > 0) mbar_wait_short(&bar_o[(gc - 1) & 1], ((gc - 1) >> 1) & 1, abort_flag);  // the chunk before is through with the tile
                     const uint32_t to = sP + (((4 * h + (lane >> 3)) ^ (lane & 7)) << 4);  // lane 8m + r: row r (of 8), columns 8 (4 h + m)
                     stmatrix_x4(to, w[0], w[1], w[2], w[3]);
                     stmatrix_x4(to + 1024, w[4], w[5], w[6], w[7]);
                 }
                 if (__builtin_expect(!plain, 0)) {  // Q, which Q K^T has been through with, takes its decay where it lies
-                    const uint32_t s = gc % kStages;
-                    mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
-                    uint8_t* q = smem + s * L::kStage + L::kOffQ;
+                    mbar_wait_short(&bar_full[gc % kStages], (gc / kStages) & 1, abort_flag);
+                    uint8_t* q = smem + L::kOffQ + gc % kStagesQ * L::kTileQ;
 #pragma unroll 1
                     for (int at = stid; at < L::kTileK / 16; at += 128)
                         *reinterpret_cast<uint4*>(q + at * 16) = scale8(*reinterpret_cast<const uint4*>(q + at * 16), gb[192 + ((at & 511) >> 3)]);
@@ -568,13 +596,13 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const int n = min(it.tokens - c * kChunk, kChunk);
                 const uint32_t s = gc % kStages;
-                uint8_t* stage = smem + s * L::kStage;
+                uint8_t *tk = smem + s * L::kTileK, *tv = smem + L::kOffV + s * L::kTileV;
                 const float* gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 if (gc > 1) mbar_wait_short(&bar_d[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the values of two chunks before have been read
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 tc_fence_after_sync();
-                const uint32_t sV = smem_u32(stage + L::kOffV);
+                const uint32_t sV = smem_u32(tv);
                 if (DV == 128 || lq < 2) {
 #pragma unroll 1
                     for (int hf = 0; hf < 2; ++hf) {  // 32 tokens
@@ -597,33 +625,45 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             }
                         }
                         const uint32_t to = tmem + tm_lane + 32 * (gc & 1) + 16 * hf;
-                        uint32_t u[2][2][4];
+                        const uint2* const fv = reinterpret_cast<const uint2*>(gb + 260) + t0 / 2;
+                        if (kF32) {
+                            uint32_t u[2][2][4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const f2 f = *reinterpret_cast<const f2*>(gb + t0 + 8 * i);
+                            for (int i = 0; i < 4; ++i) {
+                                const uint2 f = fv[4 * i];
 #pragma unroll
-                            for (int a = 0; a < 2; ++a) {
-                                split_bf16(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
-                                split_bf16(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
+                                for (int a = 0; a < 2; ++a) {
+                                    times_factors<true>(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                                    times_factors<true>(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
+                                }
+                            }
+                            tmem_st_frag16(to + kTmVlo, u[0][0]);
+                            tmem_st_frag16(to + kTmVlo + (16u << 16), u[1][0]);
+                        } else {
+                            uint32_t none;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint2 f = fv[4 * i];
+#pragma unroll
+                                for (int a = 0; a < 2; ++a) {
+                                    times_factors<false>(v[0][i >> 1][2 * (i & 1) + a], none, f);
+                                    times_factors<false>(v[1][i >> 1][2 * (i & 1) + a], none, f);
+                                }
                             }
                         }
                         tmem_st_frag16(to + kTmV, v[0][0]);
                         tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
-                        if (p.state_f32) {
-                            tmem_st_frag16(to + kTmVlo, u[0][0]);
-                            tmem_st_frag16(to + kTmVlo + (16u << 16), u[1][0]);
-                        }
                     }
                 }
                 if (__builtin_expect(packed && n < kChunk, 0)) {  // zero scores and values meet what the next sequence has there, but zero times its NaN is one
 #pragma unroll 1
                     for (int at = n * (DK / 8) + vtid; at < kChunk * (DK / 8); at += 128)
-                        *reinterpret_cast<uint4*>(stage + L::kOffK + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        *reinterpret_cast<uint4*>(tk + (at % (DK / 64)) * 8192 + at / (DK / 64) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     __syncwarp();
                     if (DV == 128 || lq < 2) {  // the columns of V that this warp has read itself
 #pragma unroll 1
                         for (int at = n * 4 + lane; at < kChunk * 4; at += 32)
-                            *reinterpret_cast<uint4*>(stage + L::kOffV + (lq >> 1) * 8192 + (at >> 2) * 128 + (((4 * (lq & 1) + (at & 3)) ^ ((at >> 2) & 7)) << 4)) =
+                            *reinterpret_cast<uint4*>(tv + (lq >> 1) * 8192 + (at >> 2) * 128 + (((4 * (lq & 1) + (at & 3)) ^ ((at >> 2) & 7)) << 4)) =
                                 make_uint4(0u, 0u, 0u, 0u);
                     }
                     fence_proxy_async_smem();
@@ -631,10 +671,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 tmem_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&bar_dgo[gc & 1]);
-                    mbar_arrive(&bar_p[gc & 1]);
-                }
+                if (lane == 0) mbar_arrive(&bar_dgo[gc & 1]);
             }
         }
     } else if (warp == 20) {
@@ -646,24 +683,25 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             const int tok0 = __shfl_sync(0xffffffffu, it.tok0, 0), dvt = __shfl_sync(0xffffffffu, it.dvt, 0);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                const uint32_t s = gc % kStages;
-                mbar_wait_short(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
-                uint8_t* st = smem + s * L::kStage;
+                const uint32_t s = gc % kStages, sq = gc % kStagesQ;
+                uint8_t *tk = smem + s * L::kTileK, *tq = smem + L::kOffQ + sq * L::kTileQ, *tv = smem + L::kOffV + s * L::kTileV;
                 const int tok = tok0 + c * kChunk;
+                mbar_wait_short(&bar_empty[s], ((gc / kStages) + 1) & 1, abort_flag);
+                mbar_wait_short(&bar_qempty[sq], ((gc / kStagesQ) + 1) & 1, abort_flag);
                 if (elect_one()) {
-                    mbar_arrive_expect_tx(&bar_full[s], L::kStage);
+                    mbar_arrive_expect_tx(&bar_full[s], 2 * L::kTileK + L::kTileV);
                     if (kWhole) {
-                        tma_load_5d(st + L::kOffK, &tmK, &bar_full[s], 0, tok, 0, khead, batch);
-                        tma_load_5d(st + L::kOffQ, &tmQ, &bar_full[s], 0, tok, 0, khead, batch);
-                        tma_load_5d(st + L::kOffV, &tmV, &bar_full[s], 0, tok, 2 * dvt, head, batch);
+                        tma_load_5d(tk, &tmK, &bar_full[s], 0, tok, 0, khead, batch);
+                        tma_load_5d(tq, &tmQ, &bar_full[s], 0, tok, 0, khead, batch);
+                        tma_load_5d(tv, &tmV, &bar_full[s], 0, tok, 2 * dvt, head, batch);
                     } else {
 #pragma unroll 1
                         for (int a = 0; a < DK / 64; ++a) {
-                            tma_load_4d(st + L::kOffK + a * 8192, &tmK, &bar_full[s], a * 64, khead, tok, batch);
-                            tma_load_4d(st + L::kOffQ + a * 8192, &tmQ, &bar_full[s], a * 64, khead, tok, batch);
+                            tma_load_4d(tk + a * 8192, &tmK, &bar_full[s], a * 64, khead, tok, batch);
+                            tma_load_4d(tq + a * 8192, &tmQ, &bar_full[s], a * 64, khead, tok, batch);
                         }
 #pragma unroll 1
-                        for (int a = 0; a < DV / 64; ++a) tma_load_4d(st + L::kOffV + a * 8192, &tmV, &bar_full[s], dvt * 128 + a * 64, head, tok, batch);
+                        for (int a = 0; a < DV / 64; ++a) tma_load_4d(tv + a * 8192, &tmV, &bar_full[s], dvt * 128 + a * 64, head, tok, batch);
                     }
                 }
                 __syncwarp();
@@ -679,22 +717,26 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
         // =============================================================== products of state and output
         constexpr uint32_t id_d = make_idesc_bf16(128, DK, false, true), id_o = make_idesc_bf16(128, 64, false, false), id_v = make_idesc_bf16(128, 64, true, false);
         // read MN-major (DV == 64: rows 64 on are what follows V's tile, and reach rows of O that nobody looks at)
-        const uint64_t dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 8192, 1024), dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), 8192, 1024);
+        const uint64_t dK = make_smem_desc_sw128(smem_u32(smem), 8192, 1024), dV = make_smem_desc_sw128(smem_u32(smem + L::kOffV), 8192, 1024);
         const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dP = make_smem_desc_sw128(smem_u32(smem + L::kOffP), 0, 1024);
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
                 const uint32_t s = gc % kStages, b = gc & 1;
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
-                mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
                 mbar_wait_short(&bar_dgo[b], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
-                mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmV + 32 * b, desc_advance(dK, s * L::kStage), id_d);
-                if (p.state_f32) mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmVlo + 32 * b, desc_advance(dK, s * L::kStage), id_d);
+                const uint64_t k = desc_advance(dK, s * L::kTileK), q = desc_advance(dQ, gc % kStagesQ * L::kTileQ);
+                mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmV + 32 * b, k, id_d);
+                if (kF32) mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmVlo + 32 * b, k, id_d);
                 mma_commit_w(&bar_d[b]);
-                if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
-                else mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmS, desc_advance(dQ, s * L::kStage), id_o);
-                mma_ss_k64_w<true, 128, 2>(tmem + kTmO + 64 * b, desc_advance(dV, s * L::kStage), desc_advance(dP, b * 8192), id_v);
+                if (gc > 1) mbar_wait_short(&bar_ofree[b], ((gc >> 1) + 1) & 1, abort_flag);  // O of two chunks before
+                mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);
+                tc_fence_after_sync();
+                if (DK == 128) mma_ts_k128_w<false>(tmem + kTmO + 64 * b, tmem + kTmS, q, id_o);
+                else mma_ts_k64_w<false, 2>(tmem + kTmO + 64 * b, tmem + kTmS, q, id_o);
+                mma_commit_w(&bar_s[b]);
+                mma_ss_k64_w<true, 128, 2>(tmem + kTmO + 64 * b, desc_advance(dV, s * L::kTileV), dP, id_v);
                 mma_commit_w(&bar_o[b]);
                 mma_commit_w(&bar_empty[s]);
             }
@@ -702,7 +744,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
     } else if (warp == 22) {
         // =============================================================== scores
         constexpr uint32_t id_qk = make_idesc_bf16(64, 64, false, false);
-        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem + L::kOffK), 0, 1024);
+        const uint64_t dQ = make_smem_desc_sw128(smem_u32(smem + L::kOffQ), 0, 1024), dK = make_smem_desc_sw128(smem_u32(smem), 0, 1024);
         while (next_item()) {
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
@@ -711,7 +753,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 if (gc > 1) mbar_wait_short(&bar_p[b], ((gc >> 1) + 1) & 1, abort_flag);  // the scores of two chunks before have been read
                 tc_fence_after_sync();
                 const uint32_t tP = tmem + kTmP + (b << 20);  // (16 lanes on for odd chunks)
-                const uint64_t q = desc_advance(dQ, s * L::kStage), k = desc_advance(dK, s * L::kStage);
+                const uint64_t q = desc_advance(dQ, gc % kStagesQ * L::kTileQ), k = desc_advance(dK, s * L::kTileK);
                 mma_ss_k64_w<false, 2, 2>(tP, q, k, id_qk);
                 if (DK == 128) mma_ss_k64_w<true, 2, 2>(tP, desc_advance(q, 8192), desc_advance(k, 8192), id_qk);
                 mma_commit_w(&bar_score[b]);
@@ -780,15 +822,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 if (__builtin_expect(plain, 1)) {
                     g0 += expo;
                     g1 += expo;
-                    gb[lane] = ex2(-g0);
-                    gb[lane + 32] = ex2(-g1);
+                    const float f0 = ex2(-g0), f1 = ex2(-g1);
+                    gb[lane] = f0;
+                    gb[lane + 32] = f1;
+                    put_factor(gb + 260, lane, f0);
+                    put_factor(gb + 260, lane + 32, f1);
                     gb[64 + lane] = p.scale * ex2(g0);
                     gb[96 + lane] = p.scale * ex2(g1);
                     expo += last;
                 } else {
                     behind = ex2(last);
-                    gb[lane] = ex2(last - g0);
-                    gb[lane + 32] = ex2(last - g1);
+                    put_factor(gb + 260, lane, ex2(last - g0));
+                    put_factor(gb + 260, lane + 32, ex2(last - g1));
                     gb[64 + lane] = gb[96 + lane] = p.scale;
                     gb[128 + lane] = g0;
                     gb[160 + lane] = g1;

@@ -4,6 +4,7 @@
 // so that every factor is a decay to the segment's end (at most one), the products simply accumulate, and what was read last, the
 // segment's beginning, is what the run over the chunks asks for first.
 // One CTA per segment but the last of a sequence, v-head and 128 columns of dv; two CTAs fit an SM.  HBM-bound (K and V once, 32 KB a chunk at d = 128).
+// Values as there: in two parts where the state is fp32.
 #pragma once
 #include "linear_chunked.cuh"
 
@@ -21,10 +22,10 @@ struct LinSegSmem {
 namespace lin {
 constexpr int kSegThreads = 224;   // 4 value warps, producer, issuer, gates
 constexpr uint32_t kTmSegF = 0;    // fp32 increment, 128 columns
-constexpr uint32_t kTmSegV = 128;  // 2 x bf16 V'^T, 32 columns; 2 x what is left of it
+constexpr uint32_t kTmSegV = 128;  // 2 x bf16 values times factors, 32 columns; 2 x what is left of them
 }  // namespace lin
 
-template <int DK, int DV, bool kWhole>
+template <int DK, int DV, bool kWhole, bool kF32>
 __global__ void __launch_bounds__(lin::kSegThreads, 2)
     gdn_linear_segment_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const LinChunkedParams p) {
     using namespace ptx;
@@ -89,33 +90,45 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             if (n > 1) mbar_wait_short(&bar_done[n & 1], ((n >> 1) + 1) & 1, abort_flag);
             mbar_wait_short(&bar_full[s], (n / kStages) & 1, abort_flag);
             tc_fence_after_sync();
-            const float* gb = factors(n);
+            const uint2* const fv = reinterpret_cast<const uint2*>(factors(n)) + (lane & 3);
             const uint32_t sV = smem_u32(smem + s * L::kStage + L::kOffV);
             if (DV == 128 || lq < 2) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {  // 32 tokens
-                    uint32_t v[2][2][4], u[2][2][4];
+                    uint32_t v[2][2][4];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         ldmatrix_x4_trans(sV + vsw0 + 4096 * hf + 2048 * j, v[0][j]);
                         ldmatrix_x4_trans(sV + vsw1 + 4096 * hf + 2048 * j, v[1][j]);
                     }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f2 f = *reinterpret_cast<const f2*>(gb + 32 * hf + 2 * (lane & 3) + 8 * i);
-#pragma unroll
-                        for (int a = 0; a < 2; ++a) {
-                            split_bf16(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
-                            split_bf16(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
-                        }
-                    }
                     const uint32_t to = tmem + kTmSegV + tm_lane + 32 * (n & 1) + 16 * hf;
-                    tmem_st_frag16(to, v[0][0]);
-                    tmem_st_frag16(to + (16u << 16), v[1][0]);
-                    if (p.state_f32) {
+                    if (kF32) {
+                        uint32_t u[2][2][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint2 f = fv[16 * hf + 4 * i];
+#pragma unroll
+                            for (int a = 0; a < 2; ++a) {
+                                times_factors<true>(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                                times_factors<true>(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
+                            }
+                        }
                         tmem_st_frag16(to + 64, u[0][0]);
                         tmem_st_frag16(to + 64 + (16u << 16), u[1][0]);
+                    } else {
+                        uint32_t none;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint2 f = fv[16 * hf + 4 * i];
+#pragma unroll
+                            for (int a = 0; a < 2; ++a) {
+                                times_factors<false>(v[0][i >> 1][2 * (i & 1) + a], none, f);
+                                times_factors<false>(v[1][i >> 1][2 * (i & 1) + a], none, f);
+                            }
+                        }
                     }
+                    tmem_st_frag16(to, v[0][0]);
+                    tmem_st_frag16(to + (16u << 16), v[1][0]);
                 }
             }
             tmem_wait_st();
@@ -182,7 +195,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             const uint32_t tV = tmem + kTmSegV + 32 * b;
             if (n == 0) mma_ts_k64_w<false, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
             else mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
-            if (p.state_f32) mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV + 64, desc_advance(dK, s * L::kStage), id_d);
+            if (kF32) mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV + 64, desc_advance(dK, s * L::kStage), id_d);
             mma_commit_w(&bar_done[b]);
             mma_commit_w(&bar_empty[s]);
         }
@@ -210,8 +223,8 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             const float last = __shfl_sync(0xffffffffu, g1, 31);
             mbar_wait_short(&bar_gfree[n & 3], ((n >> 2) + 1) & 1, abort_flag);
             float* gb = factors(n);
-            gb[lane] = ex2(suffix + (last - g0));
-            gb[lane + 32] = ex2(suffix + (last - g1));
+            put_factor(gb, lane, ex2(suffix + (last - g0)));
+            put_factor(gb, lane + 32, ex2(suffix + (last - g1)));
             suffix += last;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_gate[n & 3]);
