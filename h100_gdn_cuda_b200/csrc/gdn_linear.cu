@@ -116,11 +116,11 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (p.seg_state) {
-        if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole, kF32>>(LS::kBytes)) return rc;
+        if (int rc = set_smem<gdn_linear_segment_kernel<DK, DV, kWhole>>(LS::kBytes)) return rc;
         cfg.gridDim = dim3(static_cast<unsigned>(p.num_items - p.whole));
         cfg.blockDim = dim3(lin::kSegThreads);
         cfg.dynamicSmemBytes = LS::kBytes;
-        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole, kF32>, tmK, tmV, p));
+        GDN_CUDA(cudaLaunchKernelEx(&cfg, gdn_linear_segment_kernel<DK, DV, kWhole>, tmK, tmV, p));
         cfg.gridDim = dim3(static_cast<unsigned>(cut_chains), 128 * DK / 4 / kLinCombineThreads);
         cfg.blockDim = dim3(kLinCombineThreads);
         cfg.dynamicSmemBytes = 0;

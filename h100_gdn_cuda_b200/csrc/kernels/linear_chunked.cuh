@@ -12,9 +12,9 @@
 // 2^60 and more for the values in fp32.)  Other chunks form every decay as it stands in the first form, which cannot overflow: the scores take
 // e^{G_i - G_j}, the rows of Q are scaled where they lie, the values of the increment take e^{G_L - G_j} and the state is scaled between its read
 // and its increment.
-// Roundings: scores, the copy of the state that Q meets, and Q where it is scaled are bf16, once each.  Values of the increment are bf16 where the
-// state is; an fp32 state gets them in two parts, bf16 and what that leaves, by a second product (final states 2.3e-3 off without it, 5e-6 with;
-// 4 x 4096 tokens from DRAM 88 -> 91 us).
+// Roundings: scores, the copy of the state that Q meets, and Q where it is scaled are bf16, once each.  Values of the increment come in two parts, bf16
+// and what that leaves, by a second product: with one part fp32 states are 2.3e-3 off and with two 5e-6, outputs with bf16 states 2.8e-3 and 2.35e-3
+// (4 x 4096 tokens from DRAM 88 and 91 us, 2 x 131072 on 4 v-heads, back to back, 256 and 285).
 //
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
 // items and chunks, handing tiles on through mbarriers:
@@ -224,20 +224,13 @@ __device__ __forceinline__ void put_factor(float* factors, int token, float f) {
     to[0] = head;
     to[2] = __float2bfloat16(f - __bfloat162float(head));
 }
-// A pair of values times its factors: v, rounded to bf16 as an operand, and with kTwo what that leaves, to 2^-16 of it (v times a factor's head is exact in
-// the difference).
-template <bool kTwo>
+// A pair of values times its factors in two parts: v, rounded to bf16, and what that leaves, to 2^-16 of it (v times a factor's head is exact in the
+// difference).
 __device__ __forceinline__ void times_factors(uint32_t& v, uint32_t& rest, uint2 f) {
     const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162*>(&v), head = *reinterpret_cast<const __nv_bfloat162*>(&f.x), tail = *reinterpret_cast<const __nv_bfloat162*>(&f.y);
-    __nv_bfloat162 y;
-    if (kTwo) {
-        y = __hmul2_rn(x, head);
-        const __nv_bfloat162 r = __hfma2(x, tail, __hfma2(x, head, __hneg2(y)));
-        rest = *reinterpret_cast<const uint32_t*>(&r);
-    } else {
-        y = __hfma2(x, head, __hmul2_rn(x, tail));
-    }
+    const __nv_bfloat162 y = __hmul2_rn(x, head), r = __hfma2(x, tail, __hfma2(x, head, __hneg2(y)));
     v = *reinterpret_cast<const uint32_t*>(&y);
+    rest = *reinterpret_cast<const uint32_t*>(&r);
 }
 }  // namespace lin
 
@@ -626,31 +619,18 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         }
                         const uint32_t to = tmem + tm_lane + 32 * (gc & 1) + 16 * hf;
                         const uint2* const fv = reinterpret_cast<const uint2*>(gb + 260) + t0 / 2;
-                        if (kF32) {
-                            uint32_t u[2][2][4];
+                        uint32_t u[2][2][4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint2 f = fv[4 * i];
+                        for (int i = 0; i < 4; ++i) {
+                            const uint2 f = fv[4 * i];
 #pragma unroll
-                                for (int a = 0; a < 2; ++a) {
-                                    times_factors<true>(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
-                                    times_factors<true>(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
-                                }
-                            }
-                            tmem_st_frag16(to + kTmVlo, u[0][0]);
-                            tmem_st_frag16(to + kTmVlo + (16u << 16), u[1][0]);
-                        } else {
-                            uint32_t none;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint2 f = fv[4 * i];
-#pragma unroll
-                                for (int a = 0; a < 2; ++a) {
-                                    times_factors<false>(v[0][i >> 1][2 * (i & 1) + a], none, f);
-                                    times_factors<false>(v[1][i >> 1][2 * (i & 1) + a], none, f);
-                                }
+                            for (int a = 0; a < 2; ++a) {
+                                times_factors(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                                times_factors(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
                             }
                         }
+                        tmem_st_frag16(to + kTmVlo, u[0][0]);
+                        tmem_st_frag16(to + kTmVlo + (16u << 16), u[1][0]);
                         tmem_st_frag16(to + kTmV, v[0][0]);
                         tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
                     }
@@ -728,7 +708,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 tc_fence_after_sync();
                 const uint64_t k = desc_advance(dK, s * L::kTileK), q = desc_advance(dQ, gc % kStagesQ * L::kTileQ);
                 mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmV + 32 * b, k, id_d);
-                if (kF32) mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmVlo + 32 * b, k, id_d);
+                mma_ts_k64_w<true, 128>(tmem + kTmF, tmem + kTmVlo + 32 * b, k, id_d);
                 mma_commit_w(&bar_d[b]);
                 if (gc > 1) mbar_wait_short(&bar_ofree[b], ((gc >> 1) + 1) & 1, abort_flag);  // O of two chunks before
                 mbar_wait_short(&bar_p[b], (gc >> 1) & 1, abort_flag);

@@ -3,8 +3,8 @@
 // and the segment's whole decay; then the states that enter the segments, S <- e^{G} S + D from segment to segment.  The chunks are taken last to first,
 // so that every factor is a decay to the segment's end (at most one), the products simply accumulate, and what was read last, the
 // segment's beginning, is what the run over the chunks asks for first.
-// One CTA per segment but the last of a sequence, v-head and 128 columns of dv; two CTAs fit an SM.  HBM-bound (K and V once, 32 KB a chunk at d = 128).
-// Values as there: in two parts where the state is fp32.
+// One CTA per segment but the last of a sequence, v-head and 128 columns of dv; two CTAs fit an SM.  HBM-bound (K and V once, 32 KB a chunk at d = 128).  Values
+// come in two parts as there.
 #pragma once
 #include "linear_chunked.cuh"
 
@@ -25,7 +25,7 @@ constexpr uint32_t kTmSegF = 0;    // fp32 increment, 128 columns
 constexpr uint32_t kTmSegV = 128;  // 2 x bf16 values times factors, 32 columns; 2 x what is left of them
 }  // namespace lin
 
-template <int DK, int DV, bool kWhole, bool kF32>
+template <int DK, int DV, bool kWhole>
 __global__ void __launch_bounds__(lin::kSegThreads, 2)
     gdn_linear_segment_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const LinChunkedParams p) {
     using namespace ptx;
@@ -102,31 +102,18 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
                         ldmatrix_x4_trans(sV + vsw1 + 4096 * hf + 2048 * j, v[1][j]);
                     }
                     const uint32_t to = tmem + kTmSegV + tm_lane + 32 * (n & 1) + 16 * hf;
-                    if (kF32) {
-                        uint32_t u[2][2][4];
+                    uint32_t u[2][2][4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint2 f = fv[16 * hf + 4 * i];
+                    for (int i = 0; i < 4; ++i) {
+                        const uint2 f = fv[16 * hf + 4 * i];
 #pragma unroll
-                            for (int a = 0; a < 2; ++a) {
-                                times_factors<true>(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
-                                times_factors<true>(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
-                            }
-                        }
-                        tmem_st_frag16(to + 64, u[0][0]);
-                        tmem_st_frag16(to + 64 + (16u << 16), u[1][0]);
-                    } else {
-                        uint32_t none;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint2 f = fv[16 * hf + 4 * i];
-#pragma unroll
-                            for (int a = 0; a < 2; ++a) {
-                                times_factors<false>(v[0][i >> 1][2 * (i & 1) + a], none, f);
-                                times_factors<false>(v[1][i >> 1][2 * (i & 1) + a], none, f);
-                            }
+                        for (int a = 0; a < 2; ++a) {
+                            times_factors(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
+                            times_factors(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
                         }
                     }
+                    tmem_st_frag16(to + 64, u[0][0]);
+                    tmem_st_frag16(to + 64 + (16u << 16), u[1][0]);
                     tmem_st_frag16(to, v[0][0]);
                     tmem_st_frag16(to + (16u << 16), v[1][0]);
                 }
@@ -195,7 +182,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             const uint32_t tV = tmem + kTmSegV + 32 * b;
             if (n == 0) mma_ts_k64_w<false, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
             else mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV, desc_advance(dK, s * L::kStage), id_d);
-            if (kF32) mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV + 64, desc_advance(dK, s * L::kStage), id_d);
+            mma_ts_k64_w<true, 128>(tmem + kTmSegF, tV + 64, desc_advance(dK, s * L::kStage), id_d);
             mma_commit_w(&bar_done[b]);
             mma_commit_w(&bar_empty[s]);
         }

@@ -398,3 +398,13 @@ def test_fp32_states_of_prompts(shape, gate):
     ref, sref = O.linear_attention_ref(p["q"], p["k"], p["v"], p["g"], shape[4] ** -0.5, p["s"], False)
     assert s.dtype == torch.float32 and (s.double() - sref).norm() <= 2.0 ** -15 * sref.norm()
     check(o, s, p, True)
+
+
+@pytest.mark.parametrize("gate", ["head", "token"])
+def test_bf16_states_of_prompts(gate):
+    """They are the fp32 ones (test_fp32_states_of_prompts), rounded once: half a step at most for every value, and 2^-15 of the norm beside that."""
+    p = make(1, 2000, 2, 4, 128, 128, gate=gate, state=torch.bfloat16)
+    o, s = gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"], None, p["s"])
+    _, sref = O.linear_attention_ref(p["q"], p["k"], p["v"], p["g"], 128 ** -0.5, p["s"], False)
+    excess = ((s.double() - sref).abs() - U16 * sref.abs()).clamp_min(0)
+    assert s.dtype == torch.bfloat16 and excess.norm() <= 2.0 ** -15 * sref.norm()
