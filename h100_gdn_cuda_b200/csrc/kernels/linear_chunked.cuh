@@ -177,7 +177,7 @@ struct LinSmem {
     static constexpr int kOffQ = kOffV + kStages * kTileV;
     static constexpr int kOffP = kOffQ + kStagesQ * kTileQ;  // scores, 64 x 64
     // 4 x gate factors, fp32: of the scores [64]; of the output [64]; not plain: G[64] (log2), e^{G_i}[64]; of the state in front of its copy
-    // and behind it; 2^c behind the chunk; plain or not; of the values [64] (see put_factor)
+    // and behind it; 2^c behind the chunk; plain or not; of the values [64] (see factor_pair)
     static constexpr int kOffGate = kOffP + 8192;
     static constexpr int kGateStride = (5 * 64 + 4) * 4;
     static constexpr int kOffBar = kOffGate + 4 * kGateStride;
@@ -195,17 +195,17 @@ constexpr uint32_t kTmVlo = 448; // 2 x bf16: what is left of it
 constexpr float kPlainLog2 = 60.f;
 __device__ __forceinline__ void named_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 using namespace pairs;
-// the running sums of 64 log2-decays, lane l: tokens l and l + 32
+// the running sums of 64 log2-decays, lane l: tokens 2l and 2l + 1
 __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
+    float sum = g0 + g1;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
-        const float y0 = __shfl_up_sync(0xffffffffu, g0, m), y1 = __shfl_up_sync(0xffffffffu, g1, m);
-        if (lane >= m) {
-            g0 += y0;
-            g1 += y1;
-        }
+        const float y = __shfl_up_sync(0xffffffffu, sum, m);
+        if (lane >= m) sum += y;
     }
-    g1 += __shfl_sync(0xffffffffu, g0, 31);
+    sum = __shfl_up_sync(0xffffffffu, sum, 1);
+    if (lane > 0) g0 += sum;
+    g1 += g0;
 }
 // 16 bytes of K times a factor (rounded to bf16 once, as an operand)
 __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
@@ -217,12 +217,11 @@ __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
     v.w = pack2(mul2(pk(bf16_lo(v.w), bf16_hi(v.w)), w));
     return v;
 }
-// Factors of values as two bf16 numbers each, which is 2^-16 of them: those of tokens 2t and 2t + 1 are pairs behind one another.
-__device__ __forceinline__ void put_factor(float* factors, int token, float f) {
-    __nv_bfloat16* const to = reinterpret_cast<__nv_bfloat16*>(factors) + 4 * (token >> 1) + (token & 1);
-    const __nv_bfloat16 head = __float2bfloat16(f);
-    to[0] = head;
-    to[2] = __float2bfloat16(f - __bfloat162float(head));
+// Factors of values as two bf16 numbers each, which is 2^-16 of them; those of tokens 2t and 2t + 1, a pair each.
+__device__ __forceinline__ uint2 factor_pair(float f0, float f1) {
+    using namespace ptx;
+    const uint32_t head = pack2(pk(f0, f1));
+    return make_uint2(head, pack2(pk(f0 - bf16_lo(head), f1 - bf16_hi(head))));
 }
 // A pair of values times its factors in two parts: v, rounded to bf16, and what that leaves, to 2^-16 of it (v times a factor's head is exact in the
 // difference).
@@ -753,16 +752,16 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             ++n;
         };
         const int size_log2 = p.gate.is_f32 ? 2 : 1;
-        const char* from = nullptr;  // the next chunk's gate of this lane
+        const char* from = nullptr;  // the next chunk's gates of this lane
         auto load1 = [&](const char* at, bool there) {  // as bits, converted where it is used
             uint32_t bits = 0u;
             if (there) bits = size_log2 == 2 ? __ldg(reinterpret_cast<const uint32_t*>(at)) : static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(at))) << 16;
             return bits;
         };
         auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
-            const int t = c * kChunk + lane, end = p.gate.ptr ? it.tokens : 0;
+            const int t = c * kChunk + 2 * lane, end = p.gate.ptr ? it.tokens : 0;
             a0 = load1(from, t < end);
-            a1 = load1(from + (p.gate.st << (5 + size_log2)), t + 32 < end);
+            a1 = load1(from + (p.gate.st << size_log2), t + 1 < end);
             from += p.gate.st << (6 + size_log2);
         };
         // The launch has a block for every item.  A block that runs asks for the next one that has not started and takes it over.
@@ -774,7 +773,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             hand_out();
             uint32_t a0, a1, b0, b1, c0, c1;  // the gates of this chunk and the two behind it: DRAM answers later than a chunk takes
             float expo = 0.f;  // c
-            from = static_cast<const char*>(p.gate.ptr) + ((it.batch * p.gate.sb + (it.tok0 + lane) * p.gate.st + it.head * p.gate.sh) << size_log2);
+            from = static_cast<const char*>(p.gate.ptr) + ((it.batch * p.gate.sb + (it.tok0 + 2 * lane) * p.gate.st + it.head * p.gate.sh) << size_log2);
             load(0, a0, a1);
             load(1, b0, b1);
             load(2, c0, c1);
@@ -799,26 +798,22 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 }
                 mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
+                float2* const gb2 = reinterpret_cast<float2*>(gb);
+                uint2* const factors = reinterpret_cast<uint2*>(gb + 260);
                 if (__builtin_expect(plain, 1)) {
                     g0 += expo;
                     g1 += expo;
                     const float f0 = ex2(-g0), f1 = ex2(-g1);
-                    gb[lane] = f0;
-                    gb[lane + 32] = f1;
-                    put_factor(gb + 260, lane, f0);
-                    put_factor(gb + 260, lane + 32, f1);
-                    gb[64 + lane] = p.scale * ex2(g0);
-                    gb[96 + lane] = p.scale * ex2(g1);
+                    gb2[lane] = make_float2(f0, f1);
+                    gb2[32 + lane] = make_float2(p.scale * ex2(g0), p.scale * ex2(g1));
+                    factors[lane] = factor_pair(f0, f1);
                     expo += last;
                 } else {
                     behind = ex2(last);
-                    put_factor(gb + 260, lane, ex2(last - g0));
-                    put_factor(gb + 260, lane + 32, ex2(last - g1));
-                    gb[64 + lane] = gb[96 + lane] = p.scale;
-                    gb[128 + lane] = g0;
-                    gb[160 + lane] = g1;
-                    gb[192 + lane] = ex2(g0);
-                    gb[224 + lane] = ex2(g1);
+                    factors[lane] = factor_pair(ex2(last - g0), ex2(last - g1));
+                    gb2[32 + lane] = make_float2(p.scale, p.scale);
+                    gb2[64 + lane] = make_float2(g0, g1);
+                    gb2[96 + lane] = make_float2(ex2(g0), ex2(g1));
                 }
                 if (lane == 0) *reinterpret_cast<float4*>(gb + 256) = make_float4(before, behind, ex2(expo), plain ? 1.f : 0.f);
                 __syncwarp();

@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
         auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
             a0 = a1 = 0u;
             if (c >= 0 && p.gate.ptr) {  // (segments in front of the last one are whole chunks)
-                a0 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + lane, it.head);
-                a1 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + 32 + lane, it.head);
+                a0 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + 2 * lane, it.head);
+                a1 = p.gate.load_bits(it.batch, it.tok0 + c * kChunk + 2 * lane + 1, it.head);
             }
         };
         uint32_t a0, a1, b0, b1, c0, c1;  // the gates of this chunk and the two in front of it: DRAM answers later than a chunk takes
@@ -209,9 +209,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             scan64(g0, g1, lane);
             const float last = __shfl_sync(0xffffffffu, g1, 31);
             mbar_wait_short(&bar_gfree[n & 3], ((n >> 2) + 1) & 1, abort_flag);
-            float* gb = factors(n);
-            put_factor(gb, lane, ex2(suffix + (last - g0)));
-            put_factor(gb, lane + 32, ex2(suffix + (last - g1)));
+            reinterpret_cast<uint2*>(factors(n))[lane] = factor_pair(ex2(suffix + (last - g0)), ex2(suffix + (last - g1)));
             suffix += last;
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_gate[n & 3]);
