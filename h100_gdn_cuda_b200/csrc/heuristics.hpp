@@ -229,10 +229,11 @@ inline int conv_tok_block(long long tokens, long long blocks_per_token_block, in
 }
 
 // Linear attention, prompts: which of `chains` (sequence, v-head, dv tile) chains of `chunks` chunks each (packed: on average) are cut into how many
-// segments.  A chain alone takes about 0.93 us a chunk, 148 of them at once 1.15 (HBM-bound); cut ones 1.75, since K and V are read twice, and the
-// two launches more some 13 us.  Cut : whole, us, d=128: 8 chains of 2048 chunks (2 x 131072 tokens, 4 v-heads) 222 : 1745, 32 of 124 78 : 116,
-// 32 of 32 34.2 : 37.2, 8 of 16 24.7 : 23.6 (whole); 96 packed ones of 104 on average 165 : 136 (whole).  Where more chains than SMs leave a last round that is not
-// full, those of that round are cut (in no more segments than have 12 chunks each: an item has its own start): 160 of 52 106 : 119.
+// segments.  A chain alone takes about 1.02 us a chunk, 148 of them at once 1.2 (HBM-bound); cut ones 1.87, since K and V are read twice, and the
+// two launches more some 12 us.  Cut : whole, us, d=128: 8 chains of 2048 chunks (2 x 131072 tokens, 4 v-heads) 241 : 2102, 32 of 124 79 : 136,
+// 32 of 32 36.4 : 41.7, 32 of 24 33.0 : 33.6, 8 of 24 26.5 : 33.0, 8 of 16 25.5 : 25.1 (whole), 8 of 10 26.3 : 19.0 (whole); 24 packed ones of 104 on average
+// 57 : 119.  Where more chains than SMs leave a last round that is not full, those of that round are cut (in no more segments than have 12
+// chunks each: an item has its own start): 160 of 52 113 : 130.
 struct LinearCut {
     long long whole;       // the first chains, which stay whole (padded)
     long long segments;    // 1: nothing is cut
@@ -245,9 +246,9 @@ inline LinearCut linear_cut(long long chains, long long chunks, bool packed) {
     if (rest == 0 || rest > kSms / 2) return none;
     const long long parts = std::min(kSms / rest, std::max(1ll, chunks / (rounds > 0 ? 12 : 4)));
     const long long per = (chunks + parts - 1) / parts;
-    const double before = 1.15 * static_cast<double>(rounds * chunks);
-    const double cut = 20.0 + (rounds > 0 ? 10.0 : 0.0) + before + 1.75 * static_cast<double>(per);
-    const double whole = 7.0 + before + 0.93 * static_cast<double>(chunks);
+    const double before = 1.2 * static_cast<double>(rounds * chunks);
+    const double cut = 21.0 + (rounds > 0 ? 10.0 : 0.0) + before + 1.87 * static_cast<double>(per);
+    const double whole = 9.0 + before + 1.02 * static_cast<double>(chunks);
     if (parts < 2 || cut >= whole) return none;
     return LinearCut{rounds * kSms, (chunks + per - 1) / per, per};
 }
