@@ -146,7 +146,7 @@ int whole_bytes(int64_t rows, int width, int vec, int size, int threads) {
 //    channels, bf16, 32 groups of 200 KB 21 -> 30 us, of 150 KB 20 -> 16), and where CTAs come in several waves, or read a gate as well, the
 //    sectors that groups share move twice (512 groups of 64 KB 33 -> 42 us, 256 of 40 KB 20 -> 14; gated, 512 of 48 KB 30 -> 42, of 16 KB 19 -> 11).
 bool whole_groups(int64_t count, int64_t rows, int width, int vec, int size, bool gated) {
-    const int bytes = whole_bytes(rows, width, vec, size, 1024);
+    const int bytes = whole_bytes(rows, width, vec, size, 512);
     if (bytes == 0 || (rows * width * size < 16 * 1024 && count > 2048)) return false;
     return width * size % 32 == 0 || bytes <= (gated ? 24 : count > 148 ? 48 : 176) * 1024;
 }
@@ -158,14 +158,14 @@ int launch_whole(const GroupNormParams& p, cudaStream_t st) {
         constexpr bool kG = decltype(gated)::value;
         const int small = whole_bytes(p.l, p.width, V, sizeof(T), 256);
         const unsigned grid = static_cast<unsigned>(p.n * p.groups);
-        // (512 groups of 64 KB: 29 us with CTAs of 1024 threads, 20 with three of 256 on an SM; of 150 KB: 51 and 54.  Copies that go through L1
-        // are better few at a time: 128 groups of 160 KB, 20 channels, 21 and 19)
+        // (512 groups of 64 KB: 29 us with CTAs of 1024 threads, 20 with three of 256 on an SM; of 100 KB 41 with 1024 and 31 with two of 512; of 150 KB
+        // 51 with either.  Copies that go through L1 are better few at a time: 128 groups of 160 KB, 20 channels, 20 us with 512, 19 with 256)
         if (small > 0 && (small <= kNormPartBytes || V * sizeof(T) < 16)) {
             if (int rc = set_smem<gdn_group_norm_whole_kernel<T, V, 256, kG>>(kNormWholeBytes)) return rc;
             GDN_CUDA(launch_dependent(gdn_group_norm_whole_kernel<T, V, 256, kG>, grid, 256, small, st, p));
         } else {
-            if (int rc = set_smem<gdn_group_norm_whole_kernel<T, V, 1024, kG>>(kNormWholeBytes)) return rc;
-            GDN_CUDA(launch_dependent(gdn_group_norm_whole_kernel<T, V, 1024, kG>, grid, 1024, whole_bytes(p.l, p.width, V, sizeof(T), 1024), st, p));
+            if (int rc = set_smem<gdn_group_norm_whole_kernel<T, V, 512, kG>>(kNormWholeBytes)) return rc;
+            GDN_CUDA(launch_dependent(gdn_group_norm_whole_kernel<T, V, 512, kG>, grid, 512, whole_bytes(p.l, p.width, V, sizeof(T), 512), st, p));
         }
         return GDN_OK;
     };
