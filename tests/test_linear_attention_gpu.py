@@ -408,3 +408,35 @@ def test_bf16_states_of_prompts(gate):
     _, sref = O.linear_attention_ref(p["q"], p["k"], p["v"], p["g"], 128 ** -0.5, p["s"], False)
     excess = ((s.double() - sref).abs() - U16 * sref.abs()).clamp_min(0)
     assert s.dtype == torch.bfloat16 and excess.norm() <= 2.0 ** -15 * sref.norm()
+
+
+@pytest.mark.parametrize("tokens", [70, 3000])
+def test_no_states_through_the_library(tokens):
+    """initial, final and new states may be NULL; a workspace that is too small or unaligned is refused."""
+    import ctypes as C
+    from h100_gdn_cuda_b200 import _cabi as cabi, api
+    p = make(1, tokens, 1, 2, 64, 64, gate="token", state=None)
+    shape, q, k, v, g, _, _, _ = api._linear_inputs(p["q"], p["k"], p["v"], p["g"], None, None, False, False)
+    lib, st, none = cabi.load(), torch.cuda.current_stream().cuda_stream, cabi.State(None, 0, 0)
+    need = lib.gdn_linear_chunked_workspace_bytes(C.byref(shape))
+    ws = torch.empty(need + 256, dtype=torch.uint8, device="cuda")
+    want = gdn.linear_attention_chunked(p["q"], p["k"], p["v"], p["g"])[0]
+    for dtype in (cabi.GDN_F32, cabi.GDN_BF16):
+        out = torch.full_like(v, 7.0)
+        a = cabi.LinearChunkedArgs(shape, *(api._linear_tokens(t, False) for t in (q, k, v, out)), g, none, none, 64 ** -0.5, dtype, ws.data_ptr(), need)
+        cabi.check(lib.gdn_linear_chunked(C.byref(a), st), "chunked")
+        assert torch.equal(out, want)
+        if need:
+            for ptr, size in ((ws.data_ptr(), need - 1), (ws.data_ptr() + 16, need), (None, 0)):
+                a.workspace, a.workspace_bytes = ptr, size
+                assert lib.gdn_linear_chunked(C.byref(a), st) == -4
+        if tokens < 100:
+            r = cabi.LinearRecurrentArgs(shape, *(api._linear_tokens(t, False) for t in (q, k, v, out)), g, none, none, None, None, 0, 64 ** -0.5, 0, dtype)
+            cabi.check(lib.gdn_linear_recurrent(C.byref(r), st), "recurrent")
+            # (lanes hold other columns where states are fp32: sums in another order, so within the module's bound and not at the same bits)
+            ref, _ = O.linear_attention_ref(p["q"], p["k"], p["v"], p["g"], 64 ** -0.5, None, False)
+            mag, _ = O.linear_attention_ref(p["q"].abs(), p["k"].abs(), p["v"].abs(), p["g"], 64 ** -0.5, None, False)
+            assert bool(((out.double() - ref).abs() <= U16 * ref.abs() + (64 + 16 * tokens + 32) * U32 * mag).all())
+            if dtype == cabi.GDN_BF16:
+                assert torch.equal(out, gdn.linear_attention_recurrent(p["q"], p["k"], p["v"], None, p["g"])[0])
+    assert need > 0 or tokens < 100
