@@ -207,6 +207,15 @@ __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
     if (lane > 0) g0 += sum;
     g1 += g0;
 }
+// x += y for a sum of many terms, kept as two numbers: x, and what it leaves of the exact sum (`rest`, which enters with y).  With one number
+// the rounding of a sum that wanders up to 60 has the same sign chunk after chunk where a head's decay is slow: a state alone, decayed over
+// 131072 tokens at g = -1e-4, was 2.5e-4 off, at -3e-4 5.3e-4; with two 8e-7 and 1.3e-7.
+__device__ __forceinline__ void add_kept(float& x, float& rest, float y) {
+    y += rest;
+    const float sum = x + y, part = sum - x;
+    rest = (x - (sum - part)) + (y - part);
+    x = sum;
+}
 // 16 bytes of K times a factor (rounded to bf16 once, as an operand)
 __device__ __forceinline__ uint4 scale8(uint4 v, float f) {
     using namespace ptx;
@@ -772,7 +781,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             if (!walker.locate(p, i, it)) break;  // (surplus items are the last ones)
             hand_out();
             uint32_t a0, a1, b0, b1, c0, c1;  // the gates of this chunk and the two behind it: DRAM answers later than a chunk takes
-            float expo = 0.f;  // c
+            float expo = 0.f, expo_rest = 0.f;  // c
             from = static_cast<const char*>(p.gate.ptr) + ((it.batch * p.gate.sb + (it.tok0 + 2 * lane) * p.gate.st + it.head * p.gate.sh) << size_log2);
             load(0, a0, a1);
             load(1, b0, b1);
@@ -786,28 +795,29 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 scan64(g0, g1, lane);  // (tokens past the end have no decay: they carry the last one's sum)
                 const float last = __shfl_sync(0xffffffffu, g1, 31);
                 // (a NaN is not plain, neither are gates that grow)
-                auto within = [&](float c) { return __all_sync(0xffffffffu, fabsf(g0 + c) <= kPlainLog2 && fabsf(g1 + c) <= kPlainLog2); };
+                auto within = [&](float c, float rest) { return __all_sync(0xffffffffu, fabsf(g0 + rest + c) <= kPlainLog2 && fabsf(g1 + rest + c) <= kPlainLog2); };
                 float before = 1.f, behind = 1.f;
-                bool plain = within(expo);
+                bool plain = within(expo, expo_rest);
                 if (__builtin_expect(!plain, 0)) {  // the state takes another exponent, the largest one if that does
-                    plain = within(kPlainLog2);
+                    plain = within(kPlainLog2, 0.f);
                     const float other = plain ? kPlainLog2 : 0.f;
-                    if (!plain) plain = within(0.f);
-                    before = ex2(expo - other);
+                    if (!plain) plain = within(0.f, 0.f);
+                    before = ex2(expo - other + expo_rest);
                     expo = other;
+                    expo_rest = 0.f;
                 }
                 mbar_wait_short(&bar_gfree[gc & 3], ((gc >> 2) + 1) & 1, abort_flag);
                 float* gb = gate_buf(gc);
                 float2* const gb2 = reinterpret_cast<float2*>(gb);
                 uint2* const factors = reinterpret_cast<uint2*>(gb + 260);
                 if (__builtin_expect(plain, 1)) {
-                    g0 += expo;
-                    g1 += expo;
+                    g0 = g0 + expo_rest + expo;
+                    g1 = g1 + expo_rest + expo;
                     const float f0 = ex2(-g0), f1 = ex2(-g1);
                     gb2[lane] = make_float2(f0, f1);
                     gb2[32 + lane] = make_float2(p.scale * ex2(g0), p.scale * ex2(g1));
                     factors[lane] = factor_pair(f0, f1);
-                    expo += last;
+                    add_kept(expo, expo_rest, last);
                 } else {
                     behind = ex2(last);
                     factors[lane] = factor_pair(ex2(last - g0), ex2(last - g1));
@@ -815,7 +825,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     gb2[64 + lane] = make_float2(g0, g1);
                     gb2[96 + lane] = make_float2(ex2(g0), ex2(g1));
                 }
-                if (lane == 0) *reinterpret_cast<float4*>(gb + 256) = make_float4(before, behind, ex2(expo), plain ? 1.f : 0.f);
+                if (lane == 0) *reinterpret_cast<float4*>(gb + 256) = make_float4(before, behind, ex2(expo + expo_rest), plain ? 1.f : 0.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gate[gc & 3]);
             }

@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
         }
     } else {
         // =============================================================== gates
-        float suffix = 0.f;  // of the chunks behind, log2
+        float suffix = 0.f, suffix_rest = 0.f;  // of the chunks behind, log2
         auto load = [&](int c, uint32_t& a0, uint32_t& a1) {
             a0 = a1 = 0u;
             if (c >= 0 && p.gate.ptr) {  // (segments in front of the last one are whole chunks)
@@ -209,12 +209,12 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             scan64(g0, g1, lane);
             const float last = __shfl_sync(0xffffffffu, g1, 31);
             mbar_wait_short(&bar_gfree[n & 3], ((n >> 2) + 1) & 1, abort_flag);
-            reinterpret_cast<uint2*>(factors(n))[lane] = factor_pair(ex2(suffix + (last - g0)), ex2(suffix + (last - g1)));
-            suffix += last;
+            reinterpret_cast<uint2*>(factors(n))[lane] = factor_pair(ex2(suffix + (suffix_rest + (last - g0))), ex2(suffix + (suffix_rest + (last - g1))));
+            add_kept(suffix, suffix_rest, last);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_gate[n & 3]);
         }
-        if (lane == 0) p.seg_decay[it.mine] = suffix;
+        if (lane == 0) p.seg_decay[it.mine] = suffix + suffix_rest;
     }
     tc_fence_before_sync();
     __syncthreads();

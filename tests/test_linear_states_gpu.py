@@ -1,0 +1,47 @@
+"""fp32 states of linear attention's prompts against 64 bits, heads that forget slowly."""
+import pytest
+import torch
+
+import h100_gdn_cuda_b200 as gdn
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(gen, *shape):
+    return torch.randn(*shape, generator=gen, device="cuda")
+
+
+@pytest.mark.parametrize("heads,bound", [(80, 2.0 ** -16), (4, 2.0 ** -15)], ids=["whole", "cut"])
+def test_a_state_alone(heads, bound):
+    """Values of zero: a state only decays, by e^{g T}, over 1024 chunks.  Chains that stay whole (more than half as many as SMs) and cut ones.
+
+    The exponent, E = 28.4 in log2 at most, is off by the gate's conversion (two half steps, 2^-24 of it each) and by a chunk's sum (seven), 9 2^-24 E, and by half a
+    step of 2^-18 each where the state takes an exponent of up to 60 and gives it back: 1.9e-5, of which ln 2 is 1.3e-5.  Two powers of two, 2^-22 each: below 2^-16.  Cut chains take
+    a power of two, rounded, in each of up to 37 segments: 37 (2^-22 + 2^-24) = 1.1e-5 more, below 2^-15."""
+    T, d = 65536, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k = normal(gen, 1, T, 1, d).bfloat16(), normal(gen, 1, T, 1, d).bfloat16()
+    v = torch.zeros(1, T, heads, d, dtype=torch.bfloat16, device="cuda")
+    s0 = normal(gen, 1, heads, d, d)
+    g = -torch.linspace(1e-4, 3e-4, heads, device="cuda")
+    _, s = gdn.linear_attention_chunked(q, k, v, g, None, s0)
+    ref = torch.exp(g.double() * T)[None, :, None, None] * s0.double()
+    assert bool(((s.double() - ref).abs() <= bound * ref.abs()).all()), ((s.double() - ref).abs() / ref.abs()).amax((0, 2, 3))
+
+
+@pytest.mark.parametrize("heads", [80, 4], ids=["whole", "cut"])
+def test_slow_decays(heads):
+    """The same with values, as a part of the state's norm.  Values enter in two parts, within 2^-16; decays as above, within 2^-16.  Sums on the tensor cores are
+    cut off rather than rounded: a step of 2^-23 at most for each of the eight sums of 16 products that 64 tokens are, over the min(T, 1 / -g) tokens that a
+    head remembers."""
+    T, d = 16384, 64
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = normal(gen, 1, T, 1, d).bfloat16(), normal(gen, 1, T, 1, d).bfloat16(), normal(gen, 1, T, heads, d).bfloat16()
+    s0 = normal(gen, 1, heads, d, d)
+    g = -torch.logspace(-6, -1, heads, base=10.0, device="cuda")
+    _, s = gdn.linear_attention_chunked(q, k, v, g, None, s0)
+    ages = torch.arange(T - 1, -1, -1, dtype=torch.float64, device="cuda")
+    for h in range(0, heads, max(1, heads // 10)):
+        ref = (v[0, :, h].double() * torch.exp(g[h].double() * ages)[:, None]).T @ k[0, :, 0].double() + torch.exp(g[h].double() * T) * s0[0, h].double()
+        memory = min(T, -1 / g[h].item())
+        assert (s[0, h].double() - ref).norm() <= (2.0 ** -15 + memory / 8 * 2.0 ** -23) * ref.norm()
