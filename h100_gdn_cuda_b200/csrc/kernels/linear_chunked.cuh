@@ -65,7 +65,7 @@ struct LinChunkedParams {
 };
 
 // Decays are handled as powers of two; anything below 2^-160 is zero in fp32, and sums of 64 such stay exact enough to tell G_i - G_j
-// where a chunk forgets several times over (64 x 160 has a spacing of 2^-10).  A NaN stays one.
+// where a chunk forgets several times over (64 x 160 has a spacing of 2^-10, less than the scores' bf16).  A NaN stays one.
 __device__ __forceinline__ float lin_gate_log2(float g) {
     const float x = g * 1.4426950408889634f;
     return x < -160.f ? -160.f : x;
@@ -206,6 +206,20 @@ __device__ __forceinline__ void scan64(float& g0, float& g1, int lane) {
     sum = __shfl_up_sync(0xffffffffu, sum, 1);
     if (lane > 0) g0 += sum;
     g1 += g0;
+}
+// The same for what lies behind each token; returns the sum of all 64.  A difference of two sums from the front has the spacing of the larger one, 2^-10
+// where a chunk forgets 64 times over; these are off by half steps of their own size, and count where they are small.
+__device__ __forceinline__ float scan64_behind(float& g0, float& g1, int lane) {
+    float sum = g0 + g1;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+        const float y = __shfl_down_sync(0xffffffffu, sum, m);
+        if (lane + m < 32) sum += y;
+    }
+    const float all = __shfl_sync(0xffffffffu, sum, 0), behind = __shfl_down_sync(0xffffffffu, sum, 1);
+    g0 = lane < 31 ? behind + g1 : g1;
+    g1 = lane < 31 ? behind : 0.f;
+    return all;
 }
 // x += y for a sum of many terms, kept as two numbers: x, and what it leaves of the exact sum (`rest`, which enters with y).  With one number
 // the rounding of a sum that wanders up to 60 has the same sign chunk after chunk where a head's decay is slow: a state alone, decayed over
@@ -788,7 +802,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             load(2, c0, c1);
 #pragma unroll 1
             for (int c = 0; c < it.chunks; ++c, ++gc) {
-                float g0 = lin_gate_log2(__uint_as_float(a0)), g1 = lin_gate_log2(__uint_as_float(a1));
+                float g0 = lin_gate_log2(__uint_as_float(a0)), g1 = lin_gate_log2(__uint_as_float(a1)), r0 = g0, r1 = g1;
                 a0 = b0; a1 = b1;
                 b0 = c0; b1 = c1;
                 load(c + 3, c0, c1);
@@ -820,7 +834,8 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     add_kept(expo, expo_rest, last);
                 } else {
                     behind = ex2(last);
-                    factors[lane] = factor_pair(ex2(last - g0), ex2(last - g1));
+                    scan64_behind(r0, r1, lane);
+                    factors[lane] = factor_pair(ex2(r0), ex2(r1));
                     gb2[32 + lane] = make_float2(p.scale, p.scale);
                     gb2[64 + lane] = make_float2(g0, g1);
                     gb2[96 + lane] = make_float2(ex2(g0), ex2(g1));

@@ -206,11 +206,10 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
             a0 = b0; a1 = b1;
             b0 = c0; b1 = c1;
             load(chunks - 4 - n, c0, c1);
-            scan64(g0, g1, lane);
-            const float last = __shfl_sync(0xffffffffu, g1, 31);
+            const float all = scan64_behind(g0, g1, lane);
             mbar_wait_short(&bar_gfree[n & 3], ((n >> 2) + 1) & 1, abort_flag);
-            reinterpret_cast<uint2*>(factors(n))[lane] = factor_pair(ex2(suffix + (suffix_rest + (last - g0))), ex2(suffix + (suffix_rest + (last - g1))));
-            add_kept(suffix, suffix_rest, last);
+            reinterpret_cast<uint2*>(factors(n))[lane] = factor_pair(ex2(suffix + (suffix_rest + g0)), ex2(suffix + (suffix_rest + g1)));
+            add_kept(suffix, suffix_rest, all);
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar_gate[n & 3]);
         }

@@ -1,8 +1,11 @@
-"""fp32 states of linear attention's prompts against 64 bits, heads that forget slowly."""
+"""fp32 states of linear attention's prompts against 64 bits, heads that forget slowly, and chunks that forget all."""
+import math
+
 import pytest
 import torch
 
 import h100_gdn_cuda_b200 as gdn
+from oracle import gdn_oracle as O
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +48,28 @@ def test_slow_decays(heads):
         ref = (v[0, :, h].double() * torch.exp(g[h].double() * ages)[:, None]).T @ k[0, :, 0].double() + torch.exp(g[h].double() * T) * s0[0, h].double()
         memory = min(T, -1 / g[h].item())
         assert (s[0, h].double() - ref).norm() <= (2.0 ** -15 + memory / 8 * 2.0 ** -23) * ref.norm()
+
+
+@pytest.mark.parametrize("gates", ["strong", "resets", "lowest"])
+@pytest.mark.parametrize("shape", [(2, 327, 1, 3, 128, 128), (2, 1000, 2, 4, 64, 64), (1, 2000, 2, 4, 128, 64)], ids=str)
+def test_decays_that_forget_all(shape, gates):
+    """Chunks that forget by more than 2^-120, with decays as fused_gdn_gating makes them, with a token in three that resets, and with the type's lowest
+    value in every other: what is left of a decay where it matters is a sum of few and small numbers, so that only the values' two parts count,
+    2^-16, and 9 half steps of R 2^-R <= 0.53, R being the decay's log2: 2^-21.  As above a part of the norm, of each head."""
+    B, T, kh, vh, dk, dv = shape
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = normal(gen, B, T, kh, dk).bfloat16(), normal(gen, B, T, kh, dk).bfloat16(), normal(gen, B, T, vh, dv).bfloat16()
+    s0 = normal(gen, B, vh, dv, dk)
+    if gates == "strong":
+        g = -(1 + 15 * torch.rand(vh, generator=gen, device="cuda")) * torch.nn.functional.softplus(normal(gen, B, T, vh))
+        g[..., 0] *= 0.3
+    else:
+        g = -0.02 * torch.rand(B, T, vh, generator=gen, device="cuda")
+        if gates == "resets":
+            g[:, 1:-40:3] = -math.inf
+        else:
+            g[:, 1:-20:2] = torch.finfo(torch.float32).min
+    _, s = gdn.linear_attention_chunked(q, k, v, g, None, s0)
+    _, ref = O.linear_attention_ref(q, k, v, g, dk ** -0.5, s0)
+    err = (s.double() - ref).flatten(2).norm(dim=-1) / ref.flatten(2).norm(dim=-1)
+    assert bool((err <= 2.0 ** -16 + 2.0 ** -21).all()), err
