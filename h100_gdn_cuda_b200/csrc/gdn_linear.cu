@@ -214,6 +214,9 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     if (int rc = check_scalar(a->gate, "gate", false)) return rc;
     if (int rc = check_state(a->initial_state, "initial_state")) return rc;
     if (int rc = check_state(a->final_state, "final_state")) return rc;
+    const bool in_place = a->initial_state.ptr && a->initial_state.ptr == a->final_state.ptr;
+    GDN_REQUIRE(!in_place || (a->initial_state.stride_seq == a->final_state.stride_seq && a->initial_state.stride_head == a->final_state.stride_head),
+                "gdn_linear_chunked: final_state may be initial_state only with the same strides");
     GDN_REQUIRE(tokens < (1ll << 31) - kChunk, "gdn_linear_chunked: too many tokens");
     DeviceInfo* d = nullptr;
     if (int rc = get_device_info(&d)) return rc;
@@ -241,6 +244,7 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
             return fail(GDN_ERR_WORKSPACE, "gdn_linear_chunked: workspace of %zu bytes (256-byte aligned) required, got %zu", plan.bytes, a->workspace_bytes);
         p.seg_state = static_cast<float*>(a->workspace);
         p.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + plan.states);
+        p.in_place = in_place;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->state_dtype == GDN_F32 ? launch_linear_shape<true>(*a, p, plan.cut_chains, st) : launch_linear_shape<false>(*a, p, plan.cut_chains, st);

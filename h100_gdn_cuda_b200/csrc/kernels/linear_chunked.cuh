@@ -62,6 +62,9 @@ struct LinChunkedParams {
     int whole, seg_chunks, num_segments, num_items, by_length;
     float* seg_state;  // per item behind `whole`: what the segment adds to the state (gdn_linear_segment_kernel), then the state behind it
     float* seg_decay;  // and its sum of log2-decays
+    // state_out is state_in: a cut chain's last segment may write it before the first one has read it, which so finds it in the place of
+    // the last one, where nothing is added (gdn_linear_combine_kernel puts it there)
+    int in_place;
 };
 
 // Decays are handled as powers of two; anything below 2^-160 is zero in fp32, and sums of 64 such stay exact enough to tell G_i - G_j
@@ -74,7 +77,7 @@ __device__ __forceinline__ float lin_gate_log2(float g) {
 struct alignas(16) LinItem {
     int seq, head, khead, dvt;
     int batch, segment, segments, mine;  // mine: the item's place among the segments' states (packed, padded behind `whole`)
-    int before, tok0, tokens, chunks;    // before: that of the segment in front; tokens of the segment; chunks < 0: no more items
+    int before, tok0, tokens, chunks;    // before: where the state that enters the segment is, -1: state_in; tokens of the segment; chunks < 0: no more items
 };
 
 constexpr int kLinRankedSeqs = 32;  // packed sequences that are ordered by length, a lane each
@@ -91,12 +94,14 @@ struct LinWalker {
         o.segments = 1;
         if (!p.cu_seqlens) {
             o.mine = it - p.whole;
-            o.before = o.mine - 1;
+            o.before = -1;
             if (o.mine >= 0) {
                 const int r = o.mine / p.num_segments;
                 chain = p.whole + r;
                 o.segment = o.mine - r * p.num_segments;
                 o.segments = p.num_segments;
+                if (o.segment > 0) o.before = o.mine - 1;
+                else if (p.in_place) o.before = o.mine + o.segments - 1;
             }
             o.seq = chain / per;
             o.batch = o.seq;
@@ -104,7 +109,7 @@ struct LinWalker {
             const int lane = threadIdx.x & 31, slot = it / per;
             o.batch = 0;
             o.mine = it;
-            o.before = it - per;
+            o.before = -1;
             auto offset = [&](int s) { return min(max(p.cu_seqlens[s], 0), p.total_tokens); };
             if (p.by_length) {
                 if (slot >= p.num_seqs) return false;
@@ -149,6 +154,8 @@ struct LinWalker {
                     o.segment = slot - first - (__shfl_sync(0xffffffffu, incl, mine) - o.segments);
                     bos = __shfl_sync(0xffffffffu, b, mine);
                     len = __shfl_sync(0xffffffffu, e, mine) - bos;
+                    if (o.segment > 0) o.before = it - per;
+                    else if (p.in_place && o.segments > 1 && slot + o.segments <= p.num_items / per) o.before = it + (o.segments - 1) * per;
                     break;
                 }
             }
@@ -360,7 +367,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
             for (int q = 0; q < kCols; q += 16) {
                 uint32_t r[16];
                 const int cols = row_in ? p.dk - c0 - q : 0;  // columns that are there from this one on
-                if (it.segment > 0) {
+                if (it.before >= 0) {
                     const uint4* src = reinterpret_cast<const uint4*>(p.seg_state + static_cast<long long>(it.before) * (128 * DK) + (32 * lq + lane) * DK + c0 + q);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(r + 4 * e) = __ldcg(src + e);

@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
     ptx::grid_dep_launch();
     const int per = p.vh * p.dv_tiles, chain = p.whole + blockIdx.x, seq = chain / per, rest = chain % per, head = rest / p.dv_tiles, dvt = rest % p.dv_tiles;
     int place = blockIdx.x * p.num_segments, stride = 1, n = p.num_segments - 1;  // of the chain's first segment; from one to the next
+    bool keep = p.in_place != 0;
     if (p.cu_seqlens) {
         if (threadIdx.x < 32) {  // the segments of the sequences in front
             int mine = 0;
@@ -248,6 +249,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
         place = first_slot * per + rest;
         stride = per;
         n = min(segments - 1, p.num_items / per - first_slot);  // (offsets that are not in order may ask for more slots than there are)
+        keep = keep && first_slot + segments <= p.num_items / per;
     }
     if (n <= 0) return;
     const int at = (blockIdx.y * kLinCombineThreads + threadIdx.x) * 4, row = at / dk_tile, col = at % dk_tile;
@@ -265,6 +267,7 @@ __global__ void __launch_bounds__(kLinCombineThreads) gdn_linear_combine_kernel(
     const long long step = static_cast<long long>(stride) * 128 * dk_tile;
     float* from = p.seg_state + static_cast<long long>(place) * 128 * dk_tile + at;
     const float* decay = p.seg_decay + place;
+    if (keep) *reinterpret_cast<float4*>(from + n * step) = s;
     constexpr int kAhead = 8;
     float4 d[kAhead];
     float g[kAhead];
