@@ -184,9 +184,10 @@ struct LinSmem {
     static constexpr int kOffQ = kOffV + kStages * kTileV;
     static constexpr int kOffP = kOffQ + kStagesQ * kTileQ;  // scores, 64 x 64
     // 4 x gate factors, fp32: of the scores [64]; of the output [64]; not plain: G[64] (log2), e^{G_i}[64]; of the state in front of its copy
-    // and behind it; 2^c behind the chunk; plain or not; of the values [64] (see factor_pair)
+    // and behind it; 2^c behind the chunk; plain or not; of the values [64] (see factor_pair).  Beside them, from the value warps: whether any of 32 columns
+    // has a value that is not finite [4]; the first token of it in each column [128], a byte each
     static constexpr int kOffGate = kOffP + 8192;
-    static constexpr int kGateStride = (5 * 64 + 4) * 4;
+    static constexpr int kGateOdd = 5 * 64 + 4, kGateStride = (kGateOdd + 4) * 4 + 128;
     static constexpr int kOffBar = kOffGate + 4 * kGateStride;
     static constexpr int kBytes = kOffBar + 640 + 1024;
 };
@@ -482,6 +483,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 mbar_wait_short(&bar_o[gc & 1], (gc >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
+                const bool odd = (DV == 128 || lq < 2) && gate_buf(gc)[L::kGateOdd + lq] != 0.f;
 #pragma unroll 1
                 for (int i = 0; i < 4; ++i) {  // 16 rows, 32 tokens
                     const int h = i & 1, b = i >> 1;
@@ -493,6 +495,14 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) w[j] = pack2(mul2(gv[j >> 1], pk(r[2 * j], r[2 * j + 1])));
+                    if (__builtin_expect(odd, 0)) {  // NaN from the first token on whose value is not finite
+                        const uint8_t* const first = reinterpret_cast<const uint8_t*>(gate_buf(gc) + L::kGateOdd + 4) + 32 * lq + 16 * h + (lane >> 2);
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int t = 32 * b + 8 * (j >> 1) + 2 * (lane & 3), f = first[8 * (j & 1)];
+                            w[j] |= (t >= f ? 0x7FFFu : 0u) | (t + 1 >= f ? 0x7FFF0000u : 0u);
+                        }
+                    }
                     if (DV == 128 || lq < 2) {
                         const uint32_t so = sOa + (h ? osw1 : osw0) + 4096 * b;
                         stmatrix_x4_trans(so, w[0], w[1], w[2], w[3]);
@@ -619,12 +629,16 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                 const int n = min(it.tokens - c * kChunk, kChunk);
                 const uint32_t s = gc % kStages;
                 uint8_t *tk = smem + s * L::kTileK, *tv = smem + L::kOffV + s * L::kTileV;
-                const float* gb = gate_buf(gc);
+                const float* const gb = gate_buf(gc);
                 mbar_wait_short(&bar_gate[gc & 3], (gc >> 2) & 1, abort_flag);
                 if (gc > 1) mbar_wait_short(&bar_d[gc & 1], ((gc >> 1) + 1) & 1, abort_flag);  // the values of two chunks before have been read
                 mbar_wait_short(&bar_full[s], (gc / kStages) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t sV = smem_u32(tv);
+                // What rounding leaves of a value that is not finite is a NaN, and so are sums of products with it (others only where they overflow, which
+                // a look at the values tells apart).
+                __nv_bfloat162 nan[2];
+                nan[0] = nan[1] = __float2bfloat162_rn(0.f);
                 if (DV == 128 || lq < 2) {
 #pragma unroll 1
                     for (int hf = 0; hf < 2; ++hf) {  // 32 tokens
@@ -656,6 +670,8 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                             for (int a = 0; a < 2; ++a) {
                                 times_factors(v[0][i >> 1][2 * (i & 1) + a], u[0][i >> 1][2 * (i & 1) + a], f);
                                 times_factors(v[1][i >> 1][2 * (i & 1) + a], u[1][i >> 1][2 * (i & 1) + a], f);
+                                nan[a] = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&u[0][i >> 1][2 * (i & 1) + a]),
+                                                 *reinterpret_cast<const __nv_bfloat162*>(&u[1][i >> 1][2 * (i & 1) + a]), nan[a]);
                             }
                         }
                         tmem_st_frag16(to + kTmVlo, u[0][0]);
@@ -663,6 +679,24 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                         tmem_st_frag16(to + kTmV, v[0][0]);
                         tmem_st_frag16(to + kTmV + (16u << 16), v[1][0]);
                     }
+                }
+                nan[0] = __hadd2(nan[0], nan[1]);
+                if (__builtin_expect(__any_sync(0xffffffffu, !__hbeq2(nan[0], nan[0])), 0)) {
+                    // The state takes such values as they are.  For the output a zero score would still make a NaN of them in the tokens in front: they are
+                    // taken out, and the output warps write NaN from the first one on.  (A lane has a column.)
+                    uint8_t* const at = tv + (lq >> 1) * 8192 + (lane & 7) * 2;
+                    int first = kChunk;
+#pragma unroll 1
+                    for (int t = n - 1; t >= 0; --t) {
+                        unsigned short* const x = reinterpret_cast<unsigned short*>(at + t * 128 + (((4 * (lq & 1) + (lane >> 3)) ^ (t & 7)) << 4));
+                        if ((*x & 0x7F80) == 0x7F80) {
+                            first = t;
+                            *x = 0;
+                        }
+                    }
+                    reinterpret_cast<uint8_t*>(gate_buf(gc) + L::kGateOdd + 4)[32 * lq + lane] = static_cast<uint8_t>(first);
+                    if (lane == 0) gate_buf(gc)[L::kGateOdd + lq] = 1.f;
+                    fence_proxy_async_smem();
                 }
                 if (__builtin_expect(packed && n < kChunk, 0)) {  // zero scores and values meet what the next sequence has there, but zero times its NaN is one
 #pragma unroll 1
@@ -848,6 +882,7 @@ __global__ void __launch_bounds__(lin::kThreads, 1)
                     gb2[96 + lane] = make_float2(ex2(g0), ex2(g1));
                 }
                 if (lane == 0) *reinterpret_cast<float4*>(gb + 256) = make_float4(before, behind, ex2(expo + expo_rest), plain ? 1.f : 0.f);
+                if (lane == 1) *reinterpret_cast<float4*>(gb + L::kGateOdd) = make_float4(0.f, 0.f, 0.f, 0.f);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bar_gate[gc & 3]);
             }
