@@ -59,21 +59,26 @@ const std::string& cuda_home() { return g_cuda_home; }
 using namespace gdn;
 
 // ------------------------------------------------------------------ self-test of the bounded waits
-// One warp waits, with the given cycle limit, on an mbarrier that nothing ever arrives on.  The
-// wait gives up, the kernel records status 7 and returns: the same path a product kernel takes
-// when a copy or an MMA never completes, exercised without any fault.
+// Two warps wait on mbarriers that nothing ever arrives on, one with the given cycle limit, one with a limit of polls.  Both waits give up, the kernel
+// records status 7 (8: one of them came back without having given up) and returns: the same path a product kernel takes when a copy or an MMA
+// never completes, exercised without any fault.
+constexpr uint32_t kSelftestPolls = 1000;
 __global__ void gdn_selftest_wait_kernel(long long limit_cycles, int* status) {
-    __shared__ uint64_t bar;
-    __shared__ int abort_flag;
+    __shared__ uint64_t bars[2];
+    __shared__ int abort_flags[2];
+    const int warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
-        abort_flag = 0;
-        ptx::mbar_init(&bar, 1);
+        for (int i = 0; i < 2; ++i) {
+            abort_flags[i] = 0;
+            ptx::mbar_init(&bars[i], 1);
+        }
         ptx::mbar_fence_init();
     }
     __syncthreads();
-    const bool ok = ptx::mbar_wait_limit(&bar, 0, &abort_flag, limit_cycles);
+    if (warp == 0) ptx::mbar_wait_limit(&bars[0], 0, &abort_flags[0], limit_cycles);
+    else ptx::mbar_wait_short<kSelftestPolls>(&bars[1], 0, &abort_flags[1]);
     __syncthreads();
-    if (threadIdx.x == 0 && (!ok || abort_flag) && status) atomicExch(status, 7);
+    if (threadIdx.x == 0 && status) atomicExch(status, abort_flags[0] && abort_flags[1] ? 7 : 8);
 }
 
 // ------------------------------------------------------------------ recurrent
@@ -311,7 +316,7 @@ int gdn_selftest_bounded_wait(int64_t limit_cycles, gdn_stream_t stream) {
                 "gdn_selftest_bounded_wait: limit must be between 1 and 1e9 cycles (got %lld)", (long long)limit_cycles);
     DeviceInfo* d = nullptr;
     if (int rc = get_device_info(&d)) return rc;
-    gdn_selftest_wait_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(limit_cycles, d->status);
+    gdn_selftest_wait_kernel<<<1, 64, 0, static_cast<cudaStream_t>(stream)>>>(limit_cycles, d->status);
     GDN_CUDA(cudaGetLastError());
     return GDN_OK;
 }

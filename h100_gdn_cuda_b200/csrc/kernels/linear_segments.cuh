@@ -218,7 +218,10 @@ __global__ void __launch_bounds__(lin::kSegThreads, 2)
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tmem, 256);
-    if (tid == 0 && *abort_flag && p.status) atomicExch(p.status, 4);
+    if (tid == 0 && *abort_flag) {
+        p.seg_decay[it.mine] = __int_as_float(0x7FFFFFFF);  // what is made of it is a NaN, not a guess
+        if (p.status) atomicExch(p.status, 4);
+    }
 }
 
 // The states behind the segments, in the place of what the segments add: one CTA per (sequence, v-head, 128 columns of dv) and part of the

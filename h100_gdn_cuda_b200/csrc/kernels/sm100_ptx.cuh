@@ -99,11 +99,13 @@ GDN_DEVICE bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_fl
 }
 
 // The same in as few instructions as there can be, for kernels of many roles, whose code does not fit the instruction cache otherwise.  The hardware
-// is asked to keep the warp suspended for up to 4 us a poll; the limit is a number of polls, four seconds where they last that long.
+// is asked to keep the warp suspended for up to 4 us a poll; the limit is a number of polls, four seconds (a poll of a barrier
+// that nothing completes takes 4.04 us).
+template <uint32_t kPolls = 1048576>
 GDN_DEVICE void mbar_wait_short(uint64_t* bar, uint32_t parity, const int* abort_flag) {
     asm volatile(
         "{\n\t.reg .pred P;\n\t.reg .u32 left, given_up;\n\t"
-        "mov.u32 left, 1048576;\n"
+        "mov.u32 left, %3;\n"
         "WAIT:\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 P, [%0], %1, 4000;\n\t"
         "@P bra DONE;\n\t"
@@ -115,7 +117,7 @@ GDN_DEVICE void mbar_wait_short(uint64_t* bar, uint32_t parity, const int* abort
         "@P bra WAIT;\n\t"
         "st.volatile.shared.u32 [%2], 1;\n"
         "DONE:\n\t}\n" ::"r"(smem_u32(bar)),
-        "r"(parity), "r"(smem_u32(abort_flag))
+        "r"(parity), "r"(smem_u32(abort_flag)), "n"(kPolls)
         : "memory");
 }
 

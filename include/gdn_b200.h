@@ -105,14 +105,17 @@ int gdn_version(void);
 int gdn_device_status(int device, int* status_out);
 
 /* Self-test of the bounded waits every kernel of this library uses (no counterpart in the
- * reference, whose waits spin without a limit, kernels/common/sm90_utils.cuh): launches one warp
- * that waits on a barrier nothing will ever complete, with a limit of `limit_cycles` SM clock
- * cycles (1 .. 1e9).  The wait gives up, the kernel sets the device status word to 7 and returns;
- * gdn_device_status() then reads 7 and the context stays usable.  Status codes of the product
- * kernels: 1 recurrent, 2 WY/UT and chunk-parallel stage, 4 state/output stage, 6 other prefill
- * stages.  A kernel whose wait gave up writes none of its outputs where that is cheap to arrange
- * (recurrent, whole-layer prefill); the entry point has long returned GDN_OK by then, so the
- * status word, not a return code, is how GDN_ERR_DEVICE conditions are observed. */
+ * reference, whose waits spin without a limit, kernels/common/sm90_utils.cuh): launches two warps
+ * that wait on barriers nothing will ever complete, one with a limit of `limit_cycles` SM clock
+ * cycles (1 .. 1e9), one with a limit of 1000 polls.  Both waits give up, the kernel sets the device
+ * status word to 7 (8 if one of them came back without having given up) and returns;
+ * gdn_device_status() then reads it and the context stays usable.  Status codes of the product
+ * kernels: 1 recurrent, 2 WY/UT and chunk-parallel stage, 4 state/output stage and linear attention's
+ * prompts, 6 other prefill stages.  A kernel whose wait gave up writes none of its outputs where that is
+ * cheap to arrange (recurrent, whole-layer prefill); persistent kernels (linear attention's prompts) have
+ * written what they were through with, and states joined from segments that gave up are NaN.  The entry
+ * point has long returned GDN_OK by then, so the status word, not a return code, is how GDN_ERR_DEVICE
+ * conditions are observed. */
 int gdn_selftest_bounded_wait(int64_t limit_cycles, gdn_stream_t stream);
 
 /* Replaces Compiler::build (csrc/jit/compiler.hpp:82-103): compiles `source`, a complete CUDA
