@@ -25,6 +25,13 @@ int check_linear_shape(const GdnShape& s, const char* who) {
     return GDN_OK;
 }
 
+// One memory for the state that is read and the one that is written: a block of it is then the same (sequence, head) of both.
+int check_in_place(const GdnState& in, const GdnState& out, const GdnShape& s, bool several, const char* who) {
+    GDN_REQUIRE(!in.ptr || in.ptr != out.ptr || ((!several || in.stride_seq == out.stride_seq) && (s.num_v_heads == 1 || in.stride_head == out.stride_head)),
+                "%s: the state may be updated in place only with the same strides", who);
+    return GDN_OK;
+}
+
 template <bool kF32>
 int launch_linear_recurrent(const LinRecurrentParams& p, cudaStream_t st) {
     const long long grid = static_cast<long long>(p.batch) * p.vh * ((p.dv + kLinRows - 1) / kLinRows);
@@ -164,6 +171,7 @@ int gdn_linear_recurrent(const GdnLinearRecurrentArgs* a, gdn_stream_t stream) {
     GDN_REQUIRE(!(a->store_step_state && !a->state_out.ptr), "gdn_linear_recurrent: step states need state_out");
     GDN_REQUIRE(!(a->store_step_state && a->state_in.ptr && a->state_in.ptr == a->state_out.ptr),
                 "gdn_linear_recurrent: state_out may not alias state_in when step states are stored");
+    if (int rc = check_in_place(a->state_in, a->state_out, s, s.batch > 1 || a->state_indices, "gdn_linear_recurrent")) return rc;
     GDN_REQUIRE(!(a->state_indices && a->store_step_state), "gdn_linear_recurrent: state_indices cannot be combined with step states");
     GDN_REQUIRE(!a->state_indices || (a->state_in.ptr && a->num_slots > 0), "gdn_linear_recurrent: state_indices needs a state_in pool of num_slots slots");
     DeviceInfo* d = nullptr;
@@ -214,9 +222,7 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
     if (int rc = check_scalar(a->gate, "gate", false)) return rc;
     if (int rc = check_state(a->initial_state, "initial_state")) return rc;
     if (int rc = check_state(a->final_state, "final_state")) return rc;
-    const bool in_place = a->initial_state.ptr && a->initial_state.ptr == a->final_state.ptr;
-    GDN_REQUIRE(!in_place || (a->initial_state.stride_seq == a->final_state.stride_seq && a->initial_state.stride_head == a->final_state.stride_head),
-                "gdn_linear_chunked: final_state may be initial_state only with the same strides");
+    if (int rc = check_in_place(a->initial_state, a->final_state, s, s.batch > 1, "gdn_linear_chunked")) return rc;
     GDN_REQUIRE(tokens < (1ll << 31) - kChunk, "gdn_linear_chunked: too many tokens");
     DeviceInfo* d = nullptr;
     if (int rc = get_device_info(&d)) return rc;
@@ -244,7 +250,7 @@ int gdn_linear_chunked(const GdnLinearChunkedArgs* a, gdn_stream_t stream) {
             return fail(GDN_ERR_WORKSPACE, "gdn_linear_chunked: workspace of %zu bytes (256-byte aligned) required, got %zu", plan.bytes, a->workspace_bytes);
         p.seg_state = static_cast<float*>(a->workspace);
         p.seg_decay = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + plan.states);
-        p.in_place = in_place;
+        p.in_place = a->initial_state.ptr && a->initial_state.ptr == a->final_state.ptr;
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->state_dtype == GDN_F32 ? launch_linear_shape<true>(*a, p, plan.cut_chains, st) : launch_linear_shape<false>(*a, p, plan.cut_chains, st);

@@ -397,7 +397,7 @@ int gdn_group_norm(const GdnGroupNormArgs* args, gdn_stream_t stream);
  *
  * gdn_linear_recurrent: token by token, for decode, draft runs and short prompts; dk a multiple of 8 up to 256, dv a multiple of 8.
  * num_accepted_tokens, store_step_state and state_indices as in gdn_recurrent_forward; a slot outside [0, num_slots) is a padding sequence as
- * well, and the slots of a call have to differ.  state_out may be state_in; it may be NULL where no state is wanted. */
+ * well, and the slots of a call have to differ.  state_out may be state_in (same strides); it may be NULL where no state is wanted. */
 typedef struct {
     GdnShape shape;
     GdnTokenTensor q, k, v, out;
