@@ -143,7 +143,7 @@ int launch_linear_chunked(const GdnLinearChunkedArgs& a, const LinChunkedParams&
 template <bool kF32>
 int launch_linear_shape(const GdnLinearChunkedArgs& a, const LinChunkedParams& p, long long cut_chains, cudaStream_t st) {
     // (a single column block needs no rank 5: its map clips what is missing)
-    const bool whole = (p.dk <= 64 || p.dk == 128) && (p.dv <= 64 || p.dv % 128 == 0);
+    const bool whole = p.dk == 128 && p.dv % 128 == 0;
     if (p.dk <= 64 && p.dv <= 64) return launch_linear_chunked<64, 64, false, kF32>(a, p, cut_chains, st);
     if (p.dk <= 64) return launch_linear_chunked<64, 128, false, kF32>(a, p, cut_chains, st);
     if (p.dv <= 64) return launch_linear_chunked<128, 64, false, kF32>(a, p, cut_chains, st);
