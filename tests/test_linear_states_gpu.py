@@ -73,3 +73,21 @@ def test_decays_that_forget_all(shape, gates):
     _, ref = O.linear_attention_ref(q, k, v, g, dk ** -0.5, s0)
     err = (s.double() - ref).flatten(2).norm(dim=-1) / ref.flatten(2).norm(dim=-1)
     assert bool((err <= 2.0 ** -16 + 2.0 ** -21).all()), err
+
+
+@pytest.mark.parametrize("gate", ["head", "token", "none"])
+@pytest.mark.parametrize("shape", [(2, 1, 1, 1, 128, 128), (1, 65, 2, 4, 8, 16), (2, 257, 2, 2, 96, 200), (1, 130, 1, 2, 104, 40), (1, 1000, 1, 2, 128, 128), (1, 3000, 1, 1, 64, 64)], ids=str)
+def test_every_value(shape, gate):
+    """Value by value, against the same sum of absolute values R: two parts of the values and decays as above, each 2^-16 at most, the tensor cores' sums as above, fp32
+    states at the end."""
+    B, T, kh, vh, dk, dv = shape
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = normal(gen, B, T, kh, dk).bfloat16(), normal(gen, B, T, kh, dk).bfloat16(), normal(gen, B, T, vh, dv).bfloat16()
+    s0 = normal(gen, B, vh, dv, dk)
+    g = {"head": -0.3 * torch.rand(vh, generator=gen, device="cuda"), "token": -torch.nn.functional.softplus(normal(gen, B, T, vh)), "none": None}[gate]
+    _, s = gdn.linear_attention_chunked(q, k, v, g, None, s0)
+    _, ref = O.linear_attention_ref(q, k, v, g, 1.0, s0)
+    _, size = O.linear_attention_ref(q.abs(), k.abs(), v.abs(), g, 1.0, s0.abs())
+    err = (s.double() - ref).abs()
+    tol = (2.0 ** -15 + T / 8 * 2.0 ** -23) * size + 2.0 ** -24 * ref.abs()
+    assert bool((err <= tol).all()), (err / tol).max().item()
