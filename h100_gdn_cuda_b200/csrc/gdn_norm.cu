@@ -9,24 +9,32 @@ using namespace gdn;
 
 namespace {
 
-// How a long sample is cut: channels of a block (whole groups, up to 256 vectors), rows of a part.
+// How a long sample is cut: channels of a block (whole groups, up to 256 vectors), rows of a part.  Groups of more than 256 vectors are `split` pieces,
+// which are the groups of all that follows.
 struct NormPlan {
-    int block_channels, blocks, part_rows, parts;  // block_channels == 0: the groups are too wide for it
+    int block_channels, blocks, part_rows, parts, split;
 };
 
 NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int vec, int size) {
-    const int width = channels / groups;
+    int width = channels / groups;
     NormPlan plan{};
+    plan.split = 1;
+    if (width > kNormThreads * vec) {  // (whole vectors: see widest())
+        int vecs = kNormThreads;
+        while (width / vec % vecs != 0) --vecs;
+        plan.split = width / vec / vecs;
+        groups *= plan.split;
+        width = vecs * vec;
+    }
     int unit = 1;  // groups of a block come in multiples that are whole vectors
     while (unit * width % vec != 0) ++unit;
-    if (unit * width > kNormThreads * vec) return plan;
     const int per = std::min(kNormThreads * vec / (unit * width), kNormMaxGroups / unit) * unit;
     // blocks of about the same number of groups
     const int units = (groups + unit - 1) / unit, blocks = (groups + per - 1) / per;
     plan.block_channels = std::min((units + blocks - 1) / blocks * unit * width, channels);
     plan.blocks = (channels + plan.block_channels - 1) / plan.block_channels;
     const int vecs = plan.block_channels / vec, rstep = kNormThreads / vecs;
-    // three CTAs an SM, as far as rows go round; no more than the part's shared memory holds, no fewer than a few rows a thread
+    // three parts an SM, as far as rows go round; no more than the part's shared memory holds, no fewer than a few rows a thread
     const int64_t most = static_cast<int64_t>(kNormPartBytes / (kNormThreads * vec * size)) * rstep;
     const int64_t want = std::max<int64_t>(1, 3 * 148 / std::max<int64_t>(1, samples * plan.blocks));
     int64_t part = std::max<int64_t>((rows + want - 1) / want, 4 * rstep);
@@ -88,15 +96,7 @@ int launch_short(const GroupNormParams& p, cudaStream_t st) {
 constexpr long long kMostSamples = 65535;  // of a launch in parts
 
 template <typename T, int V>
-int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
-    if (plan.block_channels == 0) {
-        GDN_REQUIRE(p.n * p.groups < (1ll << 31), "gdn_group_norm: too many samples");
-        GDN_CUDA(launch_dependent(gdn_group_norm_wide_kernel<T, V>, dim3(static_cast<unsigned>(p.n * p.groups)), kNormThreads, 0, st, p));
-        return GDN_OK;
-    }
-    p.part_rows = plan.part_rows;
-    p.parts = plan.parts;
-    p.block_channels = plan.block_channels;
+int launch_parts(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     GDN_REQUIRE(plan.blocks <= kMostSamples, "gdn_group_norm: too many channels");
     if (p.n > kMostSamples) {  // a grid's limit: in turn, with the same workspace
         for (long long first = 0; first < p.n; first += kMostSamples) {
@@ -105,10 +105,17 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
             q.x = static_cast<const T*>(p.x) + first * p.x_sn;
             q.y = static_cast<T*>(p.y) + first * p.y_sn;
             if (p.z) q.z = static_cast<const T*>(p.z) + first * p.z_sn;
-            if (int rc = launch_long<T, V>(q, plan, st)) return rc;
+            if (int rc = launch_parts<T, V>(q, plan, st)) return rc;
         }
         return GDN_OK;
     }
+    const int whole = p.groups;
+    p.part_rows = plan.part_rows;
+    p.parts = plan.parts;
+    p.block_channels = plan.block_channels;
+    p.split = plan.split;
+    p.groups *= plan.split;
+    p.width /= plan.split;
     const dim3 grid(static_cast<unsigned>(plan.parts), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
     const int rstep = kNormThreads / (plan.block_channels / V), smem = (plan.part_rows + rstep - 1) / rstep * kNormThreads * V * static_cast<int>(sizeof(T));
     if (int rc = set_smem<gdn_group_norm_stats_kernel<T, V>>(kNormPartBytes)) return rc;
@@ -116,11 +123,11 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     p.join = p.partial;
     p.join_rows = p.part_rows;
     p.join_parts = p.parts;
-    if (p.parts > kNormJoinParts) {
+    if (p.parts > kNormJoinParts || p.split > 1) {
         p.join = p.partial + static_cast<size_t>(p.n) * p.parts * p.groups;
         p.join_rows = p.l;
         p.join_parts = 1;
-        const long long blocks = (p.n * p.groups + 7) / 8;
+        const long long blocks = (p.n * whole + 7) / 8;
         GDN_REQUIRE(blocks < (1ll << 31), "gdn_group_norm: too many samples");
         GDN_CUDA(launch_dependent(gdn_group_norm_join_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, p));
     }
@@ -130,6 +137,23 @@ int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     const dim3 apply(static_cast<unsigned>((p.l + p.apply_rows - 1) / p.apply_rows), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
     GDN_CUDA(launch_dependent(p.z ? gdn_group_norm_apply_kernel<T, V, true> : gdn_group_norm_apply_kernel<T, V, false>, apply, kNormThreads, 0, st, p));
     return GDN_OK;
+}
+
+// Groups that are too wide for a sweep: a CTA each in one launch where that takes it few sweeps (24 groups of 4 sweeps 9 : 18 us in pieces, of 16 24 : 17, of 64
+// 96 : 20) or where there are as many groups as CTAs fit the SMs (2500 of 16 sweeps 217 : 229, of 32 448 : 291, 4000 of 36 in pieces of 6 channels 175 : 635);
+// otherwise in pieces (one of 16384 36200 : 78, 300 of 64 163 : 71).
+bool wide_groups(long long count, int64_t rows, int width, int vec) {
+    return rows * ((width + kNormThreads * vec - 1) / (kNormThreads * vec)) <= 12 || count >= 8 * 148;
+}
+
+template <typename T, int V>
+int launch_long(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
+    if (plan.split > 1 && wide_groups(p.n * p.groups, p.l, p.width, V)) {
+        GDN_REQUIRE(p.n * p.groups < (1ll << 31), "gdn_group_norm: too many samples");
+        GDN_CUDA(launch_dependent(gdn_group_norm_wide_kernel<T, V>, dim3(static_cast<unsigned>(p.n * p.groups)), kNormThreads, 0, st, p));
+        return GDN_OK;
+    }
+    return launch_parts<T, V>(p, plan, st);
 }
 
 // Shared memory of a CTA of `threads` that keeps a (sample, group); 0: it does not fit.
@@ -187,11 +211,14 @@ extern "C" {
 // An upper bound over the vector widths, which go by the type, pointers and strides.
 size_t gdn_group_norm_workspace_bytes(int64_t samples, int64_t rows, int32_t channels, int32_t groups) {
     if (samples <= 0 || rows <= 0 || groups <= 0 || channels <= 0 || channels % groups != 0 || short_groups(rows, channels / groups)) return 0;
-    size_t parts = 0;
+    size_t entries = 0;  // of a sample and group
     for (int size = 2; size <= 4; size *= 2)
         for (int v = 1; v * size <= 16; v *= 2)
-            if (channels % v == 0) parts = std::max<size_t>(parts, norm_plan(samples, rows, channels, groups, v, size).parts);
-    return parts == 0 ? 0 : (parts + 1) * static_cast<size_t>(samples) * groups * sizeof(float2);  // (one more: the parts joined)
+            if ((channels / groups > kNormThreads ? channels / groups : channels) % v == 0) {
+                const NormPlan plan = norm_plan(samples, rows, channels, groups, v, size);
+                entries = std::max(entries, static_cast<size_t>(plan.parts) * plan.split);
+            }
+    return (entries + 1) * static_cast<size_t>(samples) * groups * sizeof(float2);  // (one more: the parts joined)
 }
 
 int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {

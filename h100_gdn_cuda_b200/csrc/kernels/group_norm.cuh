@@ -26,6 +26,8 @@ struct GroupNormParams {
     // long samples: rows of a part, parts of a sample, channels of a block (whole groups); (mean, sum of squared distances) of every
     // (sample, part, group)
     int part_rows, parts, block_channels;
+    // groups of more channels than a CTA sweeps at once are `split` pieces each: `groups` and `width` are then the pieces'
+    int split;
     float2* partial;
     int apply_rows;  // rows of a CTA of the second launch
     // what that one joins: `join_parts` entries of `join_rows` rows each (the parts, or one of all rows where those are many)
@@ -267,7 +269,7 @@ __global__ void __launch_bounds__(256) gdn_group_norm_short_kernel(const GroupNo
 // share a sector: L2 joins them.  Large groups are bound by one SM's rate of copies and of SiLU's
 // exponentials, one after the other (640 channels, 4 x 4095 rows, 128 CTAs: 18 us, of which 6 are DRAM's).
 constexpr int kNormWholeBytes = 224 * 1024;
-constexpr int kNormPartBytes = 72 * 1024;  // three CTAs share an SM
+constexpr int kNormPartBytes = 72 * 1024;  // three CTAs share an SM (two of the long groups' first launch where its sums take 4 or 8 KB more)
 
 // the sum over a CTA of `kWarps` warps; everybody gets it
 template <int kWarps>
@@ -483,14 +485,15 @@ __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_stats_kernel(cons
     for (int g = t; g < groups; g += kNormThreads) out[g] = make_float2(mean[g] / count, sq[g]);
 }
 
-// Many parts: (mean, sum of squared distances) of whole groups, a warp for each (sample, group), in front of the parts' entries.
+// Many parts, or groups in pieces: (mean, sum of squared distances) of whole groups, a warp for each (sample, group), behind the parts' entries.
 __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNormParams p) {
     ptx::grid_dep_wait();
     ptx::grid_dep_launch();
     const long long unit = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (unit >= p.n * p.groups) return;
-    const float2* in = p.partial + unit / p.groups * p.parts * p.groups + unit % p.groups;
-    auto count = [&](int i) { return static_cast<float>(min(static_cast<long long>(p.part_rows), p.l - static_cast<long long>(i) * p.part_rows)); };
+    const int whole = p.groups / p.split, entries = p.parts * p.split;
+    if (unit >= p.n * whole) return;
+    const float2* in = p.partial + unit / whole * p.parts * p.groups + unit % whole * p.split;
+    auto count = [&](int i) { return static_cast<float>(min(static_cast<long long>(p.part_rows), p.l - static_cast<long long>(i / p.split) * p.part_rows)); };
     constexpr int kMine = 8;  // entries a lane has in flight, and keeps from the means to the distances where there are no more
     const int l = threadIdx.x & 31;
     float2 mine[kMine];
@@ -499,23 +502,23 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int i = i0 + l + 32 * j;
-            mine[j] = i < p.parts ? __ldcg(in + static_cast<long long>(i) * p.groups) : make_float2(0.f, 0.f);
+            mine[j] = i < entries ? __ldcg(in + static_cast<long long>(i / p.split) * p.groups + i % p.split) : make_float2(0.f, 0.f);
         }
     };
-    for (int i0 = 0; i0 < p.parts; i0 += 32 * kMine) {
+    for (int i0 = 0; i0 < entries; i0 += 32 * kMine) {
         fetch(i0);
 #pragma unroll
         for (int j = 0; j < kMine; ++j)
-            if (i0 + l + 32 * j < p.parts) sum += count(i0 + l + 32 * j) * mine[j].x;
+            if (i0 + l + 32 * j < entries) sum += count(i0 + l + 32 * j) * mine[j].x;
     }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    const float mu = sum / static_cast<float>(p.l);
-    for (int i0 = 0; i0 < p.parts; i0 += 32 * kMine) {
-        if (p.parts > 32 * kMine) fetch(i0);
+    const float mu = sum / (static_cast<float>(p.l) * static_cast<float>(p.split));
+    for (int i0 = 0; i0 < entries; i0 += 32 * kMine) {
+        if (entries > 32 * kMine) fetch(i0);
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
-            if (i0 + l + 32 * j < p.parts) {
+            if (i0 + l + 32 * j < entries) {
                 const float d = mine[j].x - mu;
                 q += mine[j].y + count(i0 + l + 32 * j) * static_cast<float>(p.width) * d * d;
             }
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
     }
     const int l = t & 7;
     for (int g = t >> 3; g < (groups + 31) / 32 * 32; g += kNormThreads / 8) {
-        const float2* in = p.join + n * p.join_parts * p.groups + c_first / p.width + g;
+        const float2* in = p.join + n * p.join_parts * (p.groups / p.split) + (c_first / p.width + g) / p.split;
         constexpr int kMine = kNormJoinParts / 8;
         float sum = 0.f, q = 0.f;
         auto count = [&](int i) { return static_cast<float>(min(p.join_rows, p.l - i * p.join_rows)); };
@@ -570,7 +573,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
         for (int m = 4; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
         if (l == 0 && g < groups) {
             mean[g] = mu;
-            rstd[g] = rsqrtf(q / (static_cast<float>(p.l) * static_cast<float>(p.width)) + p.eps);
+            rstd[g] = rsqrtf(q / (static_cast<float>(p.l) * static_cast<float>(p.width) * static_cast<float>(p.split)) + p.eps);
         }
     }
     __syncthreads();
@@ -619,7 +622,8 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
     }
 }
 
-// Groups of more channels than a CTA has room for in one sweep (width > 256 V): one CTA per (sample, group), in three passes over memory.
+// Groups of more channels than a CTA has room for in one sweep (width > 256 V), where there are enough of them: one CTA per (sample, group), in three passes
+// over memory.
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_wide_kernel(const GroupNormParams p) {
     __shared__ float part[8];
