@@ -165,13 +165,15 @@ int whole_bytes(int64_t rows, int width, int vec, int size, int threads) {
 }
 // One launch that reads x once is faster than two or three that read it twice (4 x 32 groups of 16 KB 8.5 -> 2.8 us, of 64 KB 18 -> 7,
 // of 150 KB 24 -> 14), except where
-//  - very many groups are so small that the CTAs' turn-over shows (65536 groups of 2 KB 99 -> 280 us), or
+//  - very many groups are so small that the CTAs' turn-over shows (65536 groups of 2 KB, 32 a sample, 99 -> 280 us, 8 a sample 187 -> 276; with few a
+//    sample the sums of a part are long instead: 4 378 -> 275, 2 915 -> 273, 1 2555 -> 272; of few rows they are not, 4 rows of 4 x 256 channels 307 -> 496), or
 //  - a group's piece of a row is not whole sectors of 32 bytes: copies of less than 16 bytes go through L1, of which the tile leaves little (20
 //    channels, bf16, 32 groups of 200 KB 21 -> 30 us, of 150 KB 20 -> 16), and where CTAs come in several waves, or read a gate as well, the
 //    sectors that groups share move twice (512 groups of 64 KB 33 -> 42 us, 256 of 40 KB 20 -> 14; gated, 512 of 48 KB 30 -> 42, of 16 KB 19 -> 11).
-bool whole_groups(int64_t count, int64_t rows, int width, int vec, int size, bool gated) {
+bool whole_groups(int64_t samples, int groups, int64_t rows, int width, int vec, int size, bool gated) {
     const int bytes = whole_bytes(rows, width, vec, size, 512);
-    if (bytes == 0 || (rows * width * size < 16 * 1024 && count > 2048)) return false;
+    const int64_t count = samples * groups;
+    if (bytes == 0 || (rows * width * size < 16 * 1024 && count > 2048 && (groups > 4 || rows < 32))) return false;
     return width * size % 32 == 0 || bytes <= (gated ? 24 : count > 148 ? 48 : 176) * 1024;
 }
 
@@ -262,7 +264,7 @@ int gdn_group_norm(const GdnGroupNormArgs* a, gdn_stream_t stream) {
         return v;
     };
     const int shared = widest(true);
-    const bool is_whole = !is_short && whole_groups(a->samples * a->groups, a->rows, p.width, shared, size, p.z != nullptr);
+    const bool is_whole = !is_short && whole_groups(a->samples, a->groups, a->rows, p.width, shared, size, p.z != nullptr);
     const int v = is_short || is_whole || p.width > kNormThreads ? shared : widest(false);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a->dtype == GDN_F32) {
