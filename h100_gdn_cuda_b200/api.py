@@ -764,8 +764,9 @@ def linear_attention_chunked(query, key, value, gate=None, scale: Optional[float
     The arguments are those of linear_attention_recurrent (packed inputs need cu_seqlens alone).  Returns (output, final_state), the
     final state in initial_state's dtype (bf16 without one).  Matrix products take bf16 operands: scores with their decay and the state
     that a chunk reads are rounded to bf16 there (and the queries that read it, in a chunk that forgets by more than 2^120).  The state itself
-    is kept in fp32 throughout; values with their decay go into it to 2^-16.  A NaN or an infinity in `value` makes its column of the output NaN from
-    its token on, and its row of the state.  Key dims above 128 go token by token.  No gradients."""
+    is kept in fp32 throughout; values with their decay go into it to 2^-16, and its sums are cut off rather than rounded, some 2e-9 of it for each token
+    that a head remembers.  Sizes from 2^-60 to 2^60.  A NaN or an infinity in `value` makes its column of the output NaN from its token on, and its row
+    of the state.  Key dims above 128 go token by token.  No gradients."""
     ext = _ext if _ext is not None else _load_ext()
     if ext:
         return ext._fast_linear_attention_chunked(query, key, value, gate, scale, initial_state, cu_seqlens)

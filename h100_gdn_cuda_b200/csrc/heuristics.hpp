@@ -230,7 +230,7 @@ inline int conv_tok_block(long long tokens, long long blocks_per_token_block, in
 
 // Linear attention, prompts: which of `chains` (sequence, v-head, dv tile) chains of `chunks` chunks each (packed: on average) are cut into how many
 // segments.  A chain alone takes about 1.02 us a chunk, 148 of them at once 1.2 (HBM-bound); cut ones 1.87, since K and V are read twice, and the
-// two launches more some 12 us.  Cut : whole, us, d=128: 8 chains of 2048 chunks (2 x 131072 tokens, 4 v-heads) 241 : 2102, 32 of 124 79 : 136,
+// two launches more some 12 us.  Cut : whole, us by events (calls of a few ms in all; minutes of load are some 15 % slower), d=128: 8 chains of 2048 chunks (2 x 131072 tokens, 4 v-heads) 241 : 2102, 32 of 124 79 : 136,
 // 32 of 32 36.4 : 41.7, 32 of 24 33.0 : 33.6, 8 of 24 26.5 : 33.0, 8 of 16 25.5 : 25.1 (whole), 8 of 10 26.3 : 19.0 (whole); 24 packed ones of 104 on average
 // 57 : 119.  Where more chains than SMs leave a last round that is not full, those of that round are cut (in no more segments than have 12
 // chunks each: an item has its own start): 160 of 52 113 : 130.

@@ -14,7 +14,8 @@
 // and its increment.
 // Roundings: scores, the copy of the state that Q meets, and Q where it is scaled are bf16, once each.  Values of the increment come in two parts, bf16
 // and what that leaves, by a second product: with one part fp32 states are 2.3e-3 off and with two 5e-6, outputs with bf16 states 2.8e-3 and 2.35e-3
-// (4 x 4096 tokens from DRAM 88 and 92 us, 2 x 131072 on 4 v-heads, back to back, 256 and 285).
+// (4 x 4096 tokens from DRAM 88 and 92 us, 2 x 131072 on 4 v-heads, back to back under the power cap, 256 and 285).  The tensor cores cut the state's sums off, eight a chunk: some 2e-9 of
+// it for each token that a head remembers (131072 tokens without a decay 2.7e-4).
 //
 // A persistent CTA takes work items (sequence segment, v-head, 128 columns of dv) one after the other; its roles run over the same
 // items and chunks, handing tiles on through mbarriers:
@@ -30,12 +31,12 @@
 // came; Q, K and the scores are B operands.
 // What bounds it: HBM allows 2750 cycles a chunk at d = 128 on all SMs (2080 where two v-heads share Q and K), shared memory 1600 (208 KB of
 // copies, operands and tiles), the tensor pipe 1150; a warp of each role needs 1000 to 1700 for its part, a few hundred instructions one behind the
-// other (4300 a chunk in all).  4 x 4096 tokens from DRAM: 92 us on 32 v-heads with 16 k-heads, 100 with 32, 148 heads of 4096 110; the same copies in
-// and out and nothing else take 69, 89 and 100.  From a chunk's copies to its end are 5300 cycles and more with all SMs at work, half of them the copies:
-// the ring has four stages, and a fifth tile for Q and the output (three stages: 95 us).
+// other.  None of that is the 2300 to 2550 that a chunk takes on 128 SMs: a chain alone on the GPU takes 2000, since S Q^T is issued behind the wait for
+// the scores, these wait for the output before to be through with their one tile, and the state's next copy waits for S Q^T.
+// 4 x 4096 tokens from DRAM: 91 us on 32 v-heads with 16 k-heads; the same copies in and out and nothing else take 69.  Where chunks forget by more than 2^-120, 116 to 125.
+// The ring has four stages, and a fifth tile for Q and the output (three stages: 95 us where four took 92).
 // The instruction cache counts: the waits are the short form, the item search is one warp's, the state's type is the kernel's (104 KB of code took 5200
-// cycles a chunk with both SMs of a pair at work, 2900 with one).  The form with decays in keys and scores throughout (240 KB of shared memory
-// a chunk, two accumulators) took 118 us where this takes 100 (4 x 4096 tokens, 32 v-heads, back to back).
+// cycles a chunk with both SMs of a pair at work, 2900 with one).
 #pragma once
 #include <cuda.h>
 

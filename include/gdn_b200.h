@@ -413,7 +413,7 @@ typedef struct {
 int gdn_linear_recurrent(const GdnLinearRecurrentArgs* args, gdn_stream_t stream);
 
 /* gdn_linear_chunked: whole prompts.  dk a multiple of 8 up to 128 (up to 256 on the kernel of gdn_linear_recurrent), dv a multiple of 8.  initial_state.ptr and final_state.ptr may be NULL;
- * final_state may be initial_state itself (same strides) but not overlap it otherwise.
+ * final_state may be initial_state itself (same strides) but not overlap it otherwise.  Sizes of values, states and outputs from 2^-60 to 2^60.
  * `workspace`: gdn_linear_chunked_workspace_bytes(&shape) bytes or more, 256-byte aligned. */
 typedef struct {
     GdnShape shape;
