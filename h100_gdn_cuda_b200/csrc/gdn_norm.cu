@@ -9,30 +9,29 @@ using namespace gdn;
 
 namespace {
 
-// How a long sample is cut: channels of a block (whole groups, up to 256 vectors), rows of a part.  Groups of more than 256 vectors are `split` pieces,
-// which are the groups of all that follows.
+// How a long sample is cut: channels of a block (whole groups, up to 256 vectors, or one of the `split` pieces of a group that is wider), rows of a part.
 struct NormPlan {
     int block_channels, blocks, part_rows, parts, split;
 };
 
 NormPlan norm_plan(int64_t samples, int64_t rows, int channels, int groups, int vec, int size) {
-    int width = channels / groups;
+    const int width = channels / groups;
     NormPlan plan{};
-    plan.split = 1;
     if (width > kNormThreads * vec) {  // (whole vectors: see widest())
-        int vecs = kNormThreads;
-        while (width / vec % vecs != 0) --vecs;
-        plan.split = width / vec / vecs;
-        groups *= plan.split;
-        width = vecs * vec;
+        const int most = (width / vec + kNormThreads - 1) / kNormThreads;
+        plan.block_channels = (width / vec + most - 1) / most * vec;
+        plan.split = (width + plan.block_channels - 1) / plan.block_channels;
+        plan.blocks = groups * plan.split;
+    } else {
+        int unit = 1;  // groups of a block come in multiples that are whole vectors
+        while (unit * width % vec != 0) ++unit;
+        const int per = std::min(kNormThreads * vec / (unit * width), kNormMaxGroups / unit) * unit;
+        // blocks of about the same number of groups
+        const int units = (groups + unit - 1) / unit, blocks = (groups + per - 1) / per;
+        plan.block_channels = std::min((units + blocks - 1) / blocks * unit * width, channels);
+        plan.split = 1;
+        plan.blocks = (channels + plan.block_channels - 1) / plan.block_channels;
     }
-    int unit = 1;  // groups of a block come in multiples that are whole vectors
-    while (unit * width % vec != 0) ++unit;
-    const int per = std::min(kNormThreads * vec / (unit * width), kNormMaxGroups / unit) * unit;
-    // blocks of about the same number of groups
-    const int units = (groups + unit - 1) / unit, blocks = (groups + per - 1) / per;
-    plan.block_channels = std::min((units + blocks - 1) / blocks * unit * width, channels);
-    plan.blocks = (channels + plan.block_channels - 1) / plan.block_channels;
     const int vecs = plan.block_channels / vec, rstep = kNormThreads / vecs;
     // three parts an SM, as far as rows go round; no more than the part's shared memory holds, no fewer than a few rows a thread
     const int64_t most = static_cast<int64_t>(kNormPartBytes / (kNormThreads * vec * size)) * rstep;
@@ -109,13 +108,10 @@ int launch_parts(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
         }
         return GDN_OK;
     }
-    const int whole = p.groups;
     p.part_rows = plan.part_rows;
     p.parts = plan.parts;
     p.block_channels = plan.block_channels;
     p.split = plan.split;
-    p.groups *= plan.split;
-    p.width /= plan.split;
     const dim3 grid(static_cast<unsigned>(plan.parts), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(p.n));
     const int rstep = kNormThreads / (plan.block_channels / V), smem = (plan.part_rows + rstep - 1) / rstep * kNormThreads * V * static_cast<int>(sizeof(T));
     if (int rc = set_smem<gdn_group_norm_stats_kernel<T, V>>(kNormPartBytes)) return rc;
@@ -124,10 +120,10 @@ int launch_parts(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     p.join_rows = p.part_rows;
     p.join_parts = p.parts;
     if (p.parts > kNormJoinParts || p.split > 1) {
-        p.join = p.partial + static_cast<size_t>(p.n) * p.parts * p.groups;
+        p.join = p.partial + static_cast<size_t>(p.n) * p.parts * p.groups * p.split;
         p.join_rows = p.l;
         p.join_parts = 1;
-        const long long blocks = (p.n * whole + 7) / 8;
+        const long long blocks = (p.n * p.groups + 7) / 8;
         GDN_REQUIRE(blocks < (1ll << 31), "gdn_group_norm: too many samples");
         GDN_CUDA(launch_dependent(gdn_group_norm_join_kernel, dim3(static_cast<unsigned>(blocks)), 256, 0, st, p));
     }
@@ -139,11 +135,12 @@ int launch_parts(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
     return GDN_OK;
 }
 
-// Groups that are too wide for a sweep: a CTA each in one launch where that takes it few sweeps (24 groups of 4 sweeps 9 : 18 us in pieces, of 16 24 : 17, of 64
-// 96 : 20) or where there are as many groups as CTAs fit the SMs (2500 of 16 sweeps 217 : 229, of 32 448 : 291, 4000 of 36 in pieces of 6 channels 175 : 635);
-// otherwise in pieces (one of 16384 36200 : 78, 300 of 64 163 : 71).
+// Groups that are too wide for a sweep of a CTA's threads.  A CTA each, in one launch, where that takes it few sweeps (24 groups of 4 sweeps 9 : 18 us in
+// pieces, of 16 24 : 19, of 64 96 : 20), or not many and there are as many groups as CTAs fit the SMs (2500 groups of 16 sweeps 217 : 231, 4000 of 36 174 : 411, but 2500 of 32
+// 450 : 287); otherwise in pieces (one group of 16384 sweeps 36600 : 79 us, 300 of 64 162 : 70, 3000 of 600 2980 : 1418).
 bool wide_groups(long long count, int64_t rows, int width, int vec) {
-    return rows * ((width + kNormThreads * vec - 1) / (kNormThreads * vec)) <= 12 || count >= 8 * 148;
+    const int64_t sweeps = rows * ((width + kNormThreads * vec - 1) / (kNormThreads * vec));
+    return sweeps <= 12 || (sweeps <= 64 && count >= 8 * 148);
 }
 
 template <typename T, int V>

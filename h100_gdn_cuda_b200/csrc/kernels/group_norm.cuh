@@ -26,8 +26,7 @@ struct GroupNormParams {
     // long samples: rows of a part, parts of a sample, channels of a block (whole groups); (mean, sum of squared distances) of every
     // (sample, part, group)
     int part_rows, parts, block_channels;
-    // groups of more channels than a CTA sweeps at once are `split` pieces each: `groups` and `width` are then the pieces'
-    int split;
+    int split;  // groups of more channels than a CTA sweeps at once: the pieces of one, a block each, the last one shorter (otherwise 1)
     float2* partial;
     int apply_rows;  // rows of a CTA of the second launch
     // what that one joins: `join_parts` entries of `join_rows` rows each (the parts, or one of all rows where those are many)
@@ -393,6 +392,22 @@ constexpr int kNormThreads = 256;
 constexpr int kNormMaxGroups = 64;           // groups of a block
 constexpr int kNormJoinParts = 32;           // more parts than that are joined by a launch of their own (every CTA of the second one reads all of its sample's)
 
+// The channels of block `b`, and how wide its groups are (a piece of one for a group).
+struct NormBlock {
+    int first, channels, width;
+    __device__ __forceinline__ NormBlock(const GroupNormParams& p, int b) {
+        if (p.split == 1) {
+            first = b * p.block_channels;
+            channels = min(p.block_channels, p.channels - first);
+            width = p.width;
+        } else {
+            const int at = b % p.split * p.block_channels;
+            first = b / p.split * p.width + at;
+            width = channels = min(p.block_channels, p.width - at);
+        }
+    }
+};
+
 // From the sums of a thread's V channels (rows r0, r0 + rstep, ... of the part) to sums of groups, in `out`.  Everybody calls it.
 template <int V>
 __device__ __forceinline__ void gn_group_sums(const pairs::f2* s, int vecs, int rstep, int width, int groups, float* scratch, float* out) {
@@ -429,7 +444,8 @@ __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_stats_kernel(cons
     ptx::grid_dep_wait();
     ptx::grid_dep_launch();
     const long long n = blockIdx.z, r_first = static_cast<long long>(blockIdx.x) * p.part_rows;
-    const int c_first = blockIdx.y * p.block_channels, channels = min(p.block_channels, p.channels - c_first), groups = channels / p.width;
+    const NormBlock block(p, blockIdx.y);
+    const int c_first = block.first, channels = block.channels, groups = channels / block.width;
     const int rows = static_cast<int>(min(static_cast<long long>(p.part_rows), p.l - r_first));
     const int vecs = channels / V, rstep = kNormThreads / vecs, t = threadIdx.x;
     const int vec = t % vecs, r0 = t / vecs;  // (r0 == rstep: an idle thread)
@@ -461,13 +477,13 @@ __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_stats_kernel(cons
 #pragma unroll
         for (int e = 0; e < P; ++e) s[e] = add2(s[e], v[e]);
     }
-    const float count = static_cast<float>(rows) * static_cast<float>(p.width);
-    gn_group_sums<V>(s, vecs, rstep, p.width, groups, scratch, mean);
+    const float count = static_cast<float>(rows) * static_cast<float>(block.width);
+    gn_group_sums<V>(s, vecs, rstep, block.width, groups, scratch, mean);
     f2 m[P];
 #pragma unroll
     for (int e = 0; e < P; ++e) {
         const int c = vec * V + 2 * e;
-        m[e] = pk(-mean[c / p.width] / count, V > 1 ? -mean[(c + 1) / p.width] / count : 0.f);
+        m[e] = pk(-mean[c / block.width] / count, V > 1 ? -mean[(c + 1) / block.width] / count : 0.f);
         s[e] = 0ull;
     }
 #pragma unroll 4
@@ -480,8 +496,8 @@ __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_stats_kernel(cons
             s[e] = fma2(d, d, s[e]);
         }
     }
-    gn_group_sums<V>(s, vecs, rstep, p.width, groups, scratch, sq);
-    float2* out = p.partial + (n * p.parts + blockIdx.x) * p.groups + c_first / p.width;
+    gn_group_sums<V>(s, vecs, rstep, block.width, groups, scratch, sq);
+    float2* out = p.partial + (n * p.parts + blockIdx.x) * p.groups * p.split + (p.split == 1 ? c_first / p.width : blockIdx.y);
     for (int g = t; g < groups; g += kNormThreads) out[g] = make_float2(mean[g] / count, sq[g]);
 }
 
@@ -490,10 +506,15 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
     ptx::grid_dep_wait();
     ptx::grid_dep_launch();
     const long long unit = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int whole = p.groups / p.split, entries = p.parts * p.split;
-    if (unit >= p.n * whole) return;
-    const float2* in = p.partial + unit / whole * p.parts * p.groups + unit % whole * p.split;
-    auto count = [&](int i) { return static_cast<float>(min(static_cast<long long>(p.part_rows), p.l - static_cast<long long>(i / p.split) * p.part_rows)); };
+    const int entries = p.parts * p.split;  // of a group: parts one behind the other, of pieces
+    if (unit >= p.n * p.groups) return;
+    const long long stride = static_cast<long long>(p.groups) * p.split;
+    const float2* in = p.partial + unit / p.groups * p.parts * stride + unit % p.groups * p.split;
+    auto count = [&](int i) {  // values of an entry
+        const long long rows = min(static_cast<long long>(p.part_rows), p.l - static_cast<long long>(i / p.split) * p.part_rows);
+        const int width = p.split == 1 ? p.width : min(p.block_channels, p.width - i % p.split * p.block_channels);
+        return static_cast<float>(rows) * static_cast<float>(width);
+    };
     constexpr int kMine = 8;  // entries a lane has in flight, and keeps from the means to the distances where there are no more
     const int l = threadIdx.x & 31;
     float2 mine[kMine];
@@ -502,7 +523,7 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int i = i0 + l + 32 * j;
-            mine[j] = i < entries ? __ldcg(in + static_cast<long long>(i / p.split) * p.groups + i % p.split) : make_float2(0.f, 0.f);
+            mine[j] = i < entries ? __ldcg(in + i / p.split * stride + i % p.split) : make_float2(0.f, 0.f);
         }
     };
     for (int i0 = 0; i0 < entries; i0 += 32 * kMine) {
@@ -513,14 +534,14 @@ __global__ void __launch_bounds__(256) gdn_group_norm_join_kernel(const GroupNor
     }
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    const float mu = sum / (static_cast<float>(p.l) * static_cast<float>(p.split));
+    const float mu = sum / (static_cast<float>(p.l) * static_cast<float>(p.width));
     for (int i0 = 0; i0 < entries; i0 += 32 * kMine) {
         if (entries > 32 * kMine) fetch(i0);
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             if (i0 + l + 32 * j < entries) {
                 const float d = mine[j].x - mu;
-                q += mine[j].y + count(i0 + l + 32 * j) * static_cast<float>(p.width) * d * d;
+                q += mine[j].y + count(i0 + l + 32 * j) * d * d;
             }
         }
     }
@@ -533,7 +554,8 @@ template <typename T, int V, bool kGated>
 __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(const GroupNormParams p) {
     __shared__ float mean[kNormMaxGroups], rstd[kNormMaxGroups];
     const long long n = blockIdx.z, r_first = static_cast<long long>(blockIdx.x) * p.apply_rows;
-    const int c_first = blockIdx.y * p.block_channels, channels = min(p.block_channels, p.channels - c_first), groups = channels / p.width;
+    const NormBlock block(p, blockIdx.y);
+    const int c_first = block.first, channels = block.channels, groups = channels / block.width;
     const int rows = static_cast<int>(min(static_cast<long long>(p.apply_rows), p.l - r_first));
     const int vecs = channels / V, rstep = kNormThreads / vecs, t = threadIdx.x, vec = t % vecs, r0 = t / vecs;
     ptx::grid_dep_wait();
@@ -549,7 +571,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
     }
     const int l = t & 7;
     for (int g = t >> 3; g < (groups + 31) / 32 * 32; g += kNormThreads / 8) {
-        const float2* in = p.join + n * p.join_parts * (p.groups / p.split) + (c_first / p.width + g) / p.split;
+        const float2* in = p.join + n * p.join_parts * p.groups + c_first / p.width + g;
         constexpr int kMine = kNormJoinParts / 8;
         float sum = 0.f, q = 0.f;
         auto count = [&](int i) { return static_cast<float>(min(p.join_rows, p.l - i * p.join_rows)); };
@@ -573,7 +595,7 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
         for (int m = 4; m > 0; m >>= 1) q += __shfl_xor_sync(0xffffffffu, q, m);
         if (l == 0 && g < groups) {
             mean[g] = mu;
-            rstd[g] = rsqrtf(q / (static_cast<float>(p.l) * static_cast<float>(p.width) * static_cast<float>(p.split)) + p.eps);
+            rstd[g] = rsqrtf(q / (static_cast<float>(p.l) * static_cast<float>(p.width)) + p.eps);
         }
     }
     __syncthreads();
@@ -622,8 +644,8 @@ __global__ void __launch_bounds__(kNormThreads, 3) gdn_group_norm_apply_kernel(c
     }
 }
 
-// Groups of more channels than a CTA has room for in one sweep (width > 256 V), where there are enough of them: one CTA per (sample, group), in three passes
-// over memory.
+// Groups of more channels than a CTA has room for in one sweep (width > 256 V), where they are short or as many as fit the SMs: one CTA per (sample, group), in
+// three passes over memory.
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads) gdn_group_norm_wide_kernel(const GroupNormParams p) {
     __shared__ float part[8];

@@ -7,7 +7,7 @@ import h100_gdn_cuda_b200 as gdn
 
 pytestmark = pytest.mark.gpu
 
-# one group of many rows; several; widths that split into pieces of 2, 3 and 7, into single values (a prime) and into pairs; more parts than are joined at
+# one group of many rows; several; widths whose pieces are alike and whose last one is shorter, a prime among them; more parts than are joined at
 # once; few sweeps; as many groups as CTAs fit the SMs
 SHAPES = [((1, 700, 4096), 1), ((2, 300, 2 * 2080), 2), ((3, 90, 6144), 1), ((1, 200, 1001), 1), ((1, 120, 4099), 1), ((2, 60, 2 * 5534), 2), ((1, 6000, 2050), 1),
           ((4, 2, 9000), 1), ((1, 1, 70000), 1), ((1300, 5, 2056), 1), ((1, 33, 20, 4104), 1)]
