@@ -136,8 +136,8 @@ int launch_parts(GroupNormParams p, const NormPlan& plan, cudaStream_t st) {
 }
 
 // Groups that are too wide for a sweep of a CTA's threads.  A CTA each, in one launch, where that takes it few sweeps (24 groups of 4 sweeps 9 : 18 us in
-// pieces, of 16 24 : 19, of 64 96 : 20), or not many and there are as many groups as CTAs fit the SMs (2500 groups of 16 sweeps 217 : 231, 4000 of 36 174 : 411, but 2500 of 32
-// 450 : 287); otherwise in pieces (one group of 16384 sweeps 36600 : 79 us, 300 of 64 162 : 70, 3000 of 600 2980 : 1418).
+// pieces, of 16 24 : 17, of 64 96 : 18), or not many and there are as many groups as CTAs fit the SMs (2500 groups of 16 sweeps 217 : 231, 4000 of 36 174 : 411, but 2500 of 32
+// 450 : 287); otherwise in pieces (one group of 16384 sweeps 36600 : 69 us, 300 of 64 162 : 63, 3000 of 600 2980 : 1190).
 bool wide_groups(long long count, int64_t rows, int width, int vec) {
     const int64_t sweeps = rows * ((width + kNormThreads * vec - 1) / (kNormThreads * vec));
     return sweeps <= 12 || (sweeps <= 64 && count >= 8 * 148);
@@ -163,7 +163,7 @@ int whole_bytes(int64_t rows, int width, int vec, int size, int threads) {
 // One launch that reads x once is faster than two or three that read it twice (4 x 32 groups of 16 KB 8.5 -> 2.8 us, of 64 KB 18 -> 7,
 // of 150 KB 24 -> 14), except where
 //  - very many groups are so small that the CTAs' turn-over shows (65536 groups of 2 KB, 32 a sample, 99 -> 280 us, 8 a sample 187 -> 276; with few a
-//    sample the sums of a part are long instead: 4 378 -> 275, 2 915 -> 273, 1 2555 -> 272; of few rows they are not, 4 rows of 4 x 256 channels 307 -> 496), or
+//    sample the sums of a part are long instead: 4 378 -> 275, 2 915 -> 273; of few rows they are not, 4 rows of 4 x 256 channels 307 -> 496), or
 //  - a group's piece of a row is not whole sectors of 32 bytes: copies of less than 16 bytes go through L1, of which the tile leaves little (20
 //    channels, bf16, 32 groups of 200 KB 21 -> 30 us, of 150 KB 20 -> 16), and where CTAs come in several waves, or read a gate as well, the
 //    sectors that groups share move twice (512 groups of 64 KB 33 -> 42 us, 256 of 40 KB 20 -> 14; gated, 512 of 48 KB 30 -> 42, of 16 KB 19 -> 11).

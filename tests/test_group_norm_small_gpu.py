@@ -17,7 +17,7 @@ def test_shapes(shape, G):
         check(gdn.group_norm(x, G, w, b), x, G, w, b)
 
 
-def test_not_slower_than_elementary_operations():
-    """16384 samples of 256 rows of 8 channels."""
-    x, _, w, b = make((16384, 256, 8), torch.bfloat16)
+@pytest.mark.parametrize("shape", [(16384, 256, 8), (5378, 851, 1)], ids=str)
+def test_not_slower_than_elementary_operations(shape):
+    x, _, w, b = make(shape, torch.bfloat16)
     assert timed(lambda: gdn.group_norm(x, 1, w, b)) < timed(lambda: plain(x, w, b))
